@@ -6,6 +6,7 @@ same call, same argument and metadata types, CUDA kernels behind a C ABI (``incl
 from .metadata import (EnsembleScoreStage, EvalScoreStage, HiPAttentionArgs, HiPAttentionCacheAccessStatistics,
                        HiPAttentionOutputMetadata, HiPAttentionStageInputCache, NopStage, ScanStage, Stage)
 from .operator import PhaseTimer, hip_attention_12, hip_attention_impl, read_status
+from .paged import HiPPagePool, paged_decode_attention, write_paged_kv
 from .serving import (HiPAttentionConfig, HiPAttentionPerLayerConfig, HiPMaskRefreshState, HiPMetadataCache,
                       HiPMetadataCachePool, cuda_graph_capture_configs, forward_paged_hip)
 
@@ -23,4 +24,5 @@ __all__ = [
     "Stage", "ScanStage", "ScanStage12", "NopStage", "EvalScoreStage", "EnsembleScoreStage",
     "HiPAttentionConfig", "HiPAttentionPerLayerConfig", "HiPMaskRefreshState", "HiPMetadataCache", "HiPMetadataCachePool",
     "forward_paged_hip", "cuda_graph_capture_configs",
+    "paged_decode_attention", "write_paged_kv", "HiPPagePool",
 ]

@@ -10,9 +10,10 @@ LIB_PATH = os.path.join(_PKG, "libhipattn_sm100.so")
 
 F32, F16, BF16 = 0, 1, 2
 STATUS_PAGE_RANGE, STATUS_TOKEN_RANGE, STATUS_TIMEOUT, STATUS_CHUNK_SIZE = 1, 2, 4, 8
+STATUS_NO_PAGES, STATUS_SEQUENCE = 16, 32
 MAX_CHUNKS = 16384
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024
-ABI_VERSION = 10
+ABI_VERSION = 11
 SCAN_AUTO, SCAN_STRICT, SCAN_CHECK = 0, 1, 2
 ROPE_NONE, ROPE_RELATIVE, ROPE_STREAMING = 0, 1, 2
 
@@ -55,6 +56,26 @@ class BsaParams(C.Structure):
                 ("indices_ascending", i32), ("reserved_", i32), ("indices_order", vp)]
 
 
+class PagedDecodeParams(C.Structure):
+    _fields_ = [("q", vp), ("q_stride_b", i64), ("q_stride_h", i64), ("out", vp), ("o_stride_b", i64), ("o_stride_h", i64),
+                ("lse_out", vp), ("k", Tokens), ("v", Tokens), ("rows", vp), ("status", vp), ("scratch", vp), ("scratch_bytes", i64),
+                ("dtype", i32), ("D", i32), ("B", i32), ("H", i32), ("HKV", i32), ("n_rows", i32), ("rows_is_i64", i32), ("window", i32),
+                ("sm_scale", f32), ("logit_softcap", f32)]
+
+
+class WriteKvParams(C.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("k_stride_t", i64), ("k_stride_h", i64), ("v_stride_t", i64), ("v_stride_h", i64),
+                ("k_pool", Tokens), ("v_pool", Tokens), ("rows", vp), ("offsets", vp), ("status", vp), ("N", i64),
+                ("dtype", i32), ("D", i32), ("B", i32), ("HKV", i32), ("n_rows", i32), ("rows_is_i64", i32), ("offsets_is_i64", i32),
+                ("reserved_", i32)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("ref_counts", vp), ("seq_lens", vp), ("block_table", vp), ("caches", C.POINTER(vp)), ("page_stride", i64), ("page_bytes", i64),
+                ("status", vp), ("scratch", vp), ("n_pages", i32), ("page_size", i32), ("n_sequences", i32), ("table_width", i32),
+                ("n_caches", i32), ("reserved_", i32)]
+
+
 # name -> (restype, argtypes); every symbol include/hipattn.h declares
 SYMBOLS = {
     "hipattn_scan_stage": (i32, [C.POINTER(ScanParams), vp]),
@@ -69,6 +90,14 @@ SYMBOLS = {
     "hipattn_merge_partials": (i32, [vp, vp, i64, i32, i32, i32, vp, i64, vp, vp]),
     "hipattn_mark_attention_access": (i32, [C.POINTER(BsaParams), vp, i64, i64, i32, i32, vp]),
     "hipattn_bsa_decode_noalloc": (i32, [C.POINTER(BsaParams), vp]),
+    "hipattn_paged_decode_scratch": (i64, [C.POINTER(PagedDecodeParams)]),
+    "hipattn_paged_decode": (i32, [C.POINTER(PagedDecodeParams), vp]),
+    "hipattn_write_kv": (i32, [C.POINTER(WriteKvParams), vp]),
+    "hipattn_pool_scratch": (i64, [C.POINTER(PagePool), i32]),
+    "hipattn_pool_extend": (i32, [C.POINTER(PagePool), vp, vp, i32, i32, vp]),
+    "hipattn_pool_fork": (i32, [C.POINTER(PagePool), vp, vp, i32, vp]),
+    "hipattn_pool_free": (i32, [C.POINTER(PagePool), vp, i32, vp]),
+    "hipattn_pool_compact": (i32, [C.POINTER(PagePool), vp, vp]),
     "hipattn_encode_score": (i32, [f32]),
     "hipattn_decode_score": (f32, [i32]),
     "hipattn_decode_scores": (i32, [vp, vp, i64, vp]),

@@ -1278,6 +1278,298 @@ PyObject* pool_write(PyObject* list) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// page pools: exact decode attention, new keys and values, the pages
+// ---------------------------------------------------------------------------------------------------------------------
+void on_device(const at::Tensor& t, c10::Device dev, const char* what) {
+  if (t.defined() && t.device() != dev) VALUE_ERROR("%s is on %s, the caches are on %s", what, t.device().str().c_str(), dev.str().c_str());
+}
+void need_index(const at::Tensor& t, int64_t dim, const char* what) {
+  if (!t.defined() || t.dim() != dim || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || (dim == 1 && !t.is_contiguous()))
+    VALUE_ERROR("%s must be a contiguous int32 or int64 tensor of %d dimension%s", what, (int)dim, dim == 1 ? "" : "s");
+}
+// the pair of pools [n_pages, page_size, kv_heads, head_dim] that a call reads or writes
+void kv_pools(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens, at::ScalarType elem, hipattn_tokens_t* tk,
+              hipattn_tokens_t* tv) {
+  if (!k.defined() || !v.defined()) VALUE_ERROR("k_cache and v_cache are required");
+  if (!k.is_cuda()) VALUE_ERROR("k_cache must be a CUDA tensor: there is no CPU path");
+  need_index(table, 2, "block_table");
+  need_index(lens, 1, "cache_seq_lens");
+  *tk = tokens(at::Tensor(), k, table, lens, "k");
+  *tv = tokens(at::Tensor(), v, table, lens, "v");
+  if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
+    VALUE_ERROR("k_cache %s and v_cache %s must have the same shape and type", shape_text(k).c_str(), shape_text(v).c_str());
+  on_device(v, k.device(), "v_cache");
+  on_device(table, k.device(), "block_table");
+  on_device(lens, k.device(), "cache_seq_lens");
+  if (lens.size(0) != table.size(0)) VALUE_ERROR("block_table has %lld rows, cache_seq_lens %lld", (long long)table.size(0), (long long)lens.size(0));
+  if (dtype_of(elem) < 0) VALUE_ERROR("the element type must be float32, float16 or bfloat16");
+  if (is_fp8(k.scalar_type())) {
+    if (elem == at::kFloat) NOT_BUILT("an fp8 cache needs float16 or bfloat16 tokens");
+  } else if (k.scalar_type() != elem) {
+    VALUE_ERROR("the caches must have the element type of the other tensors, or be fp8 (float8_e5m2 or its uint8 view)");
+  }
+}
+
+// paged_decode(q, k_cache, v_cache, block_table, cache_seq_lens, rows, sm_scale, sliding_window, logit_softcap, return_lse, out)
+PyObject* paged_decode(PyObject* const* argv) {
+  const at::Tensor q = tensor_of(argv[0], "q"), k = tensor_of(argv[1], "k_cache"), v = tensor_of(argv[2], "v_cache"),
+                   table = tensor_of(argv[3], "block_table"), lens = tensor_of(argv[4], "cache_seq_lens"), rows = tensor_of(argv[5], "rows");
+  at::Tensor out = tensor_of(argv[10], "out");
+  if (!q.defined() || q.dim() != 3) VALUE_ERROR("q must be [batch, heads, head_dim]: one new token per sequence");
+  hipattn_paged_decode_params_t p;
+  memset(&p, 0, sizeof(p));
+  kv_pools(k, v, table, lens, q.scalar_type(), &p.k, &p.v);
+  const c10::Device dev = k.device();
+  on_device(q, dev, "q");
+  if (q.stride(2) != 1) VALUE_ERROR("q must have a contiguous last dim");
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), HKV = k.size(2);
+  if (k.size(3) != D) VALUE_ERROR("q %s and the caches %s differ in head_dim", shape_text(q).c_str(), shape_text(k).c_str());
+  if (HKV < 1 || H % HKV) VALUE_ERROR("%lld heads are not a multiple of %lld KV heads", (long long)H, (long long)HKV);
+  if (rows.defined()) {
+    need_index(rows, 1, "rows");
+    on_device(rows, dev, "rows");
+    if (rows.size(0) != B) VALUE_ERROR("rows names %lld sequences, q has %lld tokens", (long long)rows.size(0), (long long)B);
+  } else if (table.size(0) != B) {
+    VALUE_ERROR("q has %lld tokens, block_table %lld rows: give `rows` to attend some of them", (long long)B, (long long)table.size(0));
+  }
+  const double scale = PyFloat_AsDouble(argv[6]);
+  if (scale == -1.0 && PyErr_Occurred()) throw PyError{};
+  int64_t window = 0;
+  if (argv[7] != Py_None) {
+    window = as_int(Ref::borrow(argv[7]));
+    if (window < 1) VALUE_ERROR("sliding_window must be positive, or None");
+    if (window > 0x7fffffff) window = 0;
+  }
+  double cap = 0;
+  if (argv[8] != Py_None) {
+    cap = PyFloat_AsDouble(argv[8]);
+    if (cap == -1.0 && PyErr_Occurred()) throw PyError{};
+    if (!(cap >= 0)) VALUE_ERROR("logit_softcap must not be negative");
+  }
+  const int return_lse = PyObject_IsTrue(argv[9]);
+  if (return_lse < 0) throw PyError{};
+  const c10::cuda::CUDAGuard guard(dev);
+  const Device mem{dev};
+  if (out.defined()) {
+    on_device(out, dev, "out");
+    if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || out.stride(2) != 1)
+      VALUE_ERROR("out must be %s of q's type with a contiguous last dim", shape_text(q).c_str());
+  } else {
+    out = mem.empty(q.sizes(), q.scalar_type());
+  }
+  at::Tensor lse = return_lse ? mem.empty({B, H}, at::kFloat) : at::Tensor();
+  const at::Tensor status = status_word(dev.index());
+  p.q = q.data_ptr();
+  p.q_stride_b = q.stride(0);
+  p.q_stride_h = q.stride(1);
+  p.out = out.data_ptr();
+  p.o_stride_b = out.stride(0);
+  p.o_stride_h = out.stride(1);
+  p.lse_out = lse.defined() ? lse.data_ptr<float>() : nullptr;
+  p.rows = rows.defined() ? rows.data_ptr() : nullptr;
+  p.rows_is_i64 = rows.defined() && rows.scalar_type() == at::kLong;
+  p.status = (uint32_t*)status.data_ptr();
+  p.dtype = dtype_of(q.scalar_type());
+  p.D = (int32_t)D;
+  p.B = (int32_t)B;
+  p.H = (int32_t)H;
+  p.HKV = (int32_t)HKV;
+  p.n_rows = (int32_t)table.size(0);
+  p.window = (int32_t)window;
+  p.sm_scale = (float)scale;
+  p.logit_softcap = (float)cap;
+  if (B > 0) {
+    at::Tensor scratch;
+    if (const int64_t bytes = hipattn_paged_decode_scratch(&p)) {
+      scratch = mem.empty({bytes}, at::kByte);
+      p.scratch = scratch.data_ptr();
+      p.scratch_bytes = bytes;
+    }
+    check(hipattn_paged_decode(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "paged_decode_attention");
+  }
+  if (!return_lse) return wrap(out);
+  Ref o = checked(wrap(out)), l = checked(wrap(lse));
+  return PyTuple_Pack(2, o.get(), l.get());
+}
+
+// write_kv(k, v, k_cache, v_cache, block_table, cache_seq_lens, rows, token_offsets)
+PyObject* write_kv(PyObject* const* argv) {
+  const at::Tensor k = tensor_of(argv[0], "k"), v = tensor_of(argv[1], "v"), kc = tensor_of(argv[2], "k_cache"), vc = tensor_of(argv[3], "v_cache"),
+                   table = tensor_of(argv[4], "block_table"), lens = tensor_of(argv[5], "cache_seq_lens"), rows = tensor_of(argv[6], "rows"),
+                   offsets = tensor_of(argv[7], "token_offsets");
+  if (!k.defined() || !v.defined() || k.dim() != 3 || v.dim() != 3 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
+    VALUE_ERROR("k and v must be [tokens, kv_heads, head_dim] of one shape and type");
+  hipattn_write_kv_params_t p;
+  memset(&p, 0, sizeof(p));
+  kv_pools(kc, vc, table, lens, k.scalar_type(), &p.k_pool, &p.v_pool);
+  const c10::Device dev = kc.device();
+  on_device(k, dev, "k");
+  on_device(v, dev, "v");
+  if (k.stride(2) != 1 || v.stride(2) != 1) VALUE_ERROR("k and v must have a contiguous last dim");
+  if (k.size(1) != kc.size(2) || k.size(2) != kc.size(3))
+    VALUE_ERROR("k %s and the caches %s differ in kv_heads or head_dim", shape_text(k).c_str(), shape_text(kc).c_str());
+  int64_t B = table.size(0);
+  if (rows.defined()) {
+    need_index(rows, 1, "rows");
+    on_device(rows, dev, "rows");
+    B = rows.size(0);
+  }
+  if (offsets.defined()) {
+    need_index(offsets, 1, "token_offsets");
+    on_device(offsets, dev, "token_offsets");
+    if (offsets.size(0) != B + 1) VALUE_ERROR("token_offsets has %lld entries, %lld sequences need %lld", (long long)offsets.size(0), (long long)B, (long long)B + 1);
+  } else if (B < 1 ? k.size(0) > 0 : k.size(0) % B != 0) {
+    VALUE_ERROR("%lld tokens are not a multiple of %lld sequences: give `token_offsets`", (long long)k.size(0), (long long)B);
+  }
+  if (k.size(0) == 0 || B == 0) Py_RETURN_NONE;
+  const c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor status = status_word(dev.index());
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.k_stride_t = k.stride(0);
+  p.k_stride_h = k.stride(1);
+  p.v_stride_t = v.stride(0);
+  p.v_stride_h = v.stride(1);
+  p.rows = rows.defined() ? rows.data_ptr() : nullptr;
+  p.rows_is_i64 = rows.defined() && rows.scalar_type() == at::kLong;
+  p.offsets = offsets.defined() ? offsets.data_ptr() : nullptr;
+  p.offsets_is_i64 = offsets.defined() && offsets.scalar_type() == at::kLong;
+  p.status = (uint32_t*)status.data_ptr();
+  p.N = k.size(0);
+  p.dtype = dtype_of(k.scalar_type());
+  p.D = (int32_t)k.size(2);
+  p.B = (int32_t)B;
+  p.HKV = (int32_t)k.size(1);
+  p.n_rows = (int32_t)table.size(0);
+  check(hipattn_write_kv(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream()), "write_paged_kv");
+  Py_RETURN_NONE;
+}
+
+// What a HiPPagePool holds on the device: its tables and the caches of all layers
+struct PoolHandle {
+  std::vector<at::Tensor> keep;
+  std::vector<void*> caches;
+  hipattn_page_pool_t pool{};
+  c10::Device dev{at::kCUDA, 0};
+};
+const char* kPoolName = "hip_attention_b200.page_pool";
+void drop_pool(PyObject* o) { delete (PoolHandle*)PyCapsule_GetPointer(o, kPoolName); }
+PoolHandle* pool_of(PyObject* o) {
+  PoolHandle* h = (PoolHandle*)PyCapsule_GetPointer(o, kPoolName);
+  if (!h) throw PyError{};
+  return h;
+}
+// page_pool([caches], ref_counts, seq_lens, block_table) -> handle
+PyObject* page_pool(PyObject* const* argv) {
+  std::unique_ptr<PoolHandle> h(new PoolHandle);
+  const Py_ssize_t n = PyList_GET_SIZE(argv[0]);
+  if (n < 1 || n > HIPATTN_POOL_MAX_CACHES) VALUE_ERROR("a pool has 1 to %d caches, %lld were given", HIPATTN_POOL_MAX_CACHES, (long long)n);
+  at::Tensor first;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor c = tensor_of(PyList_GET_ITEM(argv[0], i), "cache");
+    if (!c.defined() || c.dim() != 4) VALUE_ERROR("caches must be [n_pages, page_size, kv_heads, head_dim]");
+    if (!first.defined()) first = c;
+    if (!c.is_cuda()) VALUE_ERROR("the caches must be CUDA tensors: there is no CPU path");
+    if (c.sizes() != first.sizes() || c.scalar_type() != first.scalar_type() || c.strides() != first.strides() || c.device() != first.device())
+      VALUE_ERROR("the caches of a pool must have one shape, type, layout and device");
+    if (dtype_of(c.scalar_type()) < 0 && !is_fp8(c.scalar_type())) VALUE_ERROR("caches must be float32, float16, bfloat16 or float8_e5m2 (or its uint8 view)");
+    if (c.numel() == 0) VALUE_ERROR("caches %s have no elements", shape_text(c).c_str());
+    if (c.stride(3) != 1 || c.stride(2) != c.size(3) || (c.size(1) > 1 && c.stride(1) != c.size(2) * c.size(3)))
+      VALUE_ERROR("the tokens of a page must be contiguous (the pages may lie anywhere)");
+    if (c.size(0) > 1 && c.stride(0) < c.size(1) * c.size(2) * c.size(3)) VALUE_ERROR("pages overlap");
+    h->keep.push_back(c);
+    h->caches.push_back(c.data_ptr());
+  }
+  const at::Tensor refs = tensor_of(argv[1], "ref_counts"), lens = tensor_of(argv[2], "seq_lens"), table = tensor_of(argv[3], "block_table");
+  h->dev = first.device();
+  const int64_t eb = first.element_size();
+  hipattn_page_pool_t& p = h->pool;
+  p.ref_counts = refs.data_ptr<int32_t>();
+  p.seq_lens = lens.data_ptr<int32_t>();
+  p.block_table = table.data_ptr<int32_t>();
+  p.page_bytes = first.size(1) * first.size(2) * first.size(3) * eb;
+  p.page_stride = first.size(0) > 1 ? first.stride(0) * eb : p.page_bytes;
+  p.n_pages = (int32_t)first.size(0);
+  p.page_size = (int32_t)first.size(1);
+  p.n_sequences = (int32_t)lens.size(0);
+  p.table_width = (int32_t)table.size(1);
+  p.n_caches = (int32_t)n;
+  p.caches = h->caches.data();
+  if (first.size(2) * first.size(3) * eb % 16) VALUE_ERROR("a token of %lld bytes: a multiple of 16 is needed", (long long)(first.size(2) * first.size(3) * eb));
+  if (p.page_stride % 16) VALUE_ERROR("pages must start on 16-byte boundaries");
+  for (void* c : h->caches)
+    if ((uintptr_t)c % 16) VALUE_ERROR("caches must start on 16-byte boundaries");
+  h->keep.push_back(refs);
+  h->keep.push_back(lens);
+  h->keep.push_back(table);
+  p.status = (uint32_t*)status_word(h->dev.index()).data_ptr();
+  PyObject* o = PyCapsule_New(h.get(), kPoolName, drop_pool);
+  if (o) h.release();
+  return o;
+}
+// entries of a pool call as int32 on the pool's device
+at::Tensor entries(PyObject* o, const PoolHandle* h, const char* what) {
+  at::Tensor t = tensor_of(o, what);
+  need_index(t, 1, what);
+  if (t.device() != h->dev) VALUE_ERROR("%s is on %s, the pool is on %s", what, t.device().str().c_str(), h->dev.str().c_str());
+  if (t.size(0) > HIPATTN_POOL_MAX_ENTRIES) VALUE_ERROR("%s names %lld sequences, a call takes %d", what, (long long)t.size(0), HIPATTN_POOL_MAX_ENTRIES);
+  return t.scalar_type() == at::kInt ? t : t.clamp(-1, 0x7fffffff).to(at::kInt);   // (what does not fit is beyond any table)
+}
+// pool_extend(handle, rows, n_tokens: tensor or int)
+PyObject* pool_extend(PyObject* const* argv) {
+  PoolHandle* h = pool_of(argv[0]);
+  const c10::cuda::CUDAGuard guard(h->dev);
+  const at::Tensor rows = entries(argv[1], h, "rows");
+  at::Tensor tokens;
+  int64_t every = 0;
+  if (THPVariable_Check(argv[2])) {
+    tokens = entries(argv[2], h, "n_tokens");
+    if (tokens.size(0) != rows.size(0)) VALUE_ERROR("%lld rows, but n_tokens has %lld entries", (long long)rows.size(0), (long long)tokens.size(0));
+  } else {
+    every = as_int(Ref::borrow(argv[2]));
+    if (every < 0 || every > 0x7fffffff) VALUE_ERROR("n_tokens %lld must not be negative, nor beyond 2^31", (long long)every);
+  }
+  if (rows.size(0) == 0) Py_RETURN_NONE;
+  check(hipattn_pool_extend(&h->pool, rows.data_ptr<int32_t>(), tokens.defined() ? tokens.data_ptr<int32_t>() : nullptr, (int32_t)every, (int32_t)rows.size(0),
+                            c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "extend");
+  Py_RETURN_NONE;
+}
+// pool_fork(handle, parents, children)
+PyObject* pool_fork(PyObject* const* argv) {
+  PoolHandle* h = pool_of(argv[0]);
+  const c10::cuda::CUDAGuard guard(h->dev);
+  const at::Tensor parents = entries(argv[1], h, "parents"), children = entries(argv[2], h, "children");
+  if (parents.size(0) != children.size(0)) VALUE_ERROR("%lld parents, but %lld children", (long long)parents.size(0), (long long)children.size(0));
+  const int n = (int)parents.size(0);
+  if (n == 0) Py_RETURN_NONE;
+  hipattn_page_pool_t p = h->pool;
+  const at::Tensor scratch = Device{h->dev}.empty({hipattn_pool_scratch(&p, n)}, at::kByte);
+  p.scratch = scratch.data_ptr();
+  check(hipattn_pool_fork(&p, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), n, c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "fork");
+  Py_RETURN_NONE;
+}
+// pool_free(handle, rows)
+PyObject* pool_free(PyObject* const* argv) {
+  PoolHandle* h = pool_of(argv[0]);
+  const c10::cuda::CUDAGuard guard(h->dev);
+  const at::Tensor rows = entries(argv[1], h, "rows");
+  if (rows.size(0) == 0) Py_RETURN_NONE;
+  check(hipattn_pool_free(&h->pool, rows.data_ptr<int32_t>(), (int)rows.size(0), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "free");
+  Py_RETURN_NONE;
+}
+// pool_compact(handle) -> pages in use, int32 [1]
+PyObject* pool_compact(PyObject* const* argv) {
+  PoolHandle* h = pool_of(argv[0]);
+  const c10::cuda::CUDAGuard guard(h->dev);
+  const Device mem{h->dev};
+  hipattn_page_pool_t p = h->pool;
+  const at::Tensor scratch = mem.empty({hipattn_pool_scratch(&p, 0)}, at::kByte), in_use = mem.empty({1}, at::kInt);
+  p.scratch = scratch.data_ptr();
+  check(hipattn_pool_compact(&p, in_use.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "compact");
+  return wrap(in_use);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // module
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename F>
@@ -1432,6 +1724,15 @@ PyObject* py_bind(PyObject*, PyObject* const* argv, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+template <PyObject* (*F)(PyObject* const*), int ARGS>
+PyObject* py_call(PyObject*, PyObject* const* argv, Py_ssize_t n) {
+  if (n != ARGS) {
+    PyErr_Format(PyExc_TypeError, "%d arguments are taken, %zd were given", ARGS, n);
+    return nullptr;
+  }
+  return guarded([&] { return F(argv); });
+}
+
 PyMethodDef methods[] = {
     {"forward", (PyCFunction)(void*)py_forward, METH_FASTCALL, "q, k, v, args, cached_metadata, return_lse, debug, score_reduce, timer, v_ready, shared, out, lse, fork, beside"},
     {"gather_table", (PyCFunction)(void*)py_gather_table, METH_FASTCALL, "table, rows, lens -> rows of the table, or None when it does not take them"},
@@ -1442,6 +1743,13 @@ PyMethodDef methods[] = {
     {"status_word", py_status_word, METH_O, "device index -> int32 tensor [1]"},
     {"pool_read", py_pool_read, METH_O, "[(buffer, rows), ...] -> list of tensors"},
     {"pool_write", py_pool_write, METH_O, "[(buffer, value or None, rows), ...]"},
+    {"paged_decode", (PyCFunction)(void*)py_call<paged_decode, 11>, METH_FASTCALL, "q, k_cache, v_cache, block_table, cache_seq_lens, rows, sm_scale, sliding_window, logit_softcap, return_lse, out"},
+    {"write_kv", (PyCFunction)(void*)py_call<write_kv, 8>, METH_FASTCALL, "k, v, k_cache, v_cache, block_table, cache_seq_lens, rows, token_offsets"},
+    {"page_pool", (PyCFunction)(void*)py_call<page_pool, 4>, METH_FASTCALL, "[caches], ref_counts, seq_lens, block_table -> handle"},
+    {"pool_extend", (PyCFunction)(void*)py_call<pool_extend, 3>, METH_FASTCALL, "handle, rows, n_tokens"},
+    {"pool_fork", (PyCFunction)(void*)py_call<pool_fork, 3>, METH_FASTCALL, "handle, parents, children"},
+    {"pool_free", (PyCFunction)(void*)py_call<pool_free, 2>, METH_FASTCALL, "handle, rows"},
+    {"pool_compact", (PyCFunction)(void*)py_call<pool_compact, 1>, METH_FASTCALL, "handle -> pages in use"},
     {"bind", (PyCFunction)(void*)py_bind, METH_FASTCALL, "classes of the package"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of hip_attention_12.", -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,634 @@
+// The pages of a pool: writing new keys and values into them, dealing them out, sharing, freeing and moving them.
+//
+// Which pages are free is read off the reference counts themselves: there is no list beside them that could disagree, and
+// "the lowest free pages in the order of the entries" does not depend on how threads are scheduled.  A call is planned by one
+// cluster (the counts are cut into a slice for each of its CTAs, whose sums are exchanged through distributed shared memory), which
+// also changes the tables; pages are copied by a second launch over the whole GPU that the plan is handed to in device memory.
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace hipattn {
+namespace {
+
+constexpr int kSMs = 148;
+constexpr int kPlanCtas = 8;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kMaxCachesPerLaunch = 128;
+
+struct Pool {
+  int32_t* refs;
+  int32_t* lens;
+  int32_t* table;
+  uint32_t* status;
+  int n_pages, page_size, n_seqs, width;
+};
+struct CacheList {
+  char* at[kMaxCachesPerLaunch];
+  int n;
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return (int)r;
+}
+__device__ __forceinline__ int ld_cluster_int(const int* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];\n" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// Sums over the threads of a CTA: those before this thread (returned) and all (`all`).  s: kPlanWarps words.
+template <typename N>
+__device__ __forceinline__ N scan_block(N x, N* s, N& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  N sum = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const N y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = sum;
+  __syncthreads();
+  N w = lane < kPlanWarps ? s[lane] : 0, ws = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const N y = __shfl_up_sync(0xffffffffu, ws, o);
+    if (lane >= o) ws += y;
+  }
+  all = __shfl_sync(0xffffffffu, ws, 31);
+  return sum - x + __shfl_sync(0xffffffffu, ws - w, warp);
+}
+
+// Pages [begin, end) of a CTA's slice
+struct Slice {
+  int begin, end;
+};
+__device__ __forceinline__ Slice slice_of(int n, int rank) {
+  const int per = (int)(((int64_t)n + kPlanCtas - 1) / kPlanCtas);
+  Slice s;
+  s.begin = (int)min((int64_t)n, (int64_t)per * rank);
+  s.end = (int)min((int64_t)n, (int64_t)per * (rank + 1));
+  return s;
+}
+// live pages of [begin, end)
+__device__ __forceinline__ int count_live(const int32_t* refs, int begin, int end) {
+  int n = 0;
+  for (int i = begin + (int)threadIdx.x; i < end; i += kPlanThreads) n += refs[i] > 0;
+  return n;
+}
+
+// ---------------------------------------------------------------------------------------------------
+// extend and fork
+// ---------------------------------------------------------------------------------------------------
+// A copied page: source, destination, tokens
+struct PageCopy {
+  int src, dst, tokens;
+};
+
+// extend: a[i] = row, b[i] (b null: every) = tokens that it grows by.  fork: a[i] = parent, b[i] = child.
+// plan (fork): [0] = number of copies, then PageCopy[].
+template <bool FORK>
+__global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
+    deal_pages_kernel(const Pool pool, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int every, int n, int32_t* plan) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  int* s_row = reinterpret_cast<int*>(smem);        // row that gets pages, -1: none
+  int* s_had = s_row + n;                           // pages that it has (fork: full pages of the parent)
+  int* s_new = s_had + n;                           // its new length
+  int* s_before = s_new + n;                        // pages that the entries before it get
+  uint32_t* s_named = reinterpret_cast<uint32_t*>(s_before + n);   // rows that the call names
+  __shared__ long long s_scan64[kPlanWarps];
+  __shared__ int s_scan[kPlanWarps];
+  __shared__ int s_free, s_longest;
+  const int tid = threadIdx.x, rank = cluster_rank(), P = pool.page_size;
+  if (FORK) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  for (int i = tid; i < (pool.n_seqs + 31) / 32; i += kPlanThreads) s_named[i] = 0;
+  if (tid == 0) s_longest = 0;
+  __syncthreads();
+  // ---- the entries: every CTA goes through all of them ----
+  bool bad = false;
+  long long mine = 0;
+  const int per = (n + kPlanThreads - 1) / kPlanThreads;   // consecutive entries of a thread
+  for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
+    const int x = a[i], y = b ? b[i] : every, row = FORK ? y : x;
+    int had = 0, len = 0, need = 0, at = -1;
+    if (x >= 0 && row >= 0) {
+      if (x >= pool.n_seqs || row >= pool.n_seqs || (!FORK && y < 0) || (atomicOr(&s_named[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u)) {
+        bad = true;
+      } else {
+        const int old = pool.lens[x];
+        const long long now = FORK ? old : (long long)old + y;
+        if (old < 0 || now > 0x7fff0000LL || (now + P - 1) / P > pool.width || (FORK && pool.lens[row] != 0)) {
+          bad = true;
+        } else {
+          len = (int)now;
+          had = FORK ? len / P : (old + P - 1) / P;
+          need = (len + P - 1) / P - had;
+          at = row;
+          if (FORK) atomicMax(&s_longest, had);
+        }
+      }
+    }
+    s_row[i] = at;
+    s_had[i] = had;
+    s_new[i] = len;
+    s_before[i] = need;
+    mine += need;
+  }
+  long long total;
+  long long before = scan_block(mine, s_scan64, total);
+  for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
+    const int need = s_before[i];
+    s_before[i] = (int)min(before, (long long)0x7fffffff);
+    before += need;
+  }
+  bad = __syncthreads_or(bad);
+
+  // ---- free pages before this CTA's slice, and in all ----
+  const Slice sl = slice_of(pool.n_pages, rank);
+  int live;
+  scan_block(count_live(pool.refs, sl.begin, sl.end), s_scan, live);
+  if (tid == 0) s_free = sl.end - sl.begin - live;
+  cluster_sync();
+  int base = 0;
+  long long free_pages = 0;
+  for (int r = 0; r < kPlanCtas; ++r) {
+    const int f = ld_cluster_int(&s_free, r);
+    if (r < rank) base += f;
+    free_pages += f;
+  }
+  cluster_sync();   // (everybody has read the lengths and the sums: from here on they may change, and CTAs may leave)
+  if (bad || total > free_pages) {
+    if (rank == 0 && tid == 0) {
+      atomicOr(pool.status, bad ? HIPATTN_STATUS_SEQUENCE : HIPATTN_STATUS_NO_PAGES);
+      if (FORK) plan[0] = 0;
+    }
+    return;
+  }
+
+  // ---- deal out the free pages of the slice ----
+  for (int i0 = sl.begin; i0 < sl.end && base < total; i0 += kPlanThreads) {
+    const int page = i0 + tid;
+    const int is_free = page < sl.end && pool.refs[page] <= 0;
+    int all;
+    const int nth = base + scan_block(is_free, s_scan, all);
+    base += all;
+    if (is_free && nth < total) {
+      int lo = 0, hi = n - 1;                // the last entry that begins at or before nth
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_before[mid] <= nth) lo = mid;
+        else hi = mid - 1;
+      }
+      pool.refs[page] = 1;
+      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + (nth - s_before[lo])] = page;
+      if (FORK) {
+        int src = pool.table[(int64_t)a[lo] * pool.width + s_had[lo]];
+        int tokens = s_new[lo] - s_had[lo] * P;
+        if (src < 0 || src >= pool.n_pages) {
+          atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+          src = page;
+          tokens = 0;
+        }
+        reinterpret_cast<PageCopy*>(plan + 1)[nth] = PageCopy{src, page, tokens};
+      }
+    }
+  }
+  if (FORK) {
+    // ---- full pages are shared: 128 entries of a table at a time ----
+    const int warp = tid >> 5, lane = tid & 31, chunks = (s_longest + 127) / 128;
+    for (int64_t it = rank * kPlanWarps + warp; it < (int64_t)chunks * n; it += kPlanCtas * kPlanWarps) {
+      const int i = (int)(it % n), j0 = (int)(it / n) * 128 + lane;
+      if (s_row[i] < 0) continue;
+      const int32_t* from = pool.table + (int64_t)a[i] * pool.width;
+      int32_t* to = pool.table + (int64_t)s_row[i] * pool.width;
+      int page[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) page[k] = j0 + k * 32 < s_had[i] ? from[j0 + k * 32] : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (j0 + k * 32 < s_had[i]) {
+          to[j0 + k * 32] = page[k];
+          if (page[k] >= 0 && page[k] < pool.n_pages) atomicAdd(pool.refs + page[k], 1);
+          else atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+        }
+      }
+    }
+  }
+  if (rank == 0) {
+    for (int i = tid; i < n; i += kPlanThreads)
+      if (s_row[i] >= 0) pool.lens[s_row[i]] = s_new[i];
+    if (FORK && tid == 0) plan[0] = (int)total;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// copies of pages
+// ---------------------------------------------------------------------------------------------------
+constexpr int kCopyThreads = 256;
+constexpr int kCopyBytes = 16384;     // of a page, to a CTA at a time: four 16-byte pieces a thread in flight
+
+__device__ __forceinline__ void copy_piece(const char* src, char* dst, int64_t bytes) {
+  uint4 v[kCopyBytes / 16 / kCopyThreads];
+#pragma unroll
+  for (int k = 0; k < kCopyBytes / 16 / kCopyThreads; ++k) {
+    const int o = (k * kCopyThreads + threadIdx.x) * 16;
+    if (o < bytes) v[k] = *reinterpret_cast<const uint4*>(src + o);
+  }
+#pragma unroll
+  for (int k = 0; k < kCopyBytes / 16 / kCopyThreads; ++k) {
+    const int o = (k * kCopyThreads + threadIdx.x) * 16;
+    if (o < bytes) *reinterpret_cast<uint4*>(dst + o) = v[k];
+  }
+}
+
+// The begun pages of a fork
+__global__ void __launch_bounds__(kCopyThreads) copy_begun_pages_kernel(const CacheList caches, const int32_t* plan, int64_t page_stride, int64_t token_bytes,
+                                                                        int pieces) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int count = plan[0];
+  const PageCopy* copies = reinterpret_cast<const PageCopy*>(plan + 1);
+  for (int64_t it = blockIdx.x; it < (int64_t)count * caches.n * pieces; it += gridDim.x) {
+    const int piece = (int)(it % pieces);
+    const int cache = (int)(it / pieces % caches.n);
+    const PageCopy c = copies[it / pieces / caches.n];
+    const int64_t at = (int64_t)piece * kCopyBytes, bytes = c.tokens * token_bytes - at;
+    if (bytes > 0) copy_piece(caches.at[cache] + c.src * page_stride + at, caches.at[cache] + c.dst * page_stride + at, bytes);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// free
+// ---------------------------------------------------------------------------------------------------
+// One cluster per row.  Its first CTA takes the length and leaves 0, so that a row that is named twice is freed once.
+__global__ void __launch_bounds__(256) free_rows_kernel(const Pool pool, const int32_t* __restrict__ rows, int ctas) {
+  __shared__ int s_len;
+  const int rank = ctas > 1 ? cluster_rank() : 0;
+  const int row = rows[blockIdx.x / ctas];
+  const bool there = row >= 0 && row < pool.n_seqs;
+  if (threadIdx.x == 0 && rank == 0) {
+    s_len = there ? atomicExch(pool.lens + row, 0) : 0;
+    if (row >= pool.n_seqs) atomicOr(pool.status, HIPATTN_STATUS_SEQUENCE);
+  }
+  int len;
+  if (ctas > 1) {
+    cluster_sync();
+    len = ld_cluster_int(&s_len, 0);
+    cluster_sync();
+  } else {
+    __syncthreads();
+    len = s_len;
+  }
+  const int64_t pages = min(((int64_t)max(len, 0) + pool.page_size - 1) / pool.page_size, (int64_t)pool.width);
+  for (int64_t i = (int64_t)rank * 256 + threadIdx.x; i < pages; i += 256 * ctas) {
+    const int page = pool.table[(int64_t)row * pool.width + i];
+    if (page < 0 || page >= pool.n_pages) atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+    else atomicSub(pool.refs + page, 1);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// compact
+// ---------------------------------------------------------------------------------------------------
+// plan: [0] = pages that move, [1] = pages in use, then holes [half], movers [half], nth [n_pages] (which mover a page is)
+struct CompactPlan {
+  int32_t *count, *holes, *movers, *nth;
+};
+__host__ __device__ __forceinline__ int64_t half_of(int64_t n) { return n / 2 + 1; }
+__host__ __device__ __forceinline__ CompactPlan compact_plan(int32_t* scratch, int n_pages) {
+  CompactPlan c;
+  c.count = scratch;
+  c.holes = scratch + 2;
+  c.movers = c.holes + half_of(n_pages);
+  c.nth = c.movers + half_of(n_pages);
+  return c;
+}
+
+__global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Pool pool, int32_t* scratch, int32_t* in_use) {
+  __shared__ int s_scan[kPlanWarps];
+  __shared__ int s_live, s_below;
+  const int tid = threadIdx.x, rank = cluster_rank();
+  const CompactPlan plan = compact_plan(scratch, pool.n_pages);
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  const Slice sl = slice_of(pool.n_pages, rank);
+  int live;
+  scan_block(count_live(pool.refs, sl.begin, sl.end), s_scan, live);
+  if (tid == 0) s_live = live;
+  cluster_sync();
+  int base = 0, m = 0;               // pages in use before the slice, and in all
+  for (int r = 0; r < kPlanCtas; ++r) {
+    const int f = ld_cluster_int(&s_live, r);
+    if (r < rank) base += f;
+    m += f;
+  }
+  int below = live;                  // of them, numbered below m
+  if (sl.begin >= m) below = 0;
+  else if (sl.end > m) scan_block(count_live(pool.refs, sl.begin, m), s_scan, below);
+  if (tid == 0) s_below = below;
+  cluster_sync();
+  int stay = 0;
+  for (int r = 0; r < kPlanCtas; ++r) stay += ld_cluster_int(&s_below, r);
+  cluster_sync();
+  if (rank == 0 && tid == 0) {
+    plan.count[0] = m - stay;
+    plan.count[1] = m;
+    if (in_use) *in_use = m;
+  }
+  if (stay == m) return;
+  for (int i0 = sl.begin; i0 < sl.end; i0 += kPlanThreads) {
+    const int page = i0 + tid;
+    const int is_live = page < sl.end && pool.refs[page] > 0;
+    int all;
+    const int lower = base + scan_block(is_live, s_scan, all);   // pages in use below this one
+    base += all;
+    if (page < sl.end) {
+      if (!is_live && page < m) plan.holes[page - lower] = page;
+      if (is_live && page >= m) {
+        plan.movers[lower - stay] = page;
+        plan.nth[page] = lower - stay;
+      }
+    }
+  }
+}
+
+// Pages, counts and (first launch) tables
+__global__ void __launch_bounds__(kCopyThreads) move_pages_kernel(const Pool pool, const CacheList caches, int32_t* scratch, int64_t page_stride, int64_t page_bytes,
+                                                                  int pieces, int tables) {
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const CompactPlan plan = compact_plan(scratch, pool.n_pages);
+  const int moves = plan.count[0], m = plan.count[1];
+  if (moves == 0) return;
+  if (tables) {
+    const int64_t thread = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x, threads = (int64_t)gridDim.x * kCopyThreads;
+    for (int64_t i = thread; i < moves; i += threads) {
+      pool.refs[plan.holes[i]] = pool.refs[plan.movers[i]];
+      pool.refs[plan.movers[i]] = 0;
+    }
+    // a warp takes 32 entries of a row
+    const int chunks = (pool.width + 31) / 32, lane = threadIdx.x & 31;
+    for (int64_t it = thread >> 5; it < (int64_t)pool.n_seqs * chunks; it += threads >> 5) {
+      const int row = (int)(it / chunks), j = (int)(it % chunks) * 32 + lane;
+      const int64_t pages = ((int64_t)max(pool.lens[row], 0) + pool.page_size - 1) / pool.page_size;
+      if (j >= pool.width || j >= pages) continue;
+      int32_t* e = pool.table + (int64_t)row * pool.width + j;
+      const int page = *e;
+      if (page < 0 || page >= pool.n_pages) {
+        atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+      } else if (page >= m) {
+        // (a table that names a page which the counts call free: the list of the movers does not have it)
+        const int k = plan.nth[page];
+        if (k >= 0 && k < moves && plan.movers[k] == page) *e = plan.holes[k];
+        else atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+      }
+    }
+  }
+  for (int64_t it = blockIdx.x; it < (int64_t)moves * caches.n * pieces; it += gridDim.x) {
+    const int piece = (int)(it % pieces);
+    const int cache = (int)(it / pieces % caches.n);
+    const int64_t i = it / pieces / caches.n, at = (int64_t)piece * kCopyBytes;
+    copy_piece(caches.at[cache] + plan.movers[i] * page_stride + at, caches.at[cache] + plan.holes[i] * page_stride + at, page_bytes - at);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// new keys and values
+// ---------------------------------------------------------------------------------------------------
+// Eight elements of a row to a thread
+template <int DT>
+__device__ __forceinline__ uint2 narrow_e5m2(const uint4& w) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+  uint32_t o[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint16_t h = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+    float f;
+    if (DT == HIPATTN_BF16) f = __uint_as_float((uint32_t)h << 16);
+    else f = __half2float(__ushort_as_half(h));
+    o[i >> 2] |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_NOSAT, __NV_E5M2) << (8 * (i & 3));
+  }
+  return make_uint2(o[0], o[1]);
+}
+
+template <int DT, bool F8>
+__global__ void __launch_bounds__(256) write_kv_kernel(const hipattn_write_kv_params_t p) {
+  constexpr int EB = Elem<DT>::bytes, VEC = 16 / EB, CB = F8 ? 1 : EB;
+  const int row_pieces = p.D / VEC, pieces = p.HKV * row_pieces;       // of a token, keys or values
+  const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t tok = it / (2 * pieces);
+  if (tok >= p.N) return;
+  const int which = (int)(it % (2 * pieces)) / pieces, pc = (int)(it % pieces), h = pc / row_pieces, d = pc % row_pieces * VEC;
+  const hipattn_tokens_t& pool = which ? p.v_pool : p.k_pool;
+  const char* src = which ? (const char*)p.v + (tok * p.v_stride_t + (int64_t)h * p.v_stride_h + d) * EB
+                          : (const char*)p.k + (tok * p.k_stride_t + (int64_t)h * p.k_stride_h + d) * EB;
+  const uint4 x = *reinterpret_cast<const uint4*>(src);
+  auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldg((const long long*)q + i) : (int64_t)__ldg((const int*)q + i); };
+  // the token's sequence and place in it
+  int64_t first, count;
+  int b;
+  if (p.offsets) {
+    int lo = 0, hi = p.B;                  // the first b with tok < offsets[b + 1]
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (index(p.offsets, p.offsets_is_i64, mid + 1) <= tok) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo == p.B) return;                 // behind the last sequence
+    b = lo;
+    first = index(p.offsets, p.offsets_is_i64, b);
+    count = index(p.offsets, p.offsets_is_i64, b + 1) - first;
+    if (tok < first) return;               // before the first
+  } else {
+    count = p.N / p.B;
+    b = (int)(tok / count);
+    first = b * count;
+  }
+  const int64_t row = p.rows ? index(p.rows, p.rows_is_i64, b) : b;
+  if (row < 0) return;
+  if (row >= p.n_rows) {
+    atomicOr(p.status, HIPATTN_STATUS_SEQUENCE);
+    return;
+  }
+  const int64_t t = index(pool.cache_seq_lens, pool.seq_lens_is_i64, row) - count + (tok - first);
+  if (t < 0 || t >= (int64_t)pool.table_width * pool.page_size) {
+    atomicOr(p.status, HIPATTN_STATUS_TOKEN_RANGE);
+    return;
+  }
+  const int64_t page = index(pool.block_table, pool.table_is_i64, row * pool.table_stride_b + t / pool.page_size);
+  if (page < 0 || page >= pool.n_pages) {
+    atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
+    return;
+  }
+  char* dst = (char*)pool.cache + (page * pool.stride_page + t % pool.page_size * pool.stride_off + (int64_t)h * pool.stride_ch + d) * CB;
+  if constexpr (F8) *reinterpret_cast<uint2*>(dst) = narrow_e5m2<DT>(x);
+  else *reinterpret_cast<uint4*>(dst) = x;
+}
+
+int validate_pool(const hipattn_page_pool_t* p, const char* what, bool caches) {
+  HIPATTN_REQUIRE(p != nullptr, HIPATTN_ERR_INVALID, "%s: the pool is null", what);
+  HIPATTN_REQUIRE(p->ref_counts && p->seq_lens && p->block_table && p->status, HIPATTN_ERR_INVALID, "%s: ref_counts, seq_lens, block_table and status are required", what);
+  HIPATTN_REQUIRE(p->n_pages > 0 && p->page_size > 0 && p->n_sequences > 0 && p->table_width > 0, HIPATTN_ERR_INVALID,
+                  "%s: n_pages %d, page_size %d, n_sequences %d, table_width %d must be positive", what, p->n_pages, p->page_size, p->n_sequences, p->table_width);
+  HIPATTN_REQUIRE(p->n_pages <= 0x7fff0000 && p->n_sequences <= HIPATTN_POOL_MAX_SEQUENCES, HIPATTN_ERR_UNSUPPORTED, "%s: %d pages, %d sequences are too many",
+                  what, p->n_pages, p->n_sequences);
+  if (!caches) return HIPATTN_OK;
+  HIPATTN_REQUIRE(p->caches && p->n_caches > 0 && p->n_caches <= HIPATTN_POOL_MAX_CACHES, HIPATTN_ERR_INVALID, "%s: %d caches outside [1, %d]", what, p->n_caches,
+                  HIPATTN_POOL_MAX_CACHES);
+  HIPATTN_REQUIRE(p->page_bytes > 0 && p->page_bytes % ((int64_t)p->page_size * 16) == 0 && p->page_stride >= p->page_bytes && p->page_stride % 16 == 0,
+                  HIPATTN_ERR_INVALID, "%s: pages of %lld bytes, %lld apart: tokens must be multiples of 16 bytes", what, (long long)p->page_bytes, (long long)p->page_stride);
+  for (int i = 0; i < p->n_caches; ++i)
+    HIPATTN_REQUIRE(p->caches[i] && (uintptr_t)p->caches[i] % 16 == 0, HIPATTN_ERR_INVALID, "%s: cache %d is null or not 16-byte aligned", what, i);
+  return HIPATTN_OK;
+}
+Pool device_pool(const hipattn_page_pool_t& p) {
+  return Pool{p.ref_counts, p.seq_lens, p.block_table, p.status, p.n_pages, p.page_size, p.n_sequences, p.table_width};
+}
+
+template <bool FORK>
+int deal_pages(const hipattn_page_pool_t& p, const int32_t* a, const int32_t* b, int every, int n, int32_t* plan, cudaStream_t stream, const char* what) {
+  HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "%s: %d entries outside [1, %d]", what, n, HIPATTN_POOL_MAX_ENTRIES);
+  HIPATTN_REQUIRE(a && (b || !FORK), HIPATTN_ERR_INVALID, "%s: null pointer", what);
+  const size_t smem = 4 * sizeof(int) * (size_t)n + sizeof(uint32_t) * (size_t)((p.n_sequences + 31) / 32);
+  HIPATTN_CUDA_OK(allow_smem((const void*)deal_pages_kernel<FORK>, smem));
+  deal_pages_kernel<FORK><<<kPlanCtas, kPlanThreads, smem, stream>>>(device_pool(p), a, b, every, n, plan);
+  return check_launch("deal_pages_kernel");
+}
+
+// a launch that may begin while the one before it, which it waits for, is still running
+struct AfterPlan {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  AfterPlan(int64_t grid, int threads, cudaStream_t stream) {
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = stream;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+  }
+};
+int64_t copy_grid(int64_t items) {
+  const int64_t most = kSMs * 8;
+  return items < 1 ? 1 : (items < most ? items : most);
+}
+
+}  // namespace
+}  // namespace hipattn
+
+using namespace hipattn;
+
+extern "C" int64_t hipattn_pool_scratch(const hipattn_page_pool_t* p, int32_t n) {
+  if (p == nullptr || n < 0) return 0;
+  if (n > 0) return 16 + (int64_t)n * (int64_t)sizeof(PageCopy);
+  return (2 + 2 * half_of(p->n_pages) + (int64_t)p->n_pages) * 4;
+}
+
+extern "C" int hipattn_pool_extend(const hipattn_page_pool_t* p, const int32_t* rows, const int32_t* n_tokens, int32_t every, int32_t n, void* stream) {
+  const int rc = validate_pool(p, "pool_extend", false);
+  return rc ? rc : deal_pages<false>(*p, rows, n_tokens, every, n, nullptr, (cudaStream_t)stream, "pool_extend");
+}
+
+extern "C" int hipattn_pool_fork(const hipattn_page_pool_t* p, const int32_t* parents, const int32_t* children, int32_t n, void* stream) {
+  int rc = validate_pool(p, "pool_fork", true);
+  if (rc) return rc;
+  HIPATTN_REQUIRE(p->scratch != nullptr, HIPATTN_ERR_INVALID, "pool_fork: scratch is null");
+  rc = deal_pages<true>(*p, parents, children, 0, n, (int32_t*)p->scratch, (cudaStream_t)stream, "pool_fork");
+  if (rc) return rc;
+  const int pieces = (int)((p->page_bytes + kCopyBytes - 1) / kCopyBytes);
+  for (int c0 = 0; c0 < p->n_caches; c0 += kMaxCachesPerLaunch) {
+    CacheList list;
+    list.n = p->n_caches - c0 < kMaxCachesPerLaunch ? p->n_caches - c0 : kMaxCachesPerLaunch;
+    for (int i = 0; i < list.n; ++i) list.at[i] = (char*)p->caches[c0 + i];
+    AfterPlan launch(copy_grid((int64_t)n * list.n * pieces), kCopyThreads, (cudaStream_t)stream);
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, copy_begun_pages_kernel, list, (const int32_t*)p->scratch, p->page_stride, p->page_bytes / p->page_size, pieces));
+    rc = check_launch("copy_begun_pages_kernel");
+    if (rc) return rc;
+  }
+  return HIPATTN_OK;
+}
+
+extern "C" int hipattn_pool_free(const hipattn_page_pool_t* p, const int32_t* rows, int32_t n, void* stream) {
+  const int rc = validate_pool(p, "pool_free", false);
+  if (rc) return rc;
+  HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "pool_free: %d entries outside [1, %d]", n, HIPATTN_POOL_MAX_ENTRIES);
+  HIPATTN_REQUIRE(rows != nullptr, HIPATTN_ERR_INVALID, "pool_free: null pointer");
+  const int ctas = p->table_width > 1024 ? 8 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n * ctas));
+  cfg.blockDim = dim3(256);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)ctas;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, free_rows_kernel, device_pool(*p), rows, ctas));
+  return check_launch("free_rows_kernel");
+}
+
+extern "C" int hipattn_pool_compact(const hipattn_page_pool_t* p, int32_t* pages_in_use, void* stream) {
+  int rc = validate_pool(p, "pool_compact", true);
+  if (rc) return rc;
+  HIPATTN_REQUIRE(p->scratch != nullptr, HIPATTN_ERR_INVALID, "pool_compact: scratch is null");
+  plan_compact_kernel<<<kPlanCtas, kPlanThreads, 0, (cudaStream_t)stream>>>(device_pool(*p), (int32_t*)p->scratch, pages_in_use);
+  rc = check_launch("plan_compact_kernel");
+  if (rc) return rc;
+  const int pieces = (int)((p->page_bytes + kCopyBytes - 1) / kCopyBytes);
+  for (int c0 = 0; c0 < p->n_caches; c0 += kMaxCachesPerLaunch) {
+    CacheList list;
+    list.n = p->n_caches - c0 < kMaxCachesPerLaunch ? p->n_caches - c0 : kMaxCachesPerLaunch;
+    for (int i = 0; i < list.n; ++i) list.at[i] = (char*)p->caches[c0 + i];
+    AfterPlan launch(copy_grid((int64_t)half_of(p->n_pages) * list.n * pieces + (int64_t)p->n_sequences * ((p->table_width + 31) / 32) / 8), kCopyThreads, (cudaStream_t)stream);
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, move_pages_kernel, device_pool(*p), list, (int32_t*)p->scratch, p->page_stride, p->page_bytes, pieces, c0 == 0 ? 1 : 0));
+    rc = check_launch("move_pages_kernel");
+    if (rc) return rc;
+  }
+  return HIPATTN_OK;
+}
+
+extern "C" int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream) {
+  HIPATTN_REQUIRE(p != nullptr, HIPATTN_ERR_INVALID, "write_kv: params are null");
+  HIPATTN_REQUIRE(p->k && p->v && p->status, HIPATTN_ERR_INVALID, "write_kv: k, v and status are required");
+  HIPATTN_REQUIRE(p->N > 0 && p->B > 0 && p->HKV > 0 && p->D > 0 && p->n_rows > 0, HIPATTN_ERR_INVALID, "write_kv: bad shape N=%lld B=%d HKV=%d D=%d rows=%d",
+                  (long long)p->N, p->B, p->HKV, p->D, p->n_rows);
+  HIPATTN_REQUIRE(p->offsets || p->N % p->B == 0, HIPATTN_ERR_INVALID, "write_kv: %lld tokens are not a multiple of %d sequences", (long long)p->N, p->B);
+  HIPATTN_REQUIRE(p->rows || p->n_rows >= p->B, HIPATTN_ERR_INVALID, "write_kv: %d entries, but a table of %d rows", p->B, p->n_rows);
+  HIPATTN_REQUIRE(p->k_pool.cache && p->v_pool.cache, HIPATTN_ERR_INVALID, "write_kv: k and v must go to page pools");
+  HIPATTN_REQUIRE(p->k_pool.n_pages == p->v_pool.n_pages && p->k_pool.page_size == p->v_pool.page_size && p->k_pool.fp8_e5m2 == p->v_pool.fp8_e5m2,
+                  HIPATTN_ERR_INVALID, "write_kv: k and v must go to pools of the same pages and type");
+  const int eb = p->dtype == HIPATTN_F32 ? 4 : 2;
+  const int64_t ra = 16 / eb;
+  int rc = validate_tokens(p->k_pool, eb, p->D, "k");
+  if (rc) return rc;
+  rc = validate_tokens(p->v_pool, eb, p->D, "v");
+  if (rc) return rc;
+  HIPATTN_REQUIRE((uintptr_t)p->k % 16 == 0 && (uintptr_t)p->v % 16 == 0 && p->k_stride_t % ra == 0 && p->k_stride_h % ra == 0 && p->v_stride_t % ra == 0 &&
+                      p->v_stride_h % ra == 0,
+                  HIPATTN_ERR_INVALID, "write_kv: rows of k and v must start on 16-byte boundaries");
+  const int64_t blocks = (p->N * 2 * p->HKV * (p->D / ra) + 255) / 256;
+  HIPATTN_REQUIRE(blocks < 0x7fffffffLL, HIPATTN_ERR_INVALID, "write_kv: grid of %lld blocks", (long long)blocks);
+  const cudaStream_t s = (cudaStream_t)stream;
+  switch (p->dtype) {
+    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, 256, 0, s>>>(*p); break;
+    case HIPATTN_F16:
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      break;
+    case HIPATTN_BF16:
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      break;
+    default: set_error("write_kv: unknown dtype %d", p->dtype); return HIPATTN_ERR_INVALID;
+  }
+  return check_launch("write_kv_kernel");
+}

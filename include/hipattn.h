@@ -34,6 +34,8 @@ extern "C" {
 #define HIPATTN_STATUS_TOKEN_RANGE 2u /* a token index fell outside [0, T); clamped                 */
 #define HIPATTN_STATUS_CHUNK_SIZE 8u  /* a chunk was longer than the chunk size the scan was told; its tail was ignored */
 #define HIPATTN_STATUS_TIMEOUT 4u     /* a bounded on-chip wait ran out; the launch's output is invalid */
+#define HIPATTN_STATUS_NO_PAGES 16u   /* a page pool had too few free pages for a call, which changed nothing */
+#define HIPATTN_STATUS_SEQUENCE 32u   /* a call named a sequence that it cannot take (outside the table, twice, not empty, too long) */
 
 #define HIPATTN_SCORE_INIT (-32000.0f) /* attention_extend.py:2040-2045 */
 #define HIPATTN_INDEX_PAD INT64_MAX    /* attention_extend.py:2913 */
@@ -305,6 +307,93 @@ int hipattn_merge_partials(const float* part_o, const float* part_lse, int64_t r
  */
 #define HIPATTN_NOALLOC_SCRATCH_BYTES (16 * 1024 * 1024)
 int hipattn_bsa_decode_noalloc(const hipattn_bsa_params_t* p, void* stream);
+
+/*
+ * Exact attention of one new token per sequence over a page pool, for layers that are not sparse.
+ * The reference hands such layers to another attention backend (hip_config.py:97-102: decode_always_dense, force_dense).
+ *
+ * Entry b attends positions [max(0, n - window), n) of sequence r = rows[b] (b when rows is null), n = cache_seq_lens[r],
+ * read through block_table[r]; logits are sm_scale * q.k, soft-capped when logit_softcap > 0.  out [B, H, D] in the element
+ * type; lse_out (optional) [B, H] receives the base-2 log-sum-exp.  An entry with nothing to attend (n <= 0, or rows[b] < 0: a
+ * padded batch) gets zeros and -inf.  k and v are page pools of the same number and size of pages with the same table;
+ * k.block_table is [n_rows, table_width].  A length beyond table_width * page_size is cut there
+ * (HIPATTN_STATUS_TOKEN_RANGE), a row beyond the table is empty (HIPATTN_STATUS_SEQUENCE).
+ */
+typedef struct hipattn_paged_decode_params {
+  const void* q;             /* [B, H, D] */
+  int64_t q_stride_b, q_stride_h;
+  void* out;                 /* [B, H, D] */
+  int64_t o_stride_b, o_stride_h;
+  float* lse_out;            /* [B, H], contiguous, optional */
+  hipattn_tokens_t k, v;
+  const void* rows;          /* [B], int32 or int64, optional */
+  uint32_t* status;
+  void* scratch;             /* hipattn_paged_decode_scratch bytes, 16-byte aligned; not shared by calls that may overlap */
+  int64_t scratch_bytes;
+  int32_t dtype, D, B, H, HKV, n_rows;
+  int32_t rows_is_i64;
+  int32_t window;            /* 0: all positions */
+  float sm_scale, logit_softcap;
+} hipattn_paged_decode_params_t;
+
+int64_t hipattn_paged_decode_scratch(const hipattn_paged_decode_params_t* p);  /* reads shapes only; 0: none needed */
+int hipattn_paged_decode(const hipattn_paged_decode_params_t* p, void* stream);
+
+/*
+ * Writes new keys and values into their pages (the set_kv_buffer of a server's token pool; any page size, fp8 pools included).
+ * Tokens offsets[b] .. offsets[b + 1] of k / v [N, HKV, D] (offsets null: N / B tokens each) are the last ones of sequence
+ * rows[b] (b when rows is null; negative: none), whose length cache_seq_lens[.] includes them.  Values go to an fp8 pool
+ * rounded to the nearest e5m2 (ties to even, beyond its range to infinity).  Tokens at negative positions, beyond the table or
+ * on pages outside the pool are not written (HIPATTN_STATUS_TOKEN_RANGE / _PAGE_RANGE / _SEQUENCE).  The sequences of a call
+ * must be different ones.
+ */
+typedef struct hipattn_write_kv_params {
+  const void *k, *v;         /* [N, HKV, D] */
+  int64_t k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  hipattn_tokens_t k_pool, v_pool;
+  const void* rows;
+  const void* offsets;       /* [B + 1], optional */
+  uint32_t* status;
+  int64_t N;
+  int32_t dtype, D, B, HKV, n_rows;
+  int32_t rows_is_i64, offsets_is_i64;
+  int32_t reserved_;
+} hipattn_write_kv_params_t;
+int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream);
+
+/*
+ * The pages of a pool: which sequence reads which page, and how many do.  All state is on the device and every call is
+ * stream-ordered; calls on one pool must be ordered by the caller.  A call that cannot be carried out as a whole changes nothing
+ * and sets HIPATTN_STATUS_NO_PAGES or _SEQUENCE.  Pages are dealt out lowest number first, in the order of a call's entries, so a
+ * call's result does not depend on how it is scheduled.  Entries that are negative are left out.  At most
+ * HIPATTN_POOL_MAX_ENTRIES entries a call.
+ */
+#define HIPATTN_POOL_MAX_CACHES 512
+#define HIPATTN_POOL_MAX_ENTRIES 4096
+#define HIPATTN_POOL_MAX_SEQUENCES 262144
+typedef struct hipattn_page_pool {
+  int32_t* ref_counts;       /* [n_pages]: sequences that read a page, 0 = free */
+  int32_t* seq_lens;         /* [n_sequences] */
+  int32_t* block_table;      /* [n_sequences, table_width], contiguous */
+  void* const* caches;       /* n_caches device pointers, in host memory: K and V pools of all layers */
+  int64_t page_stride;       /* bytes between the pages of a cache */
+  int64_t page_bytes;        /* contiguous bytes of a page, a multiple of page_size * 16 */
+  uint32_t* status;
+  void* scratch;             /* hipattn_pool_scratch bytes (fork: of n entries; compact: n = 0) */
+  int32_t n_pages, page_size, n_sequences, table_width, n_caches;
+  int32_t reserved_;
+} hipattn_page_pool_t;
+int64_t hipattn_pool_scratch(const hipattn_page_pool_t* pool, int32_t n);
+/* rows[i] grows by n_tokens[i] (>= 0; n_tokens null: by `every`) tokens and gets the pages they need. */
+int hipattn_pool_extend(const hipattn_page_pool_t* pool, const int32_t* rows, const int32_t* n_tokens, int32_t every, int32_t n, void* stream);
+/* children[i], an empty sequence, becomes a copy of parents[i]: full pages are shared, the tokens of a begun page are copied to a
+ * page of the child's own in all caches. */
+int hipattn_pool_fork(const hipattn_page_pool_t* pool, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
+/* The sequences become empty; pages that no other sequence reads are free again.  A row named twice is freed once. */
+int hipattn_pool_free(const hipattn_page_pool_t* pool, const int32_t* rows, int32_t n, void* stream);
+/* Moves the pages in use to the front: with m pages in use, those numbered m and more go, ascending, to the free ones below m,
+ * in all caches, and the tables follow.  *pages_in_use (optional, device) receives m. */
+int hipattn_pool_compact(const hipattn_page_pool_t* pool, int32_t* pages_in_use, void* stream);
 
 /* Order-preserving image of an fp32 score: a < b  <=>  encode(a) < encode(b) as signed integers
  * (host helpers; across GPUs the head max is an int32 MAX all-reduce of score_max). */
