@@ -1,17 +1,21 @@
 // Exact attention of one new token per sequence over a page pool: o = sum_t softmax(scale q.k_t) v_t over all (or the last
-// `window`) tokens of the sequence.
+// `window`) tokens of the sequence.  Bound: HBM (every attended K and V row is read once, 4 D flop a head and key).
 //
 // Work is a row of rounds: for every sequence, for every unit of it (a KV head and a tile of its query heads), ROUND keys at a
 // time.  The host does not know the lengths, so every CTA adds them up itself and takes its share of the row, as many rounds
 // as any other, whatever the lengths are.  A unit that lies in one CTA's share is finished there; the parts of one that does not go
 // to scratch (numerators, maximum, denominator) and the merge kernel joins them in order.
-#include "common.cuh"
+//
+// A warp takes KEYS keys at a time from a ring of its own in shared memory, filled with 16-byte asynchronous copies, and keeps
+// its own running maximum, sum and output: nothing in the loop waits for another warp.  paged_decode_mma_kernel: 16-bit and fp8
+// rows; paged_decode_fma_kernel: fp32.
+#include "mma_common.cuh"
 
 namespace hipattn {
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -76,36 +80,6 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int ctas, int least) 
   return s < least ? least : s;
 }
 
-template <int DT>
-__device__ __forceinline__ void widen16(const uint4& w, float* out) {
-  if constexpr (DT == HIPATTN_F32) {
-    out[0] = __uint_as_float(w.x); out[1] = __uint_as_float(w.y); out[2] = __uint_as_float(w.z); out[3] = __uint_as_float(w.w);
-  } else {
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == HIPATTN_BF16) {
-        out[2 * i] = __uint_as_float(v[i] << 16);
-        out[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
-        out[2 * i] = f.x;
-        out[2 * i + 1] = f.y;
-      }
-    }
-  }
-}
-// sixteen bytes of a cache row as floats
-template <int DT, bool F8>
-__device__ __forceinline__ void widen_row(const uint4& w, float* out) {
-  if constexpr (F8) {
-    widen16<HIPATTN_F16>(widen_fp8_e5m2<HIPATTN_F16>(make_uint2(w.x, w.y)), out);
-    widen16<HIPATTN_F16>(widen_fp8_e5m2<HIPATTN_F16>(make_uint2(w.z, w.w)), out + 8);
-  } else {
-    widen16<DT>(w, out);
-  }
-}
-
 // element e of the output row of head h, from the joined maximum (base 2), numerator and denominator
 template <int DT>
 __device__ __forceinline__ void finish(const Params& p, int b, int h, int e, float M, float num, float den) {
@@ -115,288 +89,584 @@ __device__ __forceinline__ void finish(const Params& p, int b, int h, int e, flo
   if (e == 0 && p.lse_out) p.lse_out[(int64_t)b * p.H + h] = none ? -INFINITY : (M > -INFINITY ? M : 0.f) + log2f(den);
 }
 
-// Geometry of the kernel: RB = bytes of a row of DP elements, KEYS = keys a warp takes at once, STAGES = depth of its ring
+// Geometry of the kernels: RB = bytes of a row of DP elements, KEYS = keys a warp takes at once, STAGES = depth of its ring
 template <int DT, bool F8, int DP>
 struct Geo {
   static constexpr int EB = F8 ? 1 : Elem<DT>::bytes;
   static constexpr int RB = DP * EB;
-  static constexpr int VEC = 16 / EB;
   static constexpr int NPC = RB / 16;                         // pieces of a row
-  static constexpr int KEYS = 4096 / RB > 32 ? 32 : 4096 / RB;
-  static constexpr int LPK = 32 / KEYS;                       // lanes of a key in the logits
+  static constexpr int FIT = 4096 / RB > 32 ? 32 : 4096 / RB;
+  static constexpr int KEYS = DT != HIPATTN_F32 && FIT < 16 ? 16 : FIT;
   static constexpr int STAGES = 3;
   static constexpr int ROUND = KEYS * kWarps;
   static constexpr int STAGE_BYTES = 2 * KEYS * RB;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES * kWarps;
-  static constexpr int PPL = NPC > 32 ? NPC / 32 : 1;         // pieces of a V row that a lane owns
-  static constexpr int KP = NPC < 32 ? 32 / NPC : 1;          // V rows that a warp reads at once
+  static constexpr int CTAS = RING_BYTES <= 100 * 1024 ? 2 : 1;   // per multiprocessor
+};
+template <int DP>
+struct FmaGeo : Geo<HIPATTN_F32, false, DP> {
+  using B = Geo<HIPATTN_F32, false, DP>;
+  static constexpr int LPK = 32 / B::KEYS;                          // lanes of a key in the logits
+  static constexpr int PPL = B::NPC > 32 ? B::NPC / 32 : 1;         // pieces of a V row that a lane owns
+  static constexpr int KP = B::NPC < 32 ? 32 / B::NPC : 1;          // V rows that a warp reads at once
 };
 
-// Byte offset of piece `pc` of row `key`: the lanes of a quarter warp, LPK to a row, reach eight different bank groups.
-template <int RB, int LPK>
-__device__ __forceinline__ int place(int key, int pc) {
-  return key * RB + ((pc ^ ((key * LPK) & 7 & (RB / 16 - 1))) << 4);
-}
-
-// GT: query heads of a unit.  One warp: KEYS keys at a time from a ring of its own, its own running maximum, sum and output.
-template <int DT, bool F8, int DP, int GT>
-__global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const Params p, int tiles, int split, int least) {
-  using G = Geo<DT, F8, DP>;
-  using T = typename Elem<DT>::type;
-  constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, VEC = G::VEC, MS = DP + 2;
-  extern __shared__ __align__(128) unsigned char smem[];
-  unsigned char* ring = smem + (threadIdx.x >> 5) * (G::STAGES * G::STAGE_BYTES);
-  float* s_merge = reinterpret_cast<float*>(smem);                   // [kWarps][GT][MS], over the rings when they are empty
-  float* s_q = reinterpret_cast<float*>(smem + G::RING_BYTES);       // [GT][DP]
+// A CTA's share of the row of rounds
+struct Share {
+  int64_t first, last, unit_at;   // [first, last): what is left of it; where sequence b begins in the row
+  int b;
+};
+// false: the share is empty.  All threads.
+__device__ __forceinline__ bool find_share(const Params& p, int units, int round, int least, Share& sh) {
   __shared__ int64_t s_scan[kWarps];
   __shared__ int64_t s_found[2];
-
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int heads = p.H / p.HKV, units = p.HKV * tiles;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");   // (the merge waits for the whole of this grid)
-
-  // ---- this CTA's share of the rounds ----
-  int b = 0;
-  int64_t first = 0, last = 0, unit_at = 0;     // [first, last): what is left of the share; where sequence b begins in the row
-  if (split) {
-    int64_t total = 0, base = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-      // pass 0: the total; pass 1: the sequence that the share begins in.  (One sequence per thread: the second pass reads
-      // nothing again.)
-      const int64_t share = pass ? share_of(total * units, gridDim.x, least) : 0;
-      first = share * blockIdx.x;
-      if (pass && first >= total * units) return;
-      base = 0;
-      for (int c = 0; c < p.B; c += kThreads) {
-        const int i = c + tid;
-        int64_t x = i < p.B ? rounds_of(sequence_of(p, i, false), G::ROUND) : 0, sum = x;
+  int64_t total = 0;
+  // pass 0: the total; pass 1: the sequence that the share begins in
+  for (int pass = 0; pass < 2; ++pass) {
+    const int64_t share = pass ? share_of(total * units, gridDim.x, least) : 0;
+    sh.first = share * blockIdx.x;
+    if (pass && sh.first >= total * units) return false;
+    int64_t base = 0;
+    for (int c = 0; c < p.B; c += kThreads) {
+      const int i = c + tid;
+      const int64_t x = i < p.B ? rounds_of(sequence_of(p, i, false), round) : 0;
+      int64_t sum = x;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += y;
-        }
-        if (lane == 31) s_scan[warp] = sum;
-        __syncthreads();
-        int64_t all = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          if (w < warp) sum += s_scan[w];
-          all += s_scan[w];
-        }
-        if (pass) {
-          const int64_t end = (base + sum) * units;
-          if (first < end && first >= end - x * units) {
-            s_found[0] = i;
-            s_found[1] = end - x * units;
-          }
-        }
-        base += all;
-        __syncthreads();
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
       }
-      total = base;
-      if (pass) last = min(first + share, total * units);
+      if (lane == 31) s_scan[warp] = sum;
+      __syncthreads();
+      int64_t all = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) sum += s_scan[w];
+        all += s_scan[w];
+      }
+      if (pass) {
+        const int64_t end = (base + sum) * units;
+        if (sh.first < end && sh.first >= end - x * units) {
+          s_found[0] = i;
+          s_found[1] = end - x * units;
+        }
+      }
+      base += all;
+      __syncthreads();
     }
-    b = (int)s_found[0];
-    unit_at = s_found[1];
-  } else {
-    b = blockIdx.x / units;
+    total = base;
+    if (pass) sh.last = min(sh.first + share, total * units);
   }
-  const int64_t share_first = first;
+  sh.b = (int)s_found[0];
+  sh.unit_at = s_found[1];
+  return true;
+}
 
-  const int page_size = p.k.page_size;
-  const int page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
-  const int npc = p.D * G::EB / 16;         // pieces of a row that exist
-  const float cap = p.logit_softcap, scale = p.sm_scale;
-
-  for (;;) {
-    const Sequence seq = sequence_of(p, b, tid == 0);
-    const int rounds = rounds_of(seq, G::ROUND);
-    int u0 = 0, r0 = 0;
-    if (split) {
-      u0 = (int)((first - unit_at) / rounds);
-      r0 = (int)((first - unit_at) % rounds);
+// The rounds [r0, r1) of one unit that a CTA works on next
+struct Segment {
+  Sequence seq;
+  int rounds, r0, r1, hkv, h0, live_heads;
+};
+__device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, int tiles, int units, int split, int round, int gt) {
+  Segment g;
+  g.seq = sequence_of(p, sh.b, threadIdx.x == 0);
+  g.rounds = rounds_of(g.seq, round);
+  int u = blockIdx.x % units;
+  g.r0 = 0;
+  g.r1 = g.rounds;
+  if (split) {
+    u = (int)((sh.first - sh.unit_at) / g.rounds);
+    g.r0 = (int)((sh.first - sh.unit_at) % g.rounds);
+    g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
+  }
+  const int heads = p.H / p.HKV, tile = u % tiles;
+  g.hkv = u / tiles;
+  g.h0 = g.hkv * heads + tile * gt;
+  g.live_heads = min(gt, heads - tile * gt);
+  return g;
+}
+// The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 2]: to the output, or to scratch.  Returns whether more is to come.
+template <int DT, int DP, int GT>
+__device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, Share& sh, int64_t share_first, int units, int split, const float* s_merge) {
+  constexpr int MS = DP + 2;
+  const bool whole = g.r0 == 0 && g.r1 == g.rounds;
+  float* part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * MS;
+  for (int i = threadIdx.x; i < g.live_heads * p.D; i += kThreads) {
+    const int h = i / p.D, e = i % p.D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_merge[(w * GT + h) * MS + DP]);
+    const float base = M > -INFINITY ? M : 0.f;
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(s_merge[(w * GT + h) * MS + DP] - base);
+      num += f * s_merge[(w * GT + h) * MS + e];
+      den += f * s_merge[(w * GT + h) * MS + DP + 1];
+    }
+    if (whole) {
+      finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
     } else {
-      u0 = blockIdx.x % units;
+      part[h * MS + e] = num;
+      if (e == 0) {
+        part[h * MS + DP] = M;
+        part[h * MS + DP + 1] = den;
+      }
     }
-    const int r1 = split ? (int)min((int64_t)rounds, r0 + (last - first)) : rounds;
-    const int hkv = u0 / tiles, tile = u0 % tiles, h0 = hkv * heads + tile * GT, live_heads = min(GT, heads - tile * GT);
+  }
+  if (!split) return false;
+  sh.first += g.r1 - g.r0;
+  if (sh.first >= sh.last) return false;
+  if (sh.first == sh.unit_at + (int64_t)g.rounds * units) {
+    sh.unit_at = sh.first;
+    ++sh.b;
+  }
+  return true;
+}
 
-    // ---- the unit's queries ----
-    __syncthreads();
-    for (int i = tid; i < GT * DP; i += kThreads) {
-      const int g = i / DP, e = i % DP;
-      float x = 0.f;
-      if (g < live_heads && e < p.D) x = Elem<DT>::to_f32(reinterpret_cast<const T*>(p.q)[(int64_t)b * p.q_stride_b + (int64_t)(h0 + g) * p.q_stride_h + e]);
-      s_q[i] = x;
-    }
-    __syncthreads();
-
-    float m_run[GT], l_run[GT], acc[GT][G::PPL][VEC];
-#pragma unroll
-    for (int g = 0; g < GT; ++g) {
-      m_run[g] = -INFINITY;
-      l_run[g] = 0.f;
-#pragma unroll
-      for (int i = 0; i < G::PPL; ++i)
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[g][i][e] = 0.f;
-    }
-    const char* kb = (const char*)p.k.cache + (int64_t)hkv * p.k.stride_ch * G::EB;
-    const char* vb = (const char*)p.v.cache + (int64_t)hkv * p.v.stride_ch * G::EB;
-
-    // positions of round r: seq.lo + r * ROUND + warp * KEYS ..; lane `key` resolves a key's page one round ahead
-    int64_t page = 0;
-    auto fetch_page = [&](int r) {
-      const int t = seq.lo + r * G::ROUND + warp * KEYS + lane;
-      page = 0;
-      if (r < r1 && lane < KEYS && t < seq.hi)
-        page = load_index(p.k.block_table, p.k.table_is_i64, seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
-    };
-    auto copy = [&](int r, int slot) {
-      const int t0 = seq.lo + r * G::ROUND + warp * KEYS;
+// Asynchronous copies of a warp's keys into its ring.  Lane `key` looks up a key's page one round ahead of its copies and shares
+// out where its rows begin; a row that is not attended is sixteen zero bytes a piece (what lies there may be anything, NaN too).
+template <class G, class Place>
+struct Feeder {
+  const Params& p;
+  const Segment& g;
+  const char *kb, *vb;        // the KV head's rows, this lane's piece
+  int64_t page = 0;
+  int page_size, page_shift, warp, lane, npc;
+  bool same;                  // K and V pools are laid out alike
+  __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_) : p(p_), g(g_), warp(warp_), lane(lane_) {
+    page_size = p.k.page_size;
+    page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
+    npc = p.D * G::EB / 16;
+    kb = (const char*)p.k.cache + (int64_t)g.hkv * p.k.stride_ch * G::EB;
+    vb = (const char*)p.v.cache + (int64_t)g.hkv * p.v.stride_ch * G::EB;
+    same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
+  }
+  __device__ __forceinline__ void fetch_page(int r) {
+    const int t = g.seq.lo + r * G::ROUND + warp * G::KEYS + lane;
+    page = 0;
+    if (r < g.r1 && lane < G::KEYS && t < g.seq.hi)
+      page = load_index(p.k.block_table, p.k.table_is_i64, g.seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
+  }
+  __device__ __forceinline__ void copy(int r, unsigned char* stage) {
+    if (r < g.r1) {
+      const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS;
       if (page < 0 || page >= p.k.n_pages) {
         atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
         page = 0;
       }
       const int t = t0 + lane, off = page_shift >= 0 ? t & (page_size - 1) : t % page_size;
-      const uint32_t ks = (uint32_t)__cvta_generic_to_shared(ring + slot * G::STAGE_BYTES), vs = ks + KEYS * G::RB;
+      const int64_t ko = (page * p.k.stride_page + (int64_t)off * p.k.stride_off) * G::EB;
+      const int64_t vo = same ? ko : (page * p.v.stride_page + (int64_t)off * p.v.stride_off) * G::EB;
+      const uint32_t ks = (uint32_t)__cvta_generic_to_shared(stage), vs = ks + G::KEYS * G::RB;
 #pragma unroll
-      for (int i = 0; i < KEYS * NPC / 32; ++i) {
-        const int idx = i * 32 + lane, key = idx / NPC, pc = idx % NPC;
-        const int pg = __shfl_sync(0xffffffffu, (int)page, key), of = __shfl_sync(0xffffffffu, off, key);
-        const bool live = r < r1 && t0 + key < seq.hi && pc < npc;
-        const int64_t ko = live ? ((int64_t)pg * p.k.stride_page + (int64_t)of * p.k.stride_off) * G::EB + pc * 16 : 0;
-        const int64_t vo = live ? ((int64_t)pg * p.v.stride_page + (int64_t)of * p.v.stride_off) * G::EB + pc * 16 : 0;
-        cp_async16_zfill(ks + place<G::RB, LPK>(key, pc), kb + ko, live);
-        cp_async16_zfill(vs + place<G::RB, LPK>(key, pc), vb + vo, live);
+      for (int i = 0; i < G::KEYS * G::NPC / 32; ++i) {
+        const int idx = i * 32 + lane, key = idx / G::NPC, pc = idx % G::NPC;
+        const int64_t k0 = __shfl_sync(0xffffffffu, ko, key);
+        const int64_t v0 = same ? k0 : __shfl_sync(0xffffffffu, vo, key);
+        const bool live = t0 + key < g.seq.hi && pc < npc;
+        cp_async16_zfill(ks + Place::at(key, pc), live ? kb + k0 + pc * 16 : kb, live);
+        cp_async16_zfill(vs + Place::at(key, pc), live ? vb + v0 + pc * 16 : vb, live);
+      }
+    }
+    cp_async_commit();
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------
+// 16-bit and fp8 rows: mma.sync m16n8k16, the GT (8 or 16) query heads of a unit are the rows of the tile.
+//
+// S = Q K^T: ldmatrix gives the B operand from K rows as they lie; its columns 2 t, 2 t + 1 of a row are the A operand's of
+// O += P V, whose B operand is ldmatrix.trans of V rows.  fp8 (e5m2) rows are kept as bytes up to the registers, where an
+// element becomes the half-precision number whose upper byte it is: for K the four bytes that a lane gets are four
+// consecutive elements, so the contraction runs in that order and Q's fragments are laid out alike; for V a lane gets
+// two columns of two keys, the even columns of a block make one product and the odd ones another.  With fp8 rows all products
+// are in half precision; bfloat16 queries are brought to its range by a power of two per head (exact down to 2^-39 of the
+// head's largest element, below what the sum keeps).
+//
+// The weights go in two 16-bit terms, the rounded weight and what the rounding left.  Half-precision weights are scaled by 2^14
+// (largest: 16384), so that a weight of 2^-28 of the largest is still a normal number: many small weights add up.  The second term
+// may be zero or negative, which an infinite value turns into NaN: a warp that finds NaN in its output goes through its keys once
+// more with the first term alone.
+// ---------------------------------------------------------------------------------------------------
+template <int RB>
+struct MmaPlace {   // the eight rows that ldmatrix reads at once lie in eight different groups of banks
+  __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ (RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1))) << 4); }
+};
+
+template <int DT, bool F8, int DP, int GT>
+__global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_mma_kernel(const Params p, int tiles, int split, int least) {
+  using G = Geo<DT, F8, DP>;
+  using P = MmaPlace<G::RB>;
+  using T = typename Elem<DT>::type;
+  constexpr int MT = F8 ? HIPATTN_F16 : DT;          // type of the products
+  constexpr int KEYS = G::KEYS, MS = DP + 2, KS = DP / 16, NT = DP / 8, AR = GT / 4;   // AR: registers of an A fragment that are not padding
+  constexpr float kShift = MT == HIPATTN_F16 ? 14.f : 0.f;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, jq = lane & 3;
+  unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
+  float* s_merge = reinterpret_cast<float*>(smem);                       // over the rings when they are empty
+  uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + G::RING_BYTES);     // [KS][32][AR]: A fragments
+  __shared__ float s_up[16];                                             // power of two that a head's queries were multiplied by
+  const int units = p.HKV * tiles;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // (the merge waits for the whole of this grid)
+
+  Share sh{0, 0, 0, (int)(blockIdx.x / units)};
+  if (split && !find_share(p, units, G::ROUND, least, sh)) return;
+  const int64_t share_first = sh.first;
+
+  for (bool more = true; more;) {
+    const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
+    Feeder<G, P> feed(p, g, warp, lane);
+    auto begin = [&]() {
+      feed.fetch_page(g.r0);
+#pragma unroll
+      for (int i = 0; i < G::STAGES - 1; ++i) {
+        feed.copy(g.r0 + i, ring + i * G::STAGE_BYTES);
+        feed.fetch_page(g.r0 + i + 1);
       }
     };
-    fetch_page(r0);
+    __syncthreads();
+    begin();
+
+    // ---- the unit's queries ----
+    const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)sh.b * p.q_stride_b + (int64_t)g.h0 * p.q_stride_h;
+    if constexpr (F8 && DT == HIPATTN_BF16) {
+      for (int h = warp; h < GT; h += kWarps) {
+        float mx = 0.f;
+        if (h < g.live_heads)
+          for (int e = lane; e < p.D; e += 32) mx = fmaxf(mx, fabsf(Elem<DT>::to_f32(q[(int64_t)h * p.q_stride_h + e])));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        // 2^k with mx 2^k in [2^14, 2^15); k at most 126, so that 2^-k is a normal number too
+        int e = 0;
+        if (mx > 0.f && mx < INFINITY) frexpf(mx, &e);
+        if (lane == 0) s_up[h] = mx > 0.f && mx < INFINITY ? exp2f((float)min(15 - e, 126)) : 1.f;
+      }
+      __syncthreads();
+    }
+    for (int i = tid; i < KS * 32 * AR; i += kThreads) {
+      // register r of lane l: row l / 4 (+ 8), elements 2 (l % 4) .. (+ 8) of a step; with fp8 rows 4 (l % 4) .. (+ 2)
+      const int r = i % AR, l = i / AR % 32, ks = i / AR / 32;
+      const int row = (l >> 2) + (GT == 16 && (r & 1) ? 8 : 0), second = GT == 16 ? r >> 1 : r;
+      const int e = ks * 16 + (F8 ? (l & 3) * 4 + second * 2 : (l & 3) * 2 + second * 8);
+      float lo = 0.f, hi = 0.f;
+      if (row < g.live_heads) {
+        if (e < p.D) lo = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e]);
+        if (e + 1 < p.D) hi = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e + 1]);
+        if constexpr (F8 && DT == HIPATTN_BF16) { lo *= s_up[row]; hi *= s_up[row]; }
+      }
+      s_q[i] = pack2<MT>(lo, hi);
+    }
+    __syncthreads();
+    // logits to base 2; without a soft-cap in one product with the scale
+    float scale[GT / 8];
+#pragma unroll
+    for (int i = 0; i < GT / 8; ++i) {
+      scale[i] = p.sm_scale;
+      if constexpr (F8 && DT == HIPATTN_BF16) scale[i] /= s_up[gr + i * 8];
+      if (p.logit_softcap == 0.f) scale[i] *= kLog2e;
+    }
+
+    float o[NT][GT / 4], m_run[GT / 8], l_run[GT / 8];
+    for (bool two = true;; two = false) {      // (a second time only where there is NaN)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < GT / 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < GT / 8; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
+      int slot = 0;
+      for (int r = g.r0; r < g.r1; ++r) {
+        cp_async_wait<G::STAGES - 2>();
+        __syncwarp();
+        const unsigned char* ks = ring + slot * G::STAGE_BYTES;
+        const unsigned char* vs = ks + KEYS * G::RB;
+        // ---- S = Q K^T ----
+        float s[KEYS / 8][4];
+#pragma unroll
+        for (int i = 0; i < KEYS / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t a[4] = {0u, 0u, 0u, 0u};
+          if constexpr (GT == 16) {
+            const uint4 w = reinterpret_cast<const uint4*>(s_q)[k * 32 + lane];
+            a[0] = w.x; a[1] = w.y; a[2] = w.z; a[3] = w.w;
+          } else {
+            const uint2 w = reinterpret_cast<const uint2*>(s_q)[k * 32 + lane];
+            a[0] = w.x; a[2] = w.y;
+          }
+          if constexpr (F8) {
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; n += 4) {      // one piece of 32 keys, or of 16 and the padding of the call
+              uint32_t b[4];
+              if constexpr (KEYS >= 32) ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane, k));
+              else ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane & 15, k));
+#pragma unroll
+              for (int j = 0; j < 4 && n + j < KEYS / 8; ++j) mma16816<MT>(s[n + j], a, __byte_perm(b[j], 0, 0x1404), __byte_perm(b[j], 0, 0x3424));
+            }
+          } else {
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; n += 2) {
+              uint32_t b[4];
+              ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(n * 8 + (lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)));
+              mma16816<MT>(s[n], a, b[0], b[1]);
+              mma16816<MT>(s[n + 1], a, b[2], b[3]);
+            }
+          }
+        }
+        // ---- online softmax ----
+        const int t0 = g.seq.lo + r * G::ROUND + warp * KEYS + 2 * jq;
+        const bool tail = g.seq.lo + r * G::ROUND + (warp + 1) * KEYS > g.seq.hi;
+        uint32_t pa[KEYS / 16][4], pl[KEYS / 16][4];
+        bool moved = false;
+        float alpha[GT / 8];
+#pragma unroll
+        for (int i = 0; i < GT / 8; ++i) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = s[n][2 * i + e] * scale[i];
+              if (p.logit_softcap > 0.f) x = tanhf(x / p.logit_softcap) * p.logit_softcap * kLog2e;
+              if (tail && t0 + n * 8 + e >= g.seq.hi) x = -INFINITY;
+              s[n][2 * i + e] = x;
+              mx = fmaxf(mx, x);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m_run[i], mx), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
+          alpha[i] = exp2f(m_run[i] - base - kShift);
+          float sum = 0.f;
+#pragma unroll
+          for (int n = 0; n < KEYS / 8; ++n) {
+            const float x = exp2f(s[n][2 * i] - base), y = exp2f(s[n][2 * i + 1] - base);
+            sum += x + y;
+            const uint32_t hi = pack2<MT>(x, y);
+            pa[n / 2][(n & 1) * 2 + i] = hi;
+            pl[n / 2][(n & 1) * 2 + i] = pack2<MT>(x - Elem<MT>::round(x), y - Elem<MT>::round(y));
+          }
+          l_run[i] = l_run[i] * alpha[i] + sum;      // (this lane's keys; the four lanes of a row are added up at the end)
+          m_run[i] = m_new;
+          moved |= alpha[i] != 1.f;
+        }
+        if constexpr (GT == 8) {
+#pragma unroll
+          for (int n = 0; n < KEYS / 16; ++n) pa[n][1] = pa[n][3] = pl[n][1] = pl[n][3] = 0u;
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < GT / 4; ++e) o[n][e] *= alpha[e >> 1];
+        }
+        // ---- O += P V ----
+        auto product = [&](int n, int c, uint32_t b0, uint32_t b1) {
+          float d[4] = {o[n][0], o[n][1], 0.f, 0.f};
+          if constexpr (GT == 16) { d[2] = o[n][2]; d[3] = o[n][3]; }
+          mma16816<MT>(d, pa[c], b0, b1);
+          if (two) mma16816<MT>(d, pl[c], b0, b1);
+          o[n][0] = d[0];
+          o[n][1] = d[1];
+          if constexpr (GT == 16) { o[n][2] = d[2]; o[n][3] = d[3]; }
+        };
+#pragma unroll
+        for (int c = 0; c < KEYS / 16; ++c) {
+#pragma unroll
+          for (int pc = 0; pc < G::NPC; pc += 2) {
+            uint32_t b[4];
+            ldsm_x4_t(b[0], b[1], b[2], b[3], vs + P::at(c * 16 + (lane & 15), pc + (lane >> 4)));
+            if constexpr (F8) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                product((pc + h) * 2, c, __byte_perm(b[2 * h], 0, 0x2404), __byte_perm(b[2 * h + 1], 0, 0x2404));
+                product((pc + h) * 2 + 1, c, __byte_perm(b[2 * h], 0, 0x3414), __byte_perm(b[2 * h + 1], 0, 0x3414));
+              }
+            } else {
+              product(pc, c, b[0], b[1]);
+              product(pc + 1, c, b[2], b[3]);
+            }
+          }
+        }
+        __syncwarp();
+        feed.copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
+        feed.fetch_page(r + G::STAGES);
+        slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+      }
+      cp_async_wait<0>();
+      bool nan = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < GT / 4; ++e) nan |= o[n][e] != o[n][e];
+      if (!two || !__any_sync(0xffffffffu, nan)) break;
+      __syncwarp();
+      begin();
+    }
+    __syncthreads();
+
+    // ---- the warps' parts ----
+#pragma unroll
+    for (int i = 0; i < GT / 8; ++i) {
+      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
+      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
+      float* dst = s_merge + (warp * GT + gr + i * 8) * MS;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) dst[F8 ? (n >> 1) * 16 + (2 * jq + e) * 2 + (n & 1) : n * 8 + 2 * jq + e] = o[n][2 * i + e];
+      if (jq == 0) {
+        dst[DP] = m_run[i] - kShift;       // (numerator and denominator are 2^kShift times as large)
+        dst[DP + 1] = l_run[i];
+      }
+    }
+    __syncthreads();
+    more = end_segment<DT, DP, GT>(p, g, sh, share_first, units, split, s_merge);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------
+// fp32: FMA.  LPK lanes to a key for the logits, a lane owns columns of the output.
+// ---------------------------------------------------------------------------------------------------
+template <int RB, int LPK>
+struct FmaPlace {   // the lanes of a quarter warp, LPK to a row, reach eight different groups of banks
+  __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ ((key * LPK) & 7)) << 4); }
+};
+
+template <int DP, int GT>
+__global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_kernel(const Params p, int tiles, int split, int least) {
+  using G = FmaGeo<DP>;
+  using P = FmaPlace<G::RB, G::LPK>;
+  constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, MS = DP + 2;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
+  float* s_merge = reinterpret_cast<float*>(smem);                   // over the rings when they are empty
+  float* s_q = reinterpret_cast<float*>(smem + G::RING_BYTES);       // [GT][DP]
+  const int units = p.HKV * tiles;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  Share sh{0, 0, 0, (int)(blockIdx.x / units)};
+  if (split && !find_share(p, units, G::ROUND, least, sh)) return;
+  const int64_t share_first = sh.first;
+  const float cap = p.logit_softcap, scale = p.sm_scale;
+
+  for (bool more = true; more;) {
+    const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
+    Feeder<G, P> feed(p, g, warp, lane);
+    __syncthreads();
+    feed.fetch_page(g.r0);
 #pragma unroll
     for (int i = 0; i < G::STAGES - 1; ++i) {
-      copy(r0 + i, i);
-      cp_async_commit();
-      fetch_page(r0 + i + 1);
+      feed.copy(g.r0 + i, ring + i * G::STAGE_BYTES);
+      feed.fetch_page(g.r0 + i + 1);
+    }
+    for (int i = tid; i < GT * DP; i += kThreads) {
+      const int h = i / DP, e = i % DP;
+      float x = 0.f;
+      if (h < g.live_heads && e < p.D) x = reinterpret_cast<const float*>(p.q)[(int64_t)sh.b * p.q_stride_b + (int64_t)(g.h0 + h) * p.q_stride_h + e];
+      s_q[i] = x;
+    }
+    __syncthreads();
+
+    float m_run[GT], l_run[GT], acc[GT][G::PPL][4];
+#pragma unroll
+    for (int h = 0; h < GT; ++h) {
+      m_run[h] = -INFINITY;
+      l_run[h] = 0.f;
+#pragma unroll
+      for (int i = 0; i < G::PPL; ++i) acc[h][i][0] = acc[h][i][1] = acc[h][i][2] = acc[h][i][3] = 0.f;
     }
     int slot = 0;
-    for (int r = r0; r < r1; ++r) {
+    for (int r = g.r0; r < g.r1; ++r) {
       cp_async_wait<G::STAGES - 2>();
       __syncwarp();
       const unsigned char* ks = ring + slot * G::STAGE_BYTES;
       const unsigned char* vs = ks + KEYS * G::RB;
-      // ---- logits: LPK lanes to a key ----
+      // ---- logits ----
       const int key = lane / LPK, sub = lane % LPK;
       float s[GT];
 #pragma unroll
-      for (int g = 0; g < GT; ++g) s[g] = 0.f;
+      for (int h = 0; h < GT; ++h) s[h] = 0.f;
 #pragma unroll 4
       for (int j = 0; j < NPC / LPK; ++j) {
         const int pc = j * LPK + sub;
-        float kv[VEC];
-        widen_row<DT, F8>(*reinterpret_cast<const uint4*>(ks + place<G::RB, LPK>(key, pc)), kv);
+        const float4 kv = *reinterpret_cast<const float4*>(ks + P::at(key, pc));
 #pragma unroll
-        for (int g = 0; g < GT; ++g)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) s[g] = fmaf(s_q[g * DP + pc * VEC + e], kv[e], s[g]);
+        for (int h = 0; h < GT; ++h) {
+          const float4 qv = reinterpret_cast<const float4*>(s_q + h * DP)[pc];
+          s[h] = fmaf(qv.w, kv.w, fmaf(qv.z, kv.z, fmaf(qv.y, kv.y, fmaf(qv.x, kv.x, s[h]))));
+        }
       }
-      const bool in = seq.lo + r * G::ROUND + warp * KEYS + key < seq.hi;
+      const bool in = g.seq.lo + r * G::ROUND + warp * KEYS + key < g.seq.hi;
       float pr[GT];
 #pragma unroll
-      for (int g = 0; g < GT; ++g) {
+      for (int h = 0; h < GT; ++h) {
 #pragma unroll
-        for (int o = LPK >> 1; o > 0; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
-        s[g] *= scale;
-        if (cap > 0.f) s[g] = tanhf(s[g] / cap) * cap;
-        s[g] = in ? s[g] * kLog2e : -INFINITY;
-        float mx = s[g];
+        for (int o = LPK >> 1; o > 0; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
+        s[h] *= scale;
+        if (cap > 0.f) s[h] = tanhf(s[h] / cap) * cap;
+        s[h] = in ? s[h] * kLog2e : -INFINITY;
+        float mx = s[h];
 #pragma unroll
         for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        const float m_new = fmaxf(m_run[g], mx), base = m_new > -INFINITY ? m_new : 0.f;
-        const float alpha = exp2f(m_run[g] - base);
-        pr[g] = exp2f(s[g] - base);
-        l_run[g] = l_run[g] * alpha + (sub == 0 ? pr[g] : 0.f);
-        m_run[g] = m_new;
+        const float m_new = fmaxf(m_run[h], mx), base = m_new > -INFINITY ? m_new : 0.f;
+        const float alpha = exp2f(m_run[h] - base);
+        pr[h] = exp2f(s[h] - base);
+        l_run[h] = l_run[h] * alpha + (sub == 0 ? pr[h] : 0.f);
+        m_run[h] = m_new;
 #pragma unroll
         for (int i = 0; i < G::PPL; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[g][i][e] *= alpha;
+          for (int e = 0; e < 4; ++e) acc[h][i][e] *= alpha;
       }
-      // ---- o += p V: a lane owns pieces of the row ----
+      // ---- o += p V ----
 #pragma unroll
       for (int k0 = 0; k0 < KEYS; k0 += G::KP) {
         const int k = k0 + (G::KP > 1 ? lane / NPC : 0);
 #pragma unroll
         for (int i = 0; i < G::PPL; ++i) {
-          float vv[VEC];
-          widen_row<DT, F8>(*reinterpret_cast<const uint4*>(vs + place<G::RB, LPK>(k, lane % NPC + i * 32)), vv);
+          const float4 vv = *reinterpret_cast<const float4*>(vs + P::at(k, lane % NPC + i * 32));
 #pragma unroll
-          for (int g = 0; g < GT; ++g) {
-            const float x = __shfl_sync(0xffffffffu, pr[g], k * LPK);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[g][i][e] = fmaf(x, vv[e], acc[g][i][e]);
+          for (int h = 0; h < GT; ++h) {
+            const float x = __shfl_sync(0xffffffffu, pr[h], k * LPK);
+            acc[h][i][0] = fmaf(x, vv.x, acc[h][i][0]);
+            acc[h][i][1] = fmaf(x, vv.y, acc[h][i][1]);
+            acc[h][i][2] = fmaf(x, vv.z, acc[h][i][2]);
+            acc[h][i][3] = fmaf(x, vv.w, acc[h][i][3]);
           }
         }
       }
       __syncwarp();
-      copy(r + G::STAGES - 1, slot == 0 ? G::STAGES - 1 : slot - 1);
-      cp_async_commit();
-      fetch_page(r + G::STAGES);
+      feed.copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
+      feed.fetch_page(r + G::STAGES);
       slot = slot + 1 == G::STAGES ? 0 : slot + 1;
     }
     cp_async_wait<0>();
     __syncthreads();
 
-    // ---- join the warps ----
+    // ---- the warps' parts ----
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
+    for (int h = 0; h < GT; ++h) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l_run[g] += __shfl_xor_sync(0xffffffffu, l_run[g], o);
+      for (int o = 16; o > 0; o >>= 1) l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], o);
 #pragma unroll
       for (int i = 0; i < G::PPL; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-          for (int o = NPC; o < 32; o <<= 1) acc[g][i][e] += __shfl_xor_sync(0xffffffffu, acc[g][i][e], o);
-          if (lane < NPC) s_merge[(warp * GT + g) * MS + (lane % NPC + i * 32) * VEC + e] = acc[g][i][e];
+          for (int o = NPC; o < 32; o <<= 1) acc[h][i][e] += __shfl_xor_sync(0xffffffffu, acc[h][i][e], o);
+          if (lane < NPC) s_merge[(warp * GT + h) * MS + (lane % NPC + i * 32) * 4 + e] = acc[h][i][e];
         }
       if (lane == 0) {
-        s_merge[(warp * GT + g) * MS + DP] = m_run[g];
-        s_merge[(warp * GT + g) * MS + DP + 1] = l_run[g];
+        s_merge[(warp * GT + h) * MS + DP] = m_run[h];
+        s_merge[(warp * GT + h) * MS + DP + 1] = l_run[h];
       }
     }
     __syncthreads();
-    const bool whole = r0 == 0 && r1 == rounds;
-    float* part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (first == share_first ? 0 : 1)) * GT * MS;
-    for (int i = tid; i < live_heads * p.D; i += kThreads) {
-      const int g = i / p.D, e = i % p.D;
-      float M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_merge[(w * GT + g) * MS + DP]);
-      const float base = M > -INFINITY ? M : 0.f;
-      float num = 0.f, den = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(s_merge[(w * GT + g) * MS + DP] - base);
-        num += f * s_merge[(w * GT + g) * MS + e];
-        den += f * s_merge[(w * GT + g) * MS + DP + 1];
-      }
-      if (whole) {
-        finish<DT>(p, b, h0 + g, e, M, num, den);
-      } else {
-        part[g * MS + e] = num;
-        if (e == 0) {
-          part[g * MS + DP] = M;
-          part[g * MS + DP + 1] = den;
-        }
-      }
-    }
-    if (!split) return;
-    first += r1 - r0;
-    if (first >= last) return;
-    if (first == unit_at + (int64_t)rounds * units) {
-      unit_at = first;
-      ++b;
-    }
+    more = end_segment<HIPATTN_F32, DP, GT>(p, g, sh, share_first, units, split, s_merge);
   }
 }
 
@@ -445,14 +715,15 @@ template <int DT, bool F8, int DP>
 Layout layout_of(const Params& p) {
   Layout l;
   const int heads = p.H / p.HKV;
-  l.gt = heads <= 4 ? 4 : 8;
+  if (DT == HIPATTN_F32) l.gt = heads <= 4 ? 4 : 8;
+  else l.gt = heads <= 8 ? 8 : 16;
   l.tiles = cdiv(heads, l.gt);
   const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
   int64_t most = (int64_t)p.k.table_width * p.k.page_size;
   if (p.window > 0 && p.window < most) most = p.window;
   l.least = kLeastRounds;
   l.split = most > (int64_t)l.least * Geo<DT, F8, DP>::ROUND;
-  l.ctas = l.split ? kSMs : units;
+  l.ctas = l.split ? kSMs * Geo<DT, F8, DP>::CTAS : units;
   return l;
 }
 template <int DP>
@@ -461,10 +732,12 @@ int64_t scratch_bytes(const Layout& l) { return l.split ? l.ctas * 2 * l.gt * (D
 template <int DT, bool F8, int DP, int GT>
 int launch_gt(const Params& p, const Layout& l, cudaStream_t stream) {
   using G = Geo<DT, F8, DP>;
-  constexpr size_t smem = G::RING_BYTES + sizeof(float) * GT * DP;
+  constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP;
   static_assert(sizeof(float) * kWarps * GT * (DP + 2) <= G::RING_BYTES, "the join of the warps lies over the rings");
   HIPATTN_REQUIRE(l.ctas < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)l.ctas);
-  auto kern = paged_decode_kernel<DT, F8, DP, GT>;
+  void (*kern)(const Params, int, int, int);
+  if constexpr (DT == HIPATTN_F32) kern = paged_decode_fma_kernel<DP, GT>;
+  else kern = paged_decode_mma_kernel<DT, F8, DP, GT>;
   HIPATTN_CUDA_OK(allow_smem((const void*)kern, smem));
   kern<<<(unsigned)l.ctas, kThreads, smem, stream>>>(p, l.tiles, l.split, l.least);
   int rc = check_launch("paged_decode_kernel");
@@ -493,7 +766,8 @@ int launch_dp(const Params& p, cudaStream_t stream, int64_t* bytes) {
   }
   HIPATTN_REQUIRE(need == 0 || (p.scratch && p.scratch_bytes >= need && (uintptr_t)p.scratch % 16 == 0), HIPATTN_ERR_INVALID,
                   "paged_decode: %lld bytes of scratch are needed (16-byte aligned), %lld were given", (long long)need, (long long)p.scratch_bytes);
-  return l.gt == 4 ? launch_gt<DT, F8, DP, 4>(p, l, stream) : launch_gt<DT, F8, DP, 8>(p, l, stream);
+  constexpr int SMALL = DT == HIPATTN_F32 ? 4 : 8;
+  return l.gt == SMALL ? launch_gt<DT, F8, DP, SMALL>(p, l, stream) : launch_gt<DT, F8, DP, SMALL * 2>(p, l, stream);
 }
 template <int DT, bool F8>
 int launch_type(const Params& p, cudaStream_t stream, int64_t* bytes) {
