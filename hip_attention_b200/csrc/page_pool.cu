@@ -4,8 +4,6 @@
 // "the lowest free pages in the order of the entries" does not depend on how threads are scheduled.  A call is planned by one
 // cluster (the counts are cut into a slice for each of its CTAs, whose sums are exchanged through distributed shared memory), which
 // also changes the tables; pages are copied by a second launch over the whole GPU that the plan is handed to in device memory.
-#include <cuda_fp8.h>
-
 #include "common.cuh"
 
 namespace hipattn {
@@ -68,22 +66,42 @@ __device__ __forceinline__ N scan_block(N x, N* s, N& all) {
   return sum - x + __shfl_sync(0xffffffffu, ws - w, warp);
 }
 
-// Pages [begin, end) of a CTA's slice
-struct Slice {
-  int begin, end;
+// The counts are cut into runs of consecutive pages, one for each thread of the cluster in order (a multiple of four pages, so that
+// small pools are shared out as well); the pages of this thread are [begin, end).
+struct Run {
+  int64_t begin;
+  int end;
 };
-__device__ __forceinline__ Slice slice_of(int n, int rank) {
-  const int per = (int)(((int64_t)n + kPlanCtas - 1) / kPlanCtas);
-  Slice s;
-  s.begin = (int)min((int64_t)n, (int64_t)per * rank);
-  s.end = (int)min((int64_t)n, (int64_t)per * (rank + 1));
-  return s;
+__device__ __forceinline__ Run run_of(int n, int rank) {
+  const int per = (int)(((int64_t)n + (int64_t)kPlanCtas * kPlanThreads * 4 - 1) / ((int64_t)kPlanCtas * kPlanThreads * 4)) * 4;
+  Run r;
+  r.begin = ((int64_t)rank * kPlanThreads + threadIdx.x) * per;
+  r.end = (int)min((int64_t)n, r.begin + per);
+  return r;
 }
-// live pages of [begin, end)
-__device__ __forceinline__ int count_live(const int32_t* refs, int begin, int end) {
-  int n = 0;
-  for (int i = begin + (int)threadIdx.x; i < end; i += kPlanThreads) n += refs[i] > 0;
-  return n;
+// bit i: page `at` + i exists (below `end`)
+__device__ __forceinline__ uint32_t range_mask(int64_t at, int end) {
+  return at >= end ? 0u : (at + 32 <= end ? 0xffffffffu : (1u << (int)(end - at)) - 1u);
+}
+// bit i: page `at` + i (below `end`) is in use
+__device__ __forceinline__ uint32_t live_mask(const int32_t* refs, int64_t at, int end) {
+  uint32_t m = 0;
+  const bool aligned = ((uintptr_t)(refs + at) & 15) == 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 4) {
+    if (at + i >= end) continue;
+    int4 r = make_int4(0, 0, 0, 0);
+    if (aligned && at + i + 4 <= end) {
+      r = *reinterpret_cast<const int4*>(refs + at + i);
+    } else {
+      r.x = refs[at + i];
+      if (at + i + 1 < end) r.y = refs[at + i + 1];
+      if (at + i + 2 < end) r.z = refs[at + i + 2];
+      if (at + i + 3 < end) r.w = refs[at + i + 3];
+    }
+    m |= (uint32_t)((r.x > 0) | (r.y > 0) << 1 | (r.z > 0) << 2 | (r.w > 0) << 3) << i;
+  }
+  return m;
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -153,11 +171,17 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   }
   bad = __syncthreads_or(bad);
 
-  // ---- free pages before this CTA's slice, and in all ----
-  const Slice sl = slice_of(pool.n_pages, rank);
-  int live;
-  scan_block(count_live(pool.refs, sl.begin, sl.end), s_scan, live);
-  if (tid == 0) s_free = sl.end - sl.begin - live;
+  // ---- free pages before this thread's run, and in all ----
+  const Run run = run_of(pool.n_pages, rank);
+  int in_run = 0, in_slice;
+  uint32_t free0 = 0;                   // of the first 32 pages of the run, most often all of it
+  for (int64_t at = run.begin; at < run.end; at += 32) {
+    const uint32_t f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
+    if (at == run.begin) free0 = f;
+    in_run += __popc(f);
+  }
+  const int before_run = scan_block(in_run, s_scan, in_slice);
+  if (tid == 0) s_free = in_slice;
   cluster_sync();
   int base = 0;
   long long free_pages = 0;
@@ -175,14 +199,13 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
     return;
   }
 
-  // ---- deal out the free pages of the slice ----
-  for (int i0 = sl.begin; i0 < sl.end && base < total; i0 += kPlanThreads) {
-    const int page = i0 + tid;
-    const int is_free = page < sl.end && pool.refs[page] <= 0;
-    int all;
-    const int nth = base + scan_block(is_free, s_scan, all);
-    base += all;
-    if (is_free && nth < total) {
+  // ---- deal out the free pages of the run ----
+  long long nth = (long long)base + before_run;
+  for (int64_t at = run.begin; at < run.end && nth < total; at += 32) {
+    uint32_t f = at == run.begin ? free0 : ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
+    while (f && nth < total) {
+      const int page = (int)at + __ffs(f) - 1;
+      f &= f - 1;
       int lo = 0, hi = n - 1;                // the last entry that begins at or before nth
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -190,7 +213,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
         else hi = mid - 1;
       }
       pool.refs[page] = 1;
-      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + (nth - s_before[lo])] = page;
+      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + ((int)nth - s_before[lo])] = page;
       if (FORK) {
         int src = pool.table[(int64_t)a[lo] * pool.width + s_had[lo]];
         int tokens = s_new[lo] - s_had[lo] * P;
@@ -201,6 +224,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
         }
         reinterpret_cast<PageCopy*>(plan + 1)[nth] = PageCopy{src, page, tokens};
       }
+      ++nth;
     }
   }
   if (FORK) {
@@ -319,9 +343,15 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) p
   const int tid = threadIdx.x, rank = cluster_rank();
   const CompactPlan plan = compact_plan(scratch, pool.n_pages);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  const Slice sl = slice_of(pool.n_pages, rank);
-  int live;
-  scan_block(count_live(pool.refs, sl.begin, sl.end), s_scan, live);
+  const Run run = run_of(pool.n_pages, rank);
+  int in_run = 0, live;
+  uint32_t live0 = 0;                // of the first 32 pages of the run, most often all of it
+  for (int64_t at = run.begin; at < run.end; at += 32) {
+    const uint32_t f = live_mask(pool.refs, at, run.end);
+    if (at == run.begin) live0 = f;
+    in_run += __popc(f);
+  }
+  const int before_run = scan_block(in_run, s_scan, live);
   if (tid == 0) s_live = live;
   cluster_sync();
   int base = 0, m = 0;               // pages in use before the slice, and in all
@@ -330,10 +360,12 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) p
     if (r < rank) base += f;
     m += f;
   }
-  int below = live;                  // of them, numbered below m
-  if (sl.begin >= m) below = 0;
-  else if (sl.end > m) scan_block(count_live(pool.refs, sl.begin, m), s_scan, below);
-  if (tid == 0) s_below = below;
+  int below = 0;                     // of them, numbered below m
+  for (int64_t at = run.begin; at < min(run.end, m); at += 32)
+    below += __popc((at == run.begin ? live0 : live_mask(pool.refs, at, run.end)) & range_mask(at, m));
+  int all_below;
+  scan_block(below, s_scan, all_below);
+  if (tid == 0) s_below = all_below;
   cluster_sync();
   int stay = 0;
   for (int r = 0; r < kPlanCtas; ++r) stay += ld_cluster_int(&s_below, r);
@@ -344,19 +376,23 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) p
     if (in_use) *in_use = m;
   }
   if (stay == m) return;
-  for (int i0 = sl.begin; i0 < sl.end; i0 += kPlanThreads) {
-    const int page = i0 + tid;
-    const int is_live = page < sl.end && pool.refs[page] > 0;
-    int all;
-    const int lower = base + scan_block(is_live, s_scan, all);   // pages in use below this one
-    base += all;
-    if (page < sl.end) {
-      if (!is_live && page < m) plan.holes[page - lower] = page;
-      if (is_live && page >= m) {
-        plan.movers[lower - stay] = page;
-        plan.nth[page] = lower - stay;
+  int lower = base + before_run;     // pages in use below the next one
+  for (int64_t at = run.begin; at < run.end; at += 32) {
+    const uint32_t f = at == run.begin ? live0 : live_mask(pool.refs, at, run.end);
+    // holes below m, movers at m and beyond: the page's number less the pages in use below it, or that less those that stay
+    uint32_t pick = (~f & range_mask(at, min(run.end, m))) | (f & ~range_mask(at, m));
+    while (pick) {
+      const int i = __ffs(pick) - 1, page = (int)at + i;
+      pick &= pick - 1;
+      const int k = lower + __popc(f & ((1u << i) - 1u));
+      if (page < m) {
+        plan.holes[page - k] = page;
+      } else {
+        plan.movers[k - stay] = page;
+        plan.nth[page] = k - stay;
       }
     }
+    lower += __popc(f);
   }
 }
 
@@ -402,74 +438,126 @@ __global__ void __launch_bounds__(kCopyThreads) move_pages_kernel(const Pool poo
 // ---------------------------------------------------------------------------------------------------
 // new keys and values
 // ---------------------------------------------------------------------------------------------------
-// Eight elements of a row to a thread
+// Eight 16-bit values as e5m2, nearest, ties to even.  An e5m2 number is the upper byte of a half-precision one, so what is dropped
+// is rounded in integers: half a step less one, and one more where the byte is odd.  Subnormal numbers and the step to infinity
+// need nothing of their own; NaN keeps its top bit.  A bfloat16 value goes through half precision unharmed: that rounds only values
+// below 2^-17, which e5m2 makes zero either way (2^-17 itself is a tie), and those beyond 65504, which are infinite either way.
 template <int DT>
 __device__ __forceinline__ uint2 narrow_e5m2(const uint4& w) {
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-  uint32_t o[2] = {0, 0};
+  uint32_t o[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint16_t h = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
-    float f;
-    if (DT == HIPATTN_BF16) f = __uint_as_float((uint32_t)h << 16);
-    else f = __half2float(__ushort_as_half(h));
-    o[i >> 2] |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_NOSAT, __NV_E5M2) << (8 * (i & 3));
+  for (int i = 0; i < 4; ++i) {
+    uint32_t h = v[i];
+    if (DT == HIPATTN_BF16) h = pack2<HIPATTN_F16>(__uint_as_float(h << 16), __uint_as_float(h & 0xffff0000u));
+    const __half2 x = *reinterpret_cast<const __half2*>(&h);
+    const uint32_t nan = __hneu2_mask(x, x);
+    h = (h & ~nan) | (nan & 0x7e007e00u);
+    o[i] = h + 0x007f007fu + ((h >> 8) & 0x00010001u);
   }
-  return make_uint2(o[0], o[1]);
+  return make_uint2(__byte_perm(o[0], o[1], 0x7531), __byte_perm(o[2], o[3], 0x7531));
 }
 
+// A CTA writes `span` consecutive tokens: their slots are looked up once, by one thread each, while the first rows are on their way.
+constexpr int kWriteThreads = 256;
+constexpr int kMaxSpan = 32;
+constexpr int kWriteAhead = 4;    // 16-byte pieces of a thread in flight
 template <int DT, bool F8>
-__global__ void __launch_bounds__(256) write_kv_kernel(const hipattn_write_kv_params_t p) {
+__global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_write_kv_params_t p, int span) {
   constexpr int EB = Elem<DT>::bytes, VEC = 16 / EB, CB = F8 ? 1 : EB;
+  __shared__ int s_page[kMaxSpan], s_off[kMaxSpan];
   const int row_pieces = p.D / VEC, pieces = p.HKV * row_pieces;       // of a token, keys or values
-  const int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t tok = it / (2 * pieces);
-  if (tok >= p.N) return;
-  const int which = (int)(it % (2 * pieces)) / pieces, pc = (int)(it % pieces), h = pc / row_pieces, d = pc % row_pieces * VEC;
-  const hipattn_tokens_t& pool = which ? p.v_pool : p.k_pool;
-  const char* src = which ? (const char*)p.v + (tok * p.v_stride_t + (int64_t)h * p.v_stride_h + d) * EB
-                          : (const char*)p.k + (tok * p.k_stride_t + (int64_t)h * p.k_stride_h + d) * EB;
-  const uint4 x = *reinterpret_cast<const uint4*>(src);
-  auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldg((const long long*)q + i) : (int64_t)__ldg((const int*)q + i); };
-  // the token's sequence and place in it
-  int64_t first, count;
-  int b;
-  if (p.offsets) {
-    int lo = 0, hi = p.B;                  // the first b with tok < offsets[b + 1]
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (index(p.offsets, p.offsets_is_i64, mid + 1) <= tok) lo = mid + 1;
-      else hi = mid;
+  const int64_t tok0 = (int64_t)blockIdx.x * span;
+  const int tokens = (int)min((int64_t)span, p.N - tok0), items = tokens * 2 * pieces;
+  // item -> token, keys or values, head, element
+  struct Item {
+    int tok, which, h, d;
+  };
+  auto item_of = [&](int i) {
+    Item it;
+    const int half = i / pieces, pc = i - half * pieces;
+    it.tok = half >> 1;
+    it.which = half & 1;
+    it.h = pc / row_pieces;
+    it.d = (pc - it.h * row_pieces) * VEC;
+    return it;
+  };
+  auto load = [&](int i, uint4& x) {
+    if (i >= items) return;
+    const Item it = item_of(i);
+    const char* src = it.which ? (const char*)p.v + ((tok0 + it.tok) * p.v_stride_t + (int64_t)it.h * p.v_stride_h + it.d) * EB
+                               : (const char*)p.k + ((tok0 + it.tok) * p.k_stride_t + (int64_t)it.h * p.k_stride_h + it.d) * EB;
+    x = __ldcs(reinterpret_cast<const uint4*>(src));
+  };
+  uint4 x[kWriteAhead];
+#pragma unroll
+  for (int k = 0; k < kWriteAhead; ++k) load(k * kWriteThreads + threadIdx.x, x[k]);
+
+  if (threadIdx.x < tokens) {
+    auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldg((const long long*)q + i) : (int64_t)__ldg((const int*)q + i); };
+    const int64_t tok = tok0 + threadIdx.x;
+    int page = -1, off = 0;                  // -1: not written
+    // the token's sequence and place in it
+    int64_t first = 0, count = 0;
+    int b = -1;
+    if (p.offsets) {
+      int lo = 0, hi = p.B;                  // the first b with tok < offsets[b + 1]
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (index(p.offsets, p.offsets_is_i64, mid + 1) <= tok) lo = mid + 1;
+        else hi = mid;
+      }
+      if (lo < p.B) {                        // (else: behind the last sequence)
+        first = index(p.offsets, p.offsets_is_i64, lo);
+        count = index(p.offsets, p.offsets_is_i64, lo + 1) - first;
+        if (tok >= first) b = lo;            // (else: before the first)
+      }
+    } else {
+      count = p.N / p.B;
+      b = (int)(tok / count);
+      first = b * count;
     }
-    if (lo == p.B) return;                 // behind the last sequence
-    b = lo;
-    first = index(p.offsets, p.offsets_is_i64, b);
-    count = index(p.offsets, p.offsets_is_i64, b + 1) - first;
-    if (tok < first) return;               // before the first
-  } else {
-    count = p.N / p.B;
-    b = (int)(tok / count);
-    first = b * count;
+    const int64_t row = b < 0 ? -1 : (p.rows ? index(p.rows, p.rows_is_i64, b) : b);
+    if (row >= p.n_rows) {
+      atomicOr(p.status, HIPATTN_STATUS_SEQUENCE);
+    } else if (row >= 0) {
+      const int64_t t = index(p.k_pool.cache_seq_lens, p.k_pool.seq_lens_is_i64, row) - count + (tok - first);
+      if (t < 0 || t >= (int64_t)p.k_pool.table_width * p.k_pool.page_size || t > 0x7fffffff) {
+        atomicOr(p.status, HIPATTN_STATUS_TOKEN_RANGE);
+      } else {
+        const int pi = (int)t / p.k_pool.page_size;
+        const int64_t pg = index(p.k_pool.block_table, p.k_pool.table_is_i64, row * p.k_pool.table_stride_b + pi);
+        if (pg < 0 || pg >= p.k_pool.n_pages) {
+          atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
+        } else {
+          page = (int)pg;
+          off = (int)t - pi * p.k_pool.page_size;
+        }
+      }
+    }
+    s_page[threadIdx.x] = page;
+    s_off[threadIdx.x] = off;
   }
-  const int64_t row = p.rows ? index(p.rows, p.rows_is_i64, b) : b;
-  if (row < 0) return;
-  if (row >= p.n_rows) {
-    atomicOr(p.status, HIPATTN_STATUS_SEQUENCE);
-    return;
+  __syncthreads();
+  for (int i0 = threadIdx.x; i0 < items; i0 += kWriteAhead * kWriteThreads) {
+    uint4 now[kWriteAhead];
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) now[k] = x[k];
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) load(i0 + (kWriteAhead + k) * kWriteThreads, x[k]);
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) {
+      const int i = i0 + k * kWriteThreads;
+      if (i >= items) break;
+      const Item it = item_of(i);
+      const int page = s_page[it.tok];
+      if (page < 0) continue;
+      const hipattn_tokens_t& pool = it.which ? p.v_pool : p.k_pool;
+      char* dst = (char*)pool.cache + ((int64_t)page * pool.stride_page + (int64_t)s_off[it.tok] * pool.stride_off + (int64_t)it.h * pool.stride_ch + it.d) * CB;
+      if constexpr (F8) *reinterpret_cast<uint2*>(dst) = narrow_e5m2<DT>(now[k]);
+      else *reinterpret_cast<uint4*>(dst) = now[k];
+    }
   }
-  const int64_t t = index(pool.cache_seq_lens, pool.seq_lens_is_i64, row) - count + (tok - first);
-  if (t < 0 || t >= (int64_t)pool.table_width * pool.page_size) {
-    atomicOr(p.status, HIPATTN_STATUS_TOKEN_RANGE);
-    return;
-  }
-  const int64_t page = index(pool.block_table, pool.table_is_i64, row * pool.table_stride_b + t / pool.page_size);
-  if (page < 0 || page >= pool.n_pages) {
-    atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
-    return;
-  }
-  char* dst = (char*)pool.cache + (page * pool.stride_page + t % pool.page_size * pool.stride_off + (int64_t)h * pool.stride_ch + d) * CB;
-  if constexpr (F8) *reinterpret_cast<uint2*>(dst) = narrow_e5m2<DT>(x);
-  else *reinterpret_cast<uint4*>(dst) = x;
 }
 
 int validate_pool(const hipattn_page_pool_t* p, const char* what, bool caches) {
@@ -615,18 +703,23 @@ extern "C" int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream
   HIPATTN_REQUIRE((uintptr_t)p->k % 16 == 0 && (uintptr_t)p->v % 16 == 0 && p->k_stride_t % ra == 0 && p->k_stride_h % ra == 0 && p->v_stride_t % ra == 0 &&
                       p->v_stride_h % ra == 0,
                   HIPATTN_ERR_INVALID, "write_kv: rows of k and v must start on 16-byte boundaries");
-  const int64_t blocks = (p->N * 2 * p->HKV * (p->D / ra) + 255) / 256;
+  HIPATTN_REQUIRE((int64_t)p->HKV * p->D < (1 << 24) && p->k_pool.n_pages <= 0x7fffffffLL, HIPATTN_ERR_UNSUPPORTED, "write_kv: tokens of %lld values, %lld pages",
+                  (long long)p->HKV * p->D, (long long)p->k_pool.n_pages);
+  // tokens of a CTA: one each until the GPU is full four times over, then as many as have a few pieces for every thread
+  int64_t span = p->N / (kSMs * 4);
+  span = span < 1 ? 1 : (span > kMaxSpan ? kMaxSpan : span);
+  const int64_t blocks = (p->N + span - 1) / span;
   HIPATTN_REQUIRE(blocks < 0x7fffffffLL, HIPATTN_ERR_INVALID, "write_kv: grid of %lld blocks", (long long)blocks);
   const cudaStream_t s = (cudaStream_t)stream;
   switch (p->dtype) {
-    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, 256, 0, s>>>(*p); break;
+    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span); break;
     case HIPATTN_F16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, 256, 0, s>>>(*p);
-      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
+      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
       break;
     case HIPATTN_BF16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, 256, 0, s>>>(*p);
-      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, 256, 0, s>>>(*p);
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
+      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
       break;
     default: set_error("write_kv: unknown dtype %d", p->dtype); return HIPATTN_ERR_INVALID;
   }

@@ -80,6 +80,30 @@ __device__ __forceinline__ int64_t share_of(int64_t total, int ctas, int least) 
   return s < least ? least : s;
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// A product q.k as a logit to base 2: scale log2 e x, or with a soft-cap log2 e cap tanh(scale x / cap).  tanh(y) = 1 - 2 / (e^2y + 1) is
+// off by a few 2^-24 everywhere, which is what counts in a logit, in five instructions (tanhf, whose relative error is as small
+// near zero, and a division by the cap: 12 fp8 sequences with a soft-cap 268 us, XX so).
+struct Logit {
+  float k, cap;      // cap 0: none; else k = 2 log2 e scale / cap, cap = log2 e cap
+  __device__ __forceinline__ Logit(const Params& p, float scale) {
+    cap = p.logit_softcap * kLog2e;
+    k = p.logit_softcap > 0.f ? 2.f * kLog2e * scale / p.logit_softcap : kLog2e * scale;
+  }
+  __device__ __forceinline__ float of(float x) const {
+    if (cap > 0.f) {
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ex2(x * k) + 1.f));
+      return fmaf(-2.f * cap, r, cap);
+    }
+    return x * k;
+  }
+};
+
 // element e of the output row of head h, from the joined maximum (base 2), numerator and denominator
 template <int DT>
 __device__ __forceinline__ void finish(const Params& p, int b, int h, int e, float M, float num, float den) {
@@ -95,13 +119,12 @@ struct Geo {
   static constexpr int EB = F8 ? 1 : Elem<DT>::bytes;
   static constexpr int RB = DP * EB;
   static constexpr int NPC = RB / 16;                         // pieces of a row
-  static constexpr int FIT = 4096 / RB > 32 ? 32 : 4096 / RB;
-  static constexpr int KEYS = DT != HIPATTN_F32 && FIT < 16 ? 16 : FIT;
+  static constexpr int KEYS = DT == HIPATTN_F32 ? 4096 / RB : (RB == 64 ? 32 : 16);
   static constexpr int STAGES = 3;
   static constexpr int ROUND = KEYS * kWarps;
   static constexpr int STAGE_BYTES = 2 * KEYS * RB;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES * kWarps;
-  static constexpr int CTAS = RING_BYTES <= 100 * 1024 ? 2 : 1;   // per multiprocessor
+  static constexpr int CTAS = 200 * 1024 / RING_BYTES;        // per multiprocessor: 4, 2 or 1
 };
 template <int DP>
 struct FmaGeo : Geo<HIPATTN_F32, false, DP> {
@@ -189,9 +212,9 @@ __device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, 
 // The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 2]: to the output, or to scratch.  Returns whether more is to come.
 template <int DT, int DP, int GT>
 __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, Share& sh, int64_t share_first, int units, int split, const float* s_merge) {
-  constexpr int MS = DP + 2;
+  constexpr int MS = DP + 2, PS = DP + 4;
   const bool whole = g.r0 == 0 && g.r1 == g.rounds;
-  float* part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * MS;
+  float* part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * PS;
   for (int i = threadIdx.x; i < g.live_heads * p.D; i += kThreads) {
     const int h = i / p.D, e = i % p.D;
     float M = -INFINITY;
@@ -208,10 +231,10 @@ __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, S
     if (whole) {
       finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
     } else {
-      part[h * MS + e] = num;
+      part[h * PS + e] = num;
       if (e == 0) {
-        part[h * MS + DP] = M;
-        part[h * MS + DP + 1] = den;
+        part[h * PS + DP] = M;
+        part[h * PS + DP + 1] = den;
       }
     }
   }
@@ -225,16 +248,16 @@ __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, S
   return true;
 }
 
-// Asynchronous copies of a warp's keys into its ring.  Lane `key` looks up a key's page one round ahead of its copies and shares
+// Asynchronous copies of a warp's keys into its ring.  Lane `key` looks up a key's page two rounds ahead of its copies and shares
 // out where its rows begin; a row that is not attended is sixteen zero bytes a piece (what lies there may be anything, NaN too).
 template <class G, class Place>
 struct Feeder {
   const Params& p;
   const Segment& g;
-  const char *kb, *vb;        // the KV head's rows, this lane's piece
-  int64_t page = 0;
+  const char *kb, *vb;            // the KV head's rows
+  int64_t page = 0, page2 = 0;    // of this lane's key in the next round to be copied, and in the one after it
   int page_size, page_shift, warp, lane, npc;
-  bool same;                  // K and V pools are laid out alike
+  bool same;                      // K and V pools are laid out alike
   __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_) : p(p_), g(g_), warp(warp_), lane(lane_) {
     page_size = p.k.page_size;
     page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
@@ -245,13 +268,14 @@ struct Feeder {
   }
   __device__ __forceinline__ void fetch_page(int r) {
     const int t = g.seq.lo + r * G::ROUND + warp * G::KEYS + lane;
-    page = 0;
+    page = page2;
+    page2 = 0;
     if (r < g.r1 && lane < G::KEYS && t < g.seq.hi)
-      page = load_index(p.k.block_table, p.k.table_is_i64, g.seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
+      page2 = load_index(p.k.block_table, p.k.table_is_i64, g.seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
   }
   __device__ __forceinline__ void copy(int r, unsigned char* stage) {
     if (r < g.r1) {
-      const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS;
+      const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS, live_keys = g.seq.hi - t0;
       if (page < 0 || page >= p.k.n_pages) {
         atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
         page = 0;
@@ -265,12 +289,30 @@ struct Feeder {
         const int idx = i * 32 + lane, key = idx / G::NPC, pc = idx % G::NPC;
         const int64_t k0 = __shfl_sync(0xffffffffu, ko, key);
         const int64_t v0 = same ? k0 : __shfl_sync(0xffffffffu, vo, key);
-        const bool live = t0 + key < g.seq.hi && pc < npc;
-        cp_async16_zfill(ks + Place::at(key, pc), live ? kb + k0 + pc * 16 : kb, live);
-        cp_async16_zfill(vs + Place::at(key, pc), live ? vb + v0 + pc * 16 : vb, live);
+        // (a key that is not attended has the address of a row of page 0, which is not read)
+        const bool live = key < live_keys && pc < npc;
+        const int at = pc < npc ? pc * 16 : 0;
+        cp_async16_zfill(ks + Place::at(key, pc), kb + at + k0, live);
+        cp_async16_zfill(vs + Place::at(key, pc), vb + at + v0, live);
       }
     }
     cp_async_commit();
+  }
+  // the first rounds of a segment on their way
+  __device__ __forceinline__ void begin(unsigned char* ring) {
+    fetch_page(g.r0);
+    fetch_page(g.r0 + 1);
+#pragma unroll
+    for (int i = 0; i < G::STAGES - 1; ++i) {
+      copy(g.r0 + i, ring + i * G::STAGE_BYTES);
+      fetch_page(g.r0 + i + 2);
+    }
+  }
+  // round r is done: its place in the ring goes to round r + STAGES - 1
+  __device__ __forceinline__ void next(int r, unsigned char* ring, int& slot) {
+    copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
+    fetch_page(r + G::STAGES + 1);
+    slot = slot + 1 == G::STAGES ? 0 : slot + 1;
   }
 };
 
@@ -286,10 +328,21 @@ struct Feeder {
 // head's largest element, below what the sum keeps).
 //
 // The weights go in two 16-bit terms, the rounded weight and what the rounding left.  Half-precision weights are scaled by 2^14
-// (largest: 16384), so that a weight of 2^-28 of the largest is still a normal number: many small weights add up.  The second term
-// may be zero or negative, which an infinite value turns into NaN: a warp that finds NaN in its output goes through its keys once
-// more with the first term alone.
+// (largest: 16384), so that a weight of 2^-28 of the largest is still a normal number: many small weights add up.  Of eight heads the
+// second terms are the rows 8 to 15 of the tile, with sums of their own, and cost nothing; of sixteen they are a second product.
+// The second term may be zero or negative, which an infinite value turns into NaN: eight heads leave it out where the first sum is
+// not finite; of sixteen a warp that finds NaN in its output goes through its keys once more with the first term alone.
 // ---------------------------------------------------------------------------------------------------
+// the halves of two packed 16-bit elements
+template <int MT>
+__device__ __forceinline__ float lower(uint32_t w) {
+  return MT == HIPATTN_BF16 ? __uint_as_float(w << 16) : __low2float(*reinterpret_cast<const __half2*>(&w));
+}
+template <int MT>
+__device__ __forceinline__ float upper(uint32_t w) {
+  return MT == HIPATTN_BF16 ? __uint_as_float(w & 0xffff0000u) : __high2float(*reinterpret_cast<const __half2*>(&w));
+}
+
 template <int RB>
 struct MmaPlace {   // the eight rows that ldmatrix reads at once lie in eight different groups of banks
   __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ (RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1))) << 4); }
@@ -319,16 +372,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   for (bool more = true; more;) {
     const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
     Feeder<G, P> feed(p, g, warp, lane);
-    auto begin = [&]() {
-      feed.fetch_page(g.r0);
-#pragma unroll
-      for (int i = 0; i < G::STAGES - 1; ++i) {
-        feed.copy(g.r0 + i, ring + i * G::STAGE_BYTES);
-        feed.fetch_page(g.r0 + i + 1);
-      }
-    };
     __syncthreads();
-    begin();
+    feed.begin(ring);
 
     // ---- the unit's queries ----
     const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)sh.b * p.q_stride_b + (int64_t)g.h0 * p.q_stride_h;
@@ -360,21 +405,13 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       s_q[i] = pack2<MT>(lo, hi);
     }
     __syncthreads();
-    // logits to base 2; without a soft-cap in one product with the scale
-    float scale[GT / 8];
-#pragma unroll
-    for (int i = 0; i < GT / 8; ++i) {
-      scale[i] = p.sm_scale;
-      if constexpr (F8 && DT == HIPATTN_BF16) scale[i] /= s_up[gr + i * 8];
-      if (p.logit_softcap == 0.f) scale[i] *= kLog2e;
-    }
+    const Logit logit0(p, F8 && DT == HIPATTN_BF16 ? p.sm_scale / s_up[gr] : p.sm_scale);
+    const Logit logit1(p, F8 && DT == HIPATTN_BF16 && GT == 16 ? p.sm_scale / s_up[gr + 8] : p.sm_scale);
 
-    float o[NT][GT / 4], m_run[GT / 8], l_run[GT / 8];
-    for (bool two = true;; two = false) {      // (a second time only where there is NaN)
+    float o[NT][4], m_run[GT / 8], l_run[GT / 8];
+    for (bool two = true;; two = false) {      // (a second time only for sixteen heads, and where there is NaN)
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < GT / 4; ++e) o[i][e] = 0.f;
+      for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
       for (int i = 0; i < GT / 8; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
       int slot = 0;
@@ -384,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         const unsigned char* ks = ring + slot * G::STAGE_BYTES;
         const unsigned char* vs = ks + KEYS * G::RB;
         // ---- S = Q K^T ----
+        uint32_t kept[4];
         float s[KEYS / 8][4];
 #pragma unroll
         for (int i = 0; i < KEYS / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -398,14 +436,16 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
             a[0] = w.x; a[2] = w.y;
           }
           if constexpr (F8) {
-#pragma unroll
-            for (int n = 0; n < KEYS / 8; n += 4) {      // one piece of 32 keys, or of 16 and the padding of the call
-              uint32_t b[4];
-              if constexpr (KEYS >= 32) ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane, k));
-              else ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane & 15, k));
-#pragma unroll
-              for (int j = 0; j < 4 && n + j < KEYS / 8; ++j) mma16816<MT>(s[n + j], a, __byte_perm(b[j], 0, 0x1404), __byte_perm(b[j], 0, 0x3424));
+            uint32_t b[4];
+            if constexpr (KEYS == 32) {
+              ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane, k));
+            } else {                                   // two pieces of 16 keys
+              if ((k & 1) == 0) ldsm_x4(kept[0], kept[1], kept[2], kept[3], ks + P::at(lane & 15, k + (lane >> 4)));
+              b[0] = kept[(k & 1) * 2];
+              b[1] = kept[(k & 1) * 2 + 1];
             }
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n) mma16816<MT>(s[n], a, __byte_perm(b[n], 0, 0x1404), __byte_perm(b[n], 0, 0x3424));
           } else {
 #pragma unroll
             for (int n = 0; n < KEYS / 8; n += 2) {
@@ -419,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         // ---- online softmax ----
         const int t0 = g.seq.lo + r * G::ROUND + warp * KEYS + 2 * jq;
         const bool tail = g.seq.lo + r * G::ROUND + (warp + 1) * KEYS > g.seq.hi;
-        uint32_t pa[KEYS / 16][4], pl[KEYS / 16][4];
+        uint32_t pa[KEYS / 16][4], pl[KEYS / 16][4];     // A fragments; of eight heads pa alone, the second terms in its rows 8 to 15
         bool moved = false;
         float alpha[GT / 8];
 #pragma unroll
@@ -429,8 +469,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = s[n][2 * i + e] * scale[i];
-              if (p.logit_softcap > 0.f) x = tanhf(x / p.logit_softcap) * p.logit_softcap * kLog2e;
+              float x = (i ? logit1 : logit0).of(s[n][2 * i + e]);
               if (tail && t0 + n * 8 + e >= g.seq.hi) x = -INFINITY;
               s[n][2 * i + e] = x;
               mx = fmaxf(mx, x);
@@ -438,39 +477,33 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float m_new = fmaxf(m_run[i], mx), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
-          alpha[i] = exp2f(m_run[i] - base - kShift);
+          alpha[i] = ex2(m_run[i] - base - kShift);
           float sum = 0.f;
 #pragma unroll
           for (int n = 0; n < KEYS / 8; ++n) {
-            const float x = exp2f(s[n][2 * i] - base), y = exp2f(s[n][2 * i + 1] - base);
+            const float x = ex2(s[n][2 * i] - base), y = ex2(s[n][2 * i + 1] - base);
             sum += x + y;
-            const uint32_t hi = pack2<MT>(x, y);
+            const uint32_t hi = pack2<MT>(x, y), lo = pack2<MT>(x - lower<MT>(hi), y - upper<MT>(hi));
             pa[n / 2][(n & 1) * 2 + i] = hi;
-            pl[n / 2][(n & 1) * 2 + i] = pack2<MT>(x - Elem<MT>::round(x), y - Elem<MT>::round(y));
+            if constexpr (GT == 8) pa[n / 2][(n & 1) * 2 + 1] = lo;
+            else pl[n / 2][(n & 1) * 2 + i] = lo;
           }
           l_run[i] = l_run[i] * alpha[i] + sum;      // (this lane's keys; the four lanes of a row are added up at the end)
           m_run[i] = m_new;
           moved |= alpha[i] != 1.f;
         }
-        if constexpr (GT == 8) {
-#pragma unroll
-          for (int n = 0; n < KEYS / 16; ++n) pa[n][1] = pa[n][3] = pl[n][1] = pl[n][3] = 0u;
-        }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < GT / 4; ++e) o[n][e] *= alpha[e >> 1];
+            for (int e = 0; e < 4; ++e) o[n][e] *= alpha[GT == 16 ? e >> 1 : 0];
         }
         // ---- O += P V ----
         auto product = [&](int n, int c, uint32_t b0, uint32_t b1) {
-          float d[4] = {o[n][0], o[n][1], 0.f, 0.f};
-          if constexpr (GT == 16) { d[2] = o[n][2]; d[3] = o[n][3]; }
-          mma16816<MT>(d, pa[c], b0, b1);
-          if (two) mma16816<MT>(d, pl[c], b0, b1);
-          o[n][0] = d[0];
-          o[n][1] = d[1];
-          if constexpr (GT == 16) { o[n][2] = d[2]; o[n][3] = d[3]; }
+          mma16816<MT>(o[n], pa[c], b0, b1);
+          if constexpr (GT == 16) {
+            if (two) mma16816<MT>(o[n], pl[c], b0, b1);
+          }
         };
 #pragma unroll
         for (int c = 0; c < KEYS / 16; ++c) {
@@ -491,19 +524,27 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           }
         }
         __syncwarp();
-        feed.copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
-        feed.fetch_page(r + G::STAGES);
-        slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+        feed.next(r, ring, slot);
       }
       cp_async_wait<0>();
-      bool nan = false;
+      if constexpr (GT == 8) {
+        // the terms together; where the first is infinite or NaN the second says nothing (zero times infinity)
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < GT / 4; ++e) nan |= o[n][e] != o[n][e];
-      if (!two || !__any_sync(0xffffffffu, nan)) break;
-      __syncwarp();
-      begin();
+          for (int e = 0; e < 2; ++e)
+            if (fabsf(o[n][e]) < INFINITY) o[n][e] += o[n][e + 2];
+        break;
+      } else {
+        bool nan = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) nan |= o[n][e] != o[n][e];
+        if (!two || !__any_sync(0xffffffffu, nan)) break;
+        __syncwarp();
+        feed.begin(ring);
+      }
     }
     __syncthreads();
 
@@ -551,18 +592,13 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   Share sh{0, 0, 0, (int)(blockIdx.x / units)};
   if (split && !find_share(p, units, G::ROUND, least, sh)) return;
   const int64_t share_first = sh.first;
-  const float cap = p.logit_softcap, scale = p.sm_scale;
+  const Logit logit(p, p.sm_scale);
 
   for (bool more = true; more;) {
     const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
     Feeder<G, P> feed(p, g, warp, lane);
     __syncthreads();
-    feed.fetch_page(g.r0);
-#pragma unroll
-    for (int i = 0; i < G::STAGES - 1; ++i) {
-      feed.copy(g.r0 + i, ring + i * G::STAGE_BYTES);
-      feed.fetch_page(g.r0 + i + 1);
-    }
+    feed.begin(ring);
     for (int i = tid; i < GT * DP; i += kThreads) {
       const int h = i / DP, e = i % DP;
       float x = 0.f;
@@ -606,15 +642,13 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
       for (int h = 0; h < GT; ++h) {
 #pragma unroll
         for (int o = LPK >> 1; o > 0; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-        s[h] *= scale;
-        if (cap > 0.f) s[h] = tanhf(s[h] / cap) * cap;
-        s[h] = in ? s[h] * kLog2e : -INFINITY;
+        s[h] = in ? logit.of(s[h]) : -INFINITY;
         float mx = s[h];
 #pragma unroll
         for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         const float m_new = fmaxf(m_run[h], mx), base = m_new > -INFINITY ? m_new : 0.f;
-        const float alpha = exp2f(m_run[h] - base);
-        pr[h] = exp2f(s[h] - base);
+        const float alpha = ex2(m_run[h] - base);
+        pr[h] = ex2(s[h] - base);
         l_run[h] = l_run[h] * alpha + (sub == 0 ? pr[h] : 0.f);
         m_run[h] = m_new;
 #pragma unroll
@@ -640,9 +674,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
         }
       }
       __syncwarp();
-      feed.copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
-      feed.fetch_page(r + G::STAGES);
-      slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+      feed.next(r, ring, slot);
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -670,35 +702,69 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   }
 }
 
-// Joins the parts of a unit that lies in several shares, in their order.  One CTA per sequence and unit.
+// Joins the parts of a unit that lies in several shares, in their order.  One CTA per sequence, unit and `hb` of its heads; the
+// warps of a head (all eight of them for a single head) take the parts in turn and meet in shared memory.
+constexpr int kMergeWarps = 8;
 template <int DT, int DP, int GT>
-__global__ void __launch_bounds__(128) paged_decode_merge_kernel(const Params p, int tiles, int ctas, int round, int least) {
-  constexpr int MS = DP + 2;
-  __shared__ int64_t s_sum[8];
-  const int heads = p.H / p.HKV, units = p.HKV * tiles;
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(const Params p, int tiles, int ctas, int round, int least, int hb) {
+  constexpr int PS = DP + 4, V = DP / 4, VL = V > 32 ? V / 32 : 1;       // float4s of a row, and of a lane
+  __shared__ int64_t s_sum[2 * kMergeWarps];
+  __shared__ __align__(16) float s_num[kMergeWarps][DP];
+  const int heads = p.H / p.HKV, units = p.HKV * tiles, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
   const int rounds = rounds_of(sequence_of(p, b, false), round);
   int64_t total, before;
-  sum_rounds<128>(p, b, round, s_sum, total, before);
+  sum_rounds<kMergeWarps * 32>(p, b, round, s_sum, total, before);
   const int64_t share = share_of(total * units, ctas, least), begin = before * units + (int64_t)u * rounds;
   const int c0 = (int)(begin / share), c1 = (int)((begin + rounds - 1) / share);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (every CTA: what follows on the stream waits for this grid alone)
   if (c0 == c1) return;
   const int tile = u % tiles, h0 = u / tiles * heads + tile * GT, live_heads = min(GT, heads - tile * GT);
-  const int first_slot = begin == c0 * share ? 0 : 1;
-  const float* parts = reinterpret_cast<const float*>(p.scratch);
-  for (int i = threadIdx.x; i < live_heads * p.D; i += 128) {
-    const int g = i / p.D, e = i % p.D;
-    float M = -INFINITY, num = 0.f, den = 0.f;
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, parts[(((int64_t)c * 2 + (c == c0 ? first_slot : 0)) * GT + g) * MS + DP]);
-    const float base = M > -INFINITY ? M : 0.f;
-    for (int c = c0; c <= c1; ++c) {
-      const float* part = parts + (((int64_t)c * 2 + (c == c0 ? first_slot : 0)) * GT + g) * MS;
-      const float f = exp2f(part[DP] - base);
-      num += f * part[e];
-      den += f * part[DP + 1];
+  const float* parts = reinterpret_cast<const float*>(p.scratch) + ((int64_t)c0 * 2 + (begin == c0 * share ? 0 : 1)) * GT * PS;   // of share c0
+  const float* later = reinterpret_cast<const float*>(p.scratch);                                                               // of share c: c * 2 * GT * PS
+  const int per_head = hb < kMergeWarps ? kMergeWarps / hb : 1;           // warps of a head
+  for (int i0 = 0; i0 < hb; i0 += kMergeWarps / per_head) {
+    const int h = blockIdx.y * hb + i0 + warp / per_head, sub = warp % per_head;
+    const bool live = h < live_heads && h < (int)(blockIdx.y + 1) * hb;
+    float M = -INFINITY, den = 0.f;
+    float4 num[VL];
+#pragma unroll
+    for (int j = 0; j < VL; ++j) num[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (live) {
+      auto row = [&](int c) { return (c == c0 ? parts : later + (int64_t)c * 2 * GT * PS) + h * PS; };
+      for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, __ldcg(row(c) + DP));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      const float base = M > -INFINITY ? M : 0.f;
+      for (int c = c0 + lane; c <= c1; c += 32) den += exp2f(__ldcg(row(c) + DP) - base) * __ldcg(row(c) + DP + 1);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+#pragma unroll 4
+      for (int c = c0 + sub; c <= c1; c += per_head) {
+        const float f = exp2f(__ldcg(row(c) + DP) - base);
+#pragma unroll
+        for (int j = 0; j < VL; ++j) {
+          if (V < 32 && lane >= V) continue;
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(row(c)) + lane + j * 32);
+          num[j].x += f * x.x;
+          num[j].y += f * x.y;
+          num[j].z += f * x.z;
+          num[j].w += f * x.w;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VL; ++j)
+        if (V >= 32 || lane < V) *reinterpret_cast<float4*>(&s_num[warp][(lane + j * 32) * 4]) = num[j];
     }
-    finish<DT>(p, b, h0 + g, e, M, num, den);
+    __syncthreads();
+    if (live) {
+      for (int e = sub * 32 + lane; e < p.D; e += per_head * 32) {
+        float x = 0.f;
+        for (int w = warp - sub; w < warp - sub + per_head; ++w) x += s_num[w][e];
+        finish<DT>(p, b, h0 + h, e, M, x, den);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -727,7 +793,7 @@ Layout layout_of(const Params& p) {
   return l;
 }
 template <int DP>
-int64_t scratch_bytes(const Layout& l) { return l.split ? l.ctas * 2 * l.gt * (DP + 2) * (int64_t)sizeof(float) : 0; }
+int64_t scratch_bytes(const Layout& l) { return l.split ? l.ctas * 2 * l.gt * (DP + 4) * (int64_t)sizeof(float) : 0; }
 
 template <int DT, bool F8, int DP, int GT>
 int launch_gt(const Params& p, const Layout& l, cudaStream_t stream) {
@@ -743,15 +809,19 @@ int launch_gt(const Params& p, const Layout& l, cudaStream_t stream) {
   int rc = check_launch("paged_decode_kernel");
   if (rc || !l.split) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * p.HKV * l.tiles));
-  cfg.blockDim = dim3(128);
+  // few units have many parts each: one CTA per head then
+  const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
+  const int hb = units < kSMs ? 1 : GT, heads = p.H / p.HKV;
+  HIPATTN_REQUIRE(units < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)units);
+  cfg.gridDim = dim3((unsigned)units, (unsigned)cdiv(heads < GT ? heads : GT, hb));
+  cfg.blockDim = dim3(kMergeWarps * 32);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l.tiles, (int)l.ctas, (int)G::ROUND, l.least));
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l.tiles, (int)l.ctas, (int)G::ROUND, l.least, hb));
   return check_launch("paged_decode_merge_kernel");
 }
 
