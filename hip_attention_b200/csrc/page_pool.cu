@@ -107,6 +107,8 @@ __device__ __forceinline__ uint32_t live_mask(const int32_t* refs, int64_t at, i
 // ---------------------------------------------------------------------------------------------------
 // extend and fork
 // ---------------------------------------------------------------------------------------------------
+constexpr int kDealt = 8192;   // pages that a CTA deals out at a time
+
 // A copied page: source, destination, tokens
 struct PageCopy {
   int src, dst, tokens;
@@ -126,9 +128,19 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   __shared__ long long s_scan64[kPlanWarps];
   __shared__ int s_scan[kPlanWarps];
   __shared__ int s_free, s_longest;
+  __shared__ int s_dealt[kDealt];
   const int tid = threadIdx.x, rank = cluster_rank(), P = pool.page_size;
   if (FORK) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
+  // ---- this thread's free pages (on their way while the entries are read) ----
+  const Run run = run_of(pool.n_pages, rank);
+  int in_run = 0;
+  uint32_t free0 = 0;                   // of the first 32 pages of the run, most often all of it
+  for (int64_t at = run.begin; at < run.end; at += 32) {
+    const uint32_t f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
+    if (at == run.begin) free0 = f;
+    in_run += __popc(f);
+  }
   for (int i = tid; i < (pool.n_seqs + 31) / 32; i += kPlanThreads) s_named[i] = 0;
   if (tid == 0) s_longest = 0;
   __syncthreads();
@@ -172,14 +184,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   bad = __syncthreads_or(bad);
 
   // ---- free pages before this thread's run, and in all ----
-  const Run run = run_of(pool.n_pages, rank);
-  int in_run = 0, in_slice;
-  uint32_t free0 = 0;                   // of the first 32 pages of the run, most often all of it
-  for (int64_t at = run.begin; at < run.end; at += 32) {
-    const uint32_t f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
-    if (at == run.begin) free0 = f;
-    in_run += __popc(f);
-  }
+  int in_slice;
   const int before_run = scan_block(in_run, s_scan, in_slice);
   if (tid == 0) s_free = in_slice;
   cluster_sync();
@@ -199,21 +204,36 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
     return;
   }
 
-  // ---- deal out the free pages of the run ----
+  // ---- deal out the free pages: in order into shared memory, then to the entries, consecutive pages to consecutive threads ----
+  // (written by the threads that find them, 40000 pages of 262144 took 32 us, three multiprocessors storing word by word)
+  const long long stop = min(total, (long long)base + in_slice);
   long long nth = (long long)base + before_run;
-  for (int64_t at = run.begin; at < run.end && nth < total; at += 32) {
-    uint32_t f = at == run.begin ? free0 : ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
-    while (f && nth < total) {
-      const int page = (int)at + __ffs(f) - 1;
+  int64_t at = run.begin;
+  uint32_t f = free0;
+  for (long long from = base; from < stop; from += kDealt) {
+    const int count = (int)min((long long)kDealt, stop - from);
+    __syncthreads();
+    while (at < run.end && nth < from + count) {
+      if (f == 0) {
+        at += 32;
+        if (at < run.end) f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
+        continue;
+      }
+      s_dealt[nth - from] = (int)at + __ffs(f) - 1;
       f &= f - 1;
-      int lo = 0, hi = n - 1;                // the last entry that begins at or before nth
+      ++nth;
+    }
+    __syncthreads();
+    for (int k = tid; k < count; k += kPlanThreads) {
+      const int page = s_dealt[k], j = (int)(from + k);
+      int lo = 0, hi = n - 1;                // the last entry that begins at or before j
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (s_before[mid] <= nth) lo = mid;
+        if (s_before[mid] <= j) lo = mid;
         else hi = mid - 1;
       }
       pool.refs[page] = 1;
-      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + ((int)nth - s_before[lo])] = page;
+      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + (j - s_before[lo])] = page;
       if (FORK) {
         int src = pool.table[(int64_t)a[lo] * pool.width + s_had[lo]];
         int tokens = s_new[lo] - s_had[lo] * P;
@@ -222,9 +242,8 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
           src = page;
           tokens = 0;
         }
-        reinterpret_cast<PageCopy*>(plan + 1)[nth] = PageCopy{src, page, tokens};
+        reinterpret_cast<PageCopy*>(plan + 1)[j] = PageCopy{src, page, tokens};
       }
-      ++nth;
     }
   }
   if (FORK) {
@@ -458,40 +477,39 @@ __device__ __forceinline__ uint2 narrow_e5m2(const uint4& w) {
   return make_uint2(__byte_perm(o[0], o[1], 0x7531), __byte_perm(o[2], o[3], 0x7531));
 }
 
-// A CTA writes `span` consecutive tokens: their slots are looked up once, by one thread each, while the first rows are on their way.
+// A CTA writes `span` consecutive tokens: their slots are looked up once, by one thread each, while the first rows are on their way.  A
+// thread keeps its place in the row (keys or values, head, elements) and goes from token to token, `lanes` threads to a token.
 constexpr int kWriteThreads = 256;
 constexpr int kMaxSpan = 32;
 constexpr int kWriteAhead = 4;    // 16-byte pieces of a thread in flight
 template <int DT, bool F8>
-__global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_write_kv_params_t p, int span) {
+__global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_write_kv_params_t p, int span, int lanes) {
   constexpr int EB = Elem<DT>::bytes, VEC = 16 / EB, CB = F8 ? 1 : EB;
   __shared__ int s_page[kMaxSpan], s_off[kMaxSpan];
   const int row_pieces = p.D / VEC, pieces = p.HKV * row_pieces;       // of a token, keys or values
   const int64_t tok0 = (int64_t)blockIdx.x * span;
-  const int tokens = (int)min((int64_t)span, p.N - tok0), items = tokens * 2 * pieces;
-  // item -> token, keys or values, head, element
-  struct Item {
-    int tok, which, h, d;
-  };
-  auto item_of = [&](int i) {
-    Item it;
-    const int half = i / pieces, pc = i - half * pieces;
-    it.tok = half >> 1;
-    it.which = half & 1;
-    it.h = pc / row_pieces;
-    it.d = (pc - it.h * row_pieces) * VEC;
-    return it;
-  };
-  auto load = [&](int i, uint4& x) {
-    if (i >= items) return;
-    const Item it = item_of(i);
-    const char* src = it.which ? (const char*)p.v + ((tok0 + it.tok) * p.v_stride_t + (int64_t)it.h * p.v_stride_h + it.d) * EB
-                               : (const char*)p.k + ((tok0 + it.tok) * p.k_stride_t + (int64_t)it.h * p.k_stride_h + it.d) * EB;
-    x = __ldcs(reinterpret_cast<const uint4*>(src));
+  const int tokens = (int)min((int64_t)span, p.N - tok0);
+  const int groups = kWriteThreads / lanes, group = threadIdx.x / lanes;
+  int i = threadIdx.x % lanes;      // piece of a token: keys, then values
+  const char* src = nullptr;
+  char* dst = nullptr;
+  int64_t step = 0, page_step = 0, off_step = 0;      // bytes
+  auto place = [&]() {
+    const int which = i >= pieces, pc = i - which * pieces, h = pc / row_pieces, d = (pc - h * row_pieces) * VEC;
+    const hipattn_tokens_t& pool = which ? p.v_pool : p.k_pool;
+    step = (which ? p.v_stride_t : p.k_stride_t) * EB;
+    src = (const char*)(which ? p.v : p.k) + ((int64_t)h * (which ? p.v_stride_h : p.k_stride_h) + d) * EB + tok0 * step;
+    dst = (char*)pool.cache + ((int64_t)h * pool.stride_ch + d) * CB;
+    page_step = pool.stride_page * CB;
+    off_step = pool.stride_off * CB;
   };
   uint4 x[kWriteAhead];
+  auto load = [&](int tok, uint4& to) {
+    if (i < 2 * pieces && tok < tokens) to = __ldcs(reinterpret_cast<const uint4*>(src + tok * step));
+  };
+  if (i < 2 * pieces) place();
 #pragma unroll
-  for (int k = 0; k < kWriteAhead; ++k) load(k * kWriteThreads + threadIdx.x, x[k]);
+  for (int k = 0; k < kWriteAhead; ++k) load(group + k * groups, x[k]);
 
   if (threadIdx.x < tokens) {
     auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldg((const long long*)q + i) : (int64_t)__ldg((const int*)q + i); };
@@ -539,24 +557,29 @@ __global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_w
     s_off[threadIdx.x] = off;
   }
   __syncthreads();
-  for (int i0 = threadIdx.x; i0 < items; i0 += kWriteAhead * kWriteThreads) {
-    uint4 now[kWriteAhead];
+  for (;;) {
+    for (int t0 = group; t0 < tokens; t0 += kWriteAhead * groups) {
+      uint4 now[kWriteAhead];
 #pragma unroll
-    for (int k = 0; k < kWriteAhead; ++k) now[k] = x[k];
+      for (int k = 0; k < kWriteAhead; ++k) now[k] = x[k];
 #pragma unroll
-    for (int k = 0; k < kWriteAhead; ++k) load(i0 + (kWriteAhead + k) * kWriteThreads, x[k]);
+      for (int k = 0; k < kWriteAhead; ++k) load(t0 + (kWriteAhead + k) * groups, x[k]);
 #pragma unroll
-    for (int k = 0; k < kWriteAhead; ++k) {
-      const int i = i0 + k * kWriteThreads;
-      if (i >= items) break;
-      const Item it = item_of(i);
-      const int page = s_page[it.tok];
-      if (page < 0) continue;
-      const hipattn_tokens_t& pool = it.which ? p.v_pool : p.k_pool;
-      char* dst = (char*)pool.cache + ((int64_t)page * pool.stride_page + (int64_t)s_off[it.tok] * pool.stride_off + (int64_t)it.h * pool.stride_ch + it.d) * CB;
-      if constexpr (F8) *reinterpret_cast<uint2*>(dst) = narrow_e5m2<DT>(now[k]);
-      else *reinterpret_cast<uint4*>(dst) = now[k];
+      for (int k = 0; k < kWriteAhead; ++k) {
+        const int tok = t0 + k * groups;
+        if (i >= 2 * pieces || tok >= tokens) break;
+        const int page = s_page[tok];
+        if (page < 0) continue;
+        char* to = dst + page * page_step + s_off[tok] * off_step;
+        if constexpr (F8) *reinterpret_cast<uint2*>(to) = narrow_e5m2<DT>(now[k]);
+        else *reinterpret_cast<uint4*>(to) = now[k];
+      }
     }
+    i += lanes;                       // (tokens of more pieces than a CTA has threads)
+    if (i >= 2 * pieces) break;
+    place();
+#pragma unroll
+    for (int k = 0; k < kWriteAhead; ++k) load(group + k * groups, x[k]);
   }
 }
 
@@ -708,18 +731,20 @@ extern "C" int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream
   // tokens of a CTA: one each until the GPU is full four times over, then as many as have a few pieces for every thread
   int64_t span = p->N / (kSMs * 4);
   span = span < 1 ? 1 : (span > kMaxSpan ? kMaxSpan : span);
-  const int64_t blocks = (p->N + span - 1) / span;
+  const int64_t blocks = (p->N + span - 1) / span, pieces = 2 * (int64_t)p->HKV * (p->D / ra);
+  int lanes = 32;      // threads to a token: a power of two that its pieces fill
+  while (lanes < kWriteThreads && lanes < pieces) lanes *= 2;
   HIPATTN_REQUIRE(blocks < 0x7fffffffLL, HIPATTN_ERR_INVALID, "write_kv: grid of %lld blocks", (long long)blocks);
   const cudaStream_t s = (cudaStream_t)stream;
   switch (p->dtype) {
-    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span); break;
+    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes); break;
     case HIPATTN_F16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
-      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
+      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
       break;
     case HIPATTN_BF16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
-      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span);
+      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
+      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
       break;
     default: set_error("write_kv: unknown dtype %d", p->dtype); return HIPATTN_ERR_INVALID;
   }

@@ -134,6 +134,11 @@ struct FmaGeo : Geo<HIPATTN_F32, false, DP> {
   static constexpr int KP = B::NPC < 32 ? 32 / B::NPC : 1;          // V rows that a warp reads at once
 };
 
+// How a call is laid out.  split: every CTA takes a share of the row of rounds.  Else a unit is a CTA's, or a cluster's.
+struct Plan {
+  int tiles, split, least, cluster;   // head tiles of a KV head; rounds that a share has at least
+};
+
 // A CTA's share of the row of rounds
 struct Share {
   int64_t first, last, unit_at;   // [first, last): what is left of it; where sequence b begins in the row
@@ -141,46 +146,46 @@ struct Share {
 };
 // false: the share is empty.  All threads.
 __device__ __forceinline__ bool find_share(const Params& p, int units, int round, int least, Share& sh) {
-  __shared__ int64_t s_scan[kWarps];
+  __shared__ int64_t s_scan[2][kWarps];
   __shared__ int64_t s_found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int64_t total = 0;
-  // pass 0: the total; pass 1: the sequence that the share begins in
-  for (int pass = 0; pass < 2; ++pass) {
-    const int64_t share = pass ? share_of(total * units, gridDim.x, least) : 0;
-    sh.first = share * blockIdx.x;
-    if (pass && sh.first >= total * units) return false;
-    int64_t base = 0;
-    for (int c = 0; c < p.B; c += kThreads) {
-      const int i = c + tid;
-      const int64_t x = i < p.B ? rounds_of(sequence_of(p, i, false), round) : 0;
-      int64_t sum = x;
+  int64_t total = 0, x = 0, sum = 0;
+  // rounds of sequence c + tid (x) and of those of [c, c + tid] (sum); the sum over the CTA is returned
+  auto scan = [&](int c, int turn) {
+    const int i = c + tid;
+    x = sum = i < p.B ? rounds_of(sequence_of(p, i, false), round) : 0;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
-      }
-      if (lane == 31) s_scan[warp] = sum;
-      __syncthreads();
-      int64_t all = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) sum += s_scan[w];
-        all += s_scan[w];
-      }
-      if (pass) {
-        const int64_t end = (base + sum) * units;
-        if (sh.first < end && sh.first >= end - x * units) {
-          s_found[0] = i;
-          s_found[1] = end - x * units;
-        }
-      }
-      base += all;
-      __syncthreads();
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += y;
     }
-    total = base;
-    if (pass) sh.last = min(sh.first + share, total * units);
+    if (lane == 31) s_scan[turn & 1][warp] = sum;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) sum += s_scan[turn & 1][w];
+      all += s_scan[turn & 1][w];
+    }
+    return all;
+  };
+  int turn = 0;
+  for (int c = 0; c < p.B; c += kThreads) total += scan(c, turn++);
+  const int64_t share = share_of(total * units, gridDim.x, least);
+  sh.first = share * blockIdx.x;
+  sh.last = min(sh.first + share, total * units);
+  if (sh.first >= sh.last) return false;
+  int64_t base = 0;
+  for (int c = 0; c < p.B; c += kThreads) {
+    const int64_t all = p.B > kThreads ? scan(c, turn++) : total;   // (one sequence to a thread: it is in its registers)
+    const int64_t end = (base + sum) * units;
+    if (sh.first < end && sh.first >= end - x * units) {
+      s_found[0] = c + tid;
+      s_found[1] = end - x * units;
+    }
+    base += all;
   }
+  __syncthreads();
   sh.b = (int)s_found[0];
   sh.unit_at = s_found[1];
   return true;
@@ -191,14 +196,15 @@ struct Segment {
   Sequence seq;
   int rounds, r0, r1, hkv, h0, live_heads;
 };
-__device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, int tiles, int units, int split, int round, int gt) {
+__device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, const Plan& plan, int units, int round, int gt) {
   Segment g;
   g.seq = sequence_of(p, sh.b, threadIdx.x == 0);
   g.rounds = rounds_of(g.seq, round);
-  int u = blockIdx.x % units;
-  g.r0 = 0;
-  g.r1 = g.rounds;
-  if (split) {
+  const int tiles = plan.tiles, rank = blockIdx.x % plan.cluster, per = (g.rounds + plan.cluster - 1) / plan.cluster;
+  int u = blockIdx.x / plan.cluster % units;
+  g.r0 = min(g.rounds, rank * per);
+  g.r1 = min(g.rounds, g.r0 + per);
+  if (plan.split) {
     u = (int)((sh.first - sh.unit_at) / g.rounds);
     g.r0 = (int)((sh.first - sh.unit_at) % g.rounds);
     g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
@@ -209,12 +215,30 @@ __device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, 
   g.live_heads = min(gt, heads - tile * gt);
   return g;
 }
-// The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 2]: to the output, or to scratch.  Returns whether more is to come.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {   // the same shared-memory address in CTA `rank` of the cluster
+  uint32_t a;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+
+// The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 2]: to the output, to scratch, or (a cluster) to s_cta [GT][DP + 2],
+// where the CTAs of the cluster read one another's and each finishes some of the outputs.  Returns whether more is to come.
 template <int DT, int DP, int GT>
-__device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, Share& sh, int64_t share_first, int units, int split, const float* s_merge) {
+__device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, Share& sh, int64_t share_first, int units, const Plan& plan, const float* s_merge,
+                                            float* s_cta) {
   constexpr int MS = DP + 2, PS = DP + 4;
-  const bool whole = g.r0 == 0 && g.r1 == g.rounds;
-  float* part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * PS;
+  const bool whole = plan.split ? g.r0 == 0 && g.r1 == g.rounds : plan.cluster == 1;
+  float* part = s_cta;
+  int stride = MS;
+  if (plan.split) {
+    part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * PS;
+    stride = PS;
+  }
   for (int i = threadIdx.x; i < g.live_heads * p.D; i += kThreads) {
     const int h = i / p.D, e = i % p.D;
     float M = -INFINITY;
@@ -224,21 +248,41 @@ __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, S
     float num = 0.f, den = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = exp2f(s_merge[(w * GT + h) * MS + DP] - base);
+      const float f = ex2(s_merge[(w * GT + h) * MS + DP] - base);
       num += f * s_merge[(w * GT + h) * MS + e];
       den += f * s_merge[(w * GT + h) * MS + DP + 1];
     }
     if (whole) {
       finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
     } else {
-      part[h * PS + e] = num;
+      part[h * stride + e] = num;
       if (e == 0) {
-        part[h * PS + DP] = M;
-        part[h * PS + DP + 1] = den;
+        part[h * stride + DP] = M;
+        part[h * stride + DP + 1] = den;
       }
     }
   }
-  if (!split) return false;
+  if (plan.cluster > 1) {
+    cluster_sync();
+    const uint32_t own = (uint32_t)__cvta_generic_to_shared(s_cta);
+    for (int i = blockIdx.x % plan.cluster * kThreads + threadIdx.x; i < g.live_heads * p.D; i += plan.cluster * kThreads) {
+      const int h = i / p.D, e = i % p.D;
+      const uint32_t at = own + (uint32_t)(h * MS) * 4;
+      float M = -INFINITY, num = 0.f, den = 0.f;
+#pragma unroll 4
+      for (int r = 0; r < plan.cluster; ++r) M = fmaxf(M, ld_cluster(at + DP * 4, r));
+      const float base = M > -INFINITY ? M : 0.f;
+#pragma unroll 4
+      for (int r = 0; r < plan.cluster; ++r) {
+        const float f = ex2(ld_cluster(at + DP * 4, r) - base);
+        num += f * ld_cluster(at + e * 4, r);
+        den += f * ld_cluster(at + (DP + 1) * 4, r);
+      }
+      finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
+    }
+    cluster_sync();   // no CTA leaves while another reads its shared memory
+  }
+  if (!plan.split) return false;
   sh.first += g.r1 - g.r0;
   if (sh.first >= sh.last) return false;
   if (sh.first == sh.unit_at + (int64_t)g.rounds * units) {
@@ -256,28 +300,31 @@ struct Feeder {
   const Segment& g;
   const char *kb, *vb;            // the KV head's rows
   int64_t page = 0, page2 = 0;    // of this lane's key in the next round to be copied, and in the one after it
-  int page_size, page_shift, warp, lane, npc;
+  int page_size, page_shift, warp, lane, npc, most;
   bool same;                      // K and V pools are laid out alike
   __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_) : p(p_), g(g_), warp(warp_), lane(lane_) {
     page_size = p.k.page_size;
     page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
     npc = p.D * G::EB / 16;
+    most = (int)min((int64_t)p.k.table_width * page_size, (int64_t)0x7fff0000);
     kb = (const char*)p.k.cache + (int64_t)g.hkv * p.k.stride_ch * G::EB;
     vb = (const char*)p.v.cache + (int64_t)g.hkv * p.v.stride_ch * G::EB;
     same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
   }
-  __device__ __forceinline__ void fetch_page(int r) {
-    const int t = g.seq.lo + r * G::ROUND + warp * G::KEYS + lane;
+  // (any entry of the table may be read, so that the first are on their way before the length is known; those behind the
+  // sequence's pages are not used)
+  __device__ __forceinline__ void fetch_page(int r, int lo) {
+    const int t = lo + r * G::ROUND + warp * G::KEYS + lane;
     page = page2;
     page2 = 0;
-    if (r < g.r1 && lane < G::KEYS && t < g.seq.hi)
+    if (lane < G::KEYS && t < most)
       page2 = load_index(p.k.block_table, p.k.table_is_i64, g.seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
   }
   __device__ __forceinline__ void copy(int r, unsigned char* stage) {
     if (r < g.r1) {
       const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS, live_keys = g.seq.hi - t0;
       if (page < 0 || page >= p.k.n_pages) {
-        atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
+        if (lane < live_keys) atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
         page = 0;
       }
       const int t = t0 + lane, off = page_shift >= 0 ? t & (page_size - 1) : t % page_size;
@@ -300,18 +347,23 @@ struct Feeder {
   }
   // the first rounds of a segment on their way
   __device__ __forceinline__ void begin(unsigned char* ring) {
-    fetch_page(g.r0);
-    fetch_page(g.r0 + 1);
+    if (p.window > 0) {
+      fetch_page(g.r0, g.seq.lo);
+      fetch_page(g.r0 + 1, g.seq.lo);
+    } else {
+      fetch_page(g.r0, 0);
+      fetch_page(g.r0 + 1, 0);
+    }
 #pragma unroll
     for (int i = 0; i < G::STAGES - 1; ++i) {
       copy(g.r0 + i, ring + i * G::STAGE_BYTES);
-      fetch_page(g.r0 + i + 2);
+      fetch_page(g.r0 + i + 2, g.seq.lo);
     }
   }
   // round r is done: its place in the ring goes to round r + STAGES - 1
   __device__ __forceinline__ void next(int r, unsigned char* ring, int& slot) {
     copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
-    fetch_page(r + G::STAGES + 1);
+    fetch_page(r + G::STAGES + 1, g.seq.lo);
     slot = slot + 1 == G::STAGES ? 0 : slot + 1;
   }
 };
@@ -349,7 +401,7 @@ struct MmaPlace {   // the eight rows that ldmatrix reads at once lie in eight d
 };
 
 template <int DT, bool F8, int DP, int GT>
-__global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_mma_kernel(const Params p, int tiles, int split, int least) {
+__global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_mma_kernel(const Params p, const Plan plan) {
   using G = Geo<DT, F8, DP>;
   using P = MmaPlace<G::RB>;
   using T = typename Elem<DT>::type;
@@ -362,15 +414,15 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   float* s_merge = reinterpret_cast<float*>(smem);                       // over the rings when they are empty
   uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + G::RING_BYTES);     // [KS][32][AR]: A fragments
   __shared__ float s_up[16];                                             // power of two that a head's queries were multiplied by
-  const int units = p.HKV * tiles;
+  const int units = p.HKV * plan.tiles;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // (the merge waits for the whole of this grid)
 
-  Share sh{0, 0, 0, (int)(blockIdx.x / units)};
-  if (split && !find_share(p, units, G::ROUND, least, sh)) return;
+  Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
+  if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
   const int64_t share_first = sh.first;
 
   for (bool more = true; more;) {
-    const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
+    const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
     Feeder<G, P> feed(p, g, warp, lane);
     __syncthreads();
     feed.begin(ring);
@@ -564,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       }
     }
     __syncthreads();
-    more = end_segment<DT, DP, GT>(p, g, sh, share_first, units, split, s_merge);
+    more = end_segment<DT, DP, GT>(p, g, sh, share_first, units, plan, s_merge, s_merge + kWarps * GT * MS);
   }
 }
 
@@ -577,7 +629,7 @@ struct FmaPlace {   // the lanes of a quarter warp, LPK to a row, reach eight di
 };
 
 template <int DP, int GT>
-__global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_kernel(const Params p, int tiles, int split, int least) {
+__global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_kernel(const Params p, const Plan plan) {
   using G = FmaGeo<DP>;
   using P = FmaPlace<G::RB, G::LPK>;
   constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, MS = DP + 2;
@@ -586,16 +638,16 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
   float* s_merge = reinterpret_cast<float*>(smem);                   // over the rings when they are empty
   float* s_q = reinterpret_cast<float*>(smem + G::RING_BYTES);       // [GT][DP]
-  const int units = p.HKV * tiles;
+  const int units = p.HKV * plan.tiles;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  Share sh{0, 0, 0, (int)(blockIdx.x / units)};
-  if (split && !find_share(p, units, G::ROUND, least, sh)) return;
+  Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
+  if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
   const int64_t share_first = sh.first;
   const Logit logit(p, p.sm_scale);
 
   for (bool more = true; more;) {
-    const Segment g = segment_of(p, sh, tiles, units, split, G::ROUND, GT);
+    const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
     Feeder<G, P> feed(p, g, warp, lane);
     __syncthreads();
     feed.begin(ring);
@@ -698,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
       }
     }
     __syncthreads();
-    more = end_segment<HIPATTN_F32, DP, GT>(p, g, sh, share_first, units, split, s_merge);
+    more = end_segment<HIPATTN_F32, DP, GT>(p, g, sh, share_first, units, plan, s_merge, s_merge + kWarps * GT * MS);
   }
 }
 
@@ -736,12 +788,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       const float base = M > -INFINITY ? M : 0.f;
-      for (int c = c0 + lane; c <= c1; c += 32) den += exp2f(__ldcg(row(c) + DP) - base) * __ldcg(row(c) + DP + 1);
+      for (int c = c0 + lane; c <= c1; c += 32) den += ex2(__ldcg(row(c) + DP) - base) * __ldcg(row(c) + DP + 1);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
 #pragma unroll 4
       for (int c = c0 + sub; c <= c1; c += per_head) {
-        const float f = exp2f(__ldcg(row(c) + DP) - base);
+        const float f = ex2(__ldcg(row(c) + DP) - base);
 #pragma unroll
         for (int j = 0; j < VL; ++j) {
           if (V < 32 && lane >= V) continue;
@@ -768,83 +820,100 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   }
 }
 
-// How a call is laid out: head tiles, CTAs, whether units are cut
-struct Layout {
-  int gt, tiles, split, least;
-  int64_t ctas;
-};
-constexpr int kLeastRounds = 2;   // rounds of a share
+constexpr int kLeastRounds = 2;       // rounds of a share
+constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
+constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
-template <int DT, bool F8, int DP>
-Layout layout_of(const Params& p) {
-  Layout l;
-  const int heads = p.H / p.HKV;
-  if (DT == HIPATTN_F32) l.gt = heads <= 4 ? 4 : 8;
-  else l.gt = heads <= 8 ? 8 : 16;
-  l.tiles = cdiv(heads, l.gt);
-  const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
-  int64_t most = (int64_t)p.k.table_width * p.k.page_size;
-  if (p.window > 0 && p.window < most) most = p.window;
-  l.least = kLeastRounds;
-  l.split = most > (int64_t)l.least * Geo<DT, F8, DP>::ROUND;
-  l.ctas = l.split ? kSMs * Geo<DT, F8, DP>::CTAS : units;
-  return l;
-}
-template <int DP>
-int64_t scratch_bytes(const Layout& l) { return l.split ? l.ctas * 2 * l.gt * (DP + 4) * (int64_t)sizeof(float) : 0; }
-
 template <int DT, bool F8, int DP, int GT>
-int launch_gt(const Params& p, const Layout& l, cudaStream_t stream) {
+struct Kernel {
   using G = Geo<DT, F8, DP>;
-  constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP;
-  static_assert(sizeof(float) * kWarps * GT * (DP + 2) <= G::RING_BYTES, "the join of the warps lies over the rings");
-  HIPATTN_REQUIRE(l.ctas < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)l.ctas);
-  void (*kern)(const Params, int, int, int);
-  if constexpr (DT == HIPATTN_F32) kern = paged_decode_fma_kernel<DP, GT>;
-  else kern = paged_decode_mma_kernel<DT, F8, DP, GT>;
-  HIPATTN_CUDA_OK(allow_smem((const void*)kern, smem));
-  kern<<<(unsigned)l.ctas, kThreads, smem, stream>>>(p, l.tiles, l.split, l.least);
-  int rc = check_launch("paged_decode_kernel");
-  if (rc || !l.split) return rc;
-  cudaLaunchConfig_t cfg = {};
-  // few units have many parts each: one CTA per head then
-  const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
-  const int hb = units < kSMs ? 1 : GT, heads = p.H / p.HKV;
-  HIPATTN_REQUIRE(units < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)units);
-  cfg.gridDim = dim3((unsigned)units, (unsigned)cdiv(heads < GT ? heads : GT, hb));
-  cfg.blockDim = dim3(kMergeWarps * 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l.tiles, (int)l.ctas, (int)G::ROUND, l.least, hb));
-  return check_launch("paged_decode_merge_kernel");
-}
-
-// `stream` null with `bytes`: only the scratch of the call
-template <int DT, bool F8, int DP>
-int launch_dp(const Params& p, cudaStream_t stream, int64_t* bytes) {
-  const Layout l = layout_of<DT, F8, DP>(p);
-  const int64_t need = scratch_bytes<DP>(l);
-  if (bytes) {
-    *bytes = need;
-    return HIPATTN_OK;
+  static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP;
+  static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 2) <= G::RING_BYTES, "the join of the warps lies over the rings");
+  static void (*kern())(const Params, const Plan) {
+    if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT>;
+    else return paged_decode_mma_kernel<DT, F8, DP, GT>;
   }
-  HIPATTN_REQUIRE(need == 0 || (p.scratch && p.scratch_bytes >= need && (uintptr_t)p.scratch % 16 == 0), HIPATTN_ERR_INVALID,
-                  "paged_decode: %lld bytes of scratch are needed (16-byte aligned), %lld were given", (long long)need, (long long)p.scratch_bytes);
+  // How the call is laid out, and its CTAs.  Reads shapes and what the device holds.
+  static Plan plan(const Params& p, int64_t* ctas) {
+    Plan l;
+    l.tiles = cdiv(p.H / p.HKV, GT);
+    l.least = kLeastRounds;
+    l.split = 0;
+    l.cluster = 1;
+    const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
+    int64_t most = (int64_t)p.k.table_width * p.k.page_size;
+    if (p.window > 0 && p.window < most) most = p.window;
+    const int64_t rounds = (most + G::ROUND - 1) / G::ROUND;      // a unit has at most
+    // Few units that cannot be long: a cluster to each, joined in shared memory without a second launch
+    int64_t c = (int64_t)kSMs * G::CTAS / units;
+    if (c > kMaxCluster) c = kMaxCluster;
+    if (c > rounds) c = rounds;
+    if (c > 1 && rounds <= c * kClusterRounds && allow_smem((const void*)kern(), smem) == cudaSuccess) {
+      while (c > 1 && resident_clusters((const void*)kern(), (int)c, kThreads, smem) < units) --c;
+      if (c > 1 && rounds <= c * kClusterRounds) l.cluster = (int)c;
+    }
+    if (l.cluster == 1) l.split = rounds > l.least;
+    *ctas = l.split ? kSMs * G::CTAS : units * l.cluster;
+    return l;
+  }
+  static int64_t scratch(const Plan& l, int64_t ctas) { return l.split ? ctas * 2 * GT * (DP + 4) * (int64_t)sizeof(float) : 0; }
+
+  static int launch(const Params& p, cudaStream_t stream, int64_t* bytes) {
+    int64_t ctas;
+    const Plan l = plan(p, &ctas);
+    const int64_t need = scratch(l, ctas);
+    if (bytes) {      // only what the call needs
+      *bytes = need;
+      return HIPATTN_OK;
+    }
+    HIPATTN_REQUIRE(need == 0 || (p.scratch && p.scratch_bytes >= need && (uintptr_t)p.scratch % 16 == 0), HIPATTN_ERR_INVALID,
+                    "paged_decode: %lld bytes of scratch are needed (16-byte aligned), %lld were given", (long long)need, (long long)p.scratch_bytes);
+    const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
+    HIPATTN_REQUIRE(ctas < 0x7fffffffLL && units < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)ctas);
+    HIPATTN_CUDA_OK(allow_smem((const void*)kern(), smem));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = at;
+    if (l.cluster > 1) {
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = (unsigned)l.cluster;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.numAttrs = 1;
+    }
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern(), p, l));
+    const int rc = check_launch("paged_decode_kernel");
+    if (rc || !l.split) return rc;
+    // few units have many parts each: one CTA per head then
+    const int hb = units < kSMs ? 1 : GT, heads = p.H / p.HKV;
+    cfg.gridDim = dim3((unsigned)units, (unsigned)cdiv(heads < GT ? heads : GT, hb));
+    cfg.blockDim = dim3(kMergeWarps * 32);
+    cfg.dynamicSmemBytes = 0;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l.tiles, (int)ctas, (int)G::ROUND, l.least, hb));
+    return check_launch("paged_decode_merge_kernel");
+  }
+};
+
+// `bytes`: only the scratch of the call
+template <int DT, bool F8, int DP>
+int launch_heads(const Params& p, cudaStream_t stream, int64_t* bytes) {
   constexpr int SMALL = DT == HIPATTN_F32 ? 4 : 8;
-  return l.gt == SMALL ? launch_gt<DT, F8, DP, SMALL>(p, l, stream) : launch_gt<DT, F8, DP, SMALL * 2>(p, l, stream);
+  return p.H / p.HKV <= SMALL ? Kernel<DT, F8, DP, SMALL>::launch(p, stream, bytes) : Kernel<DT, F8, DP, SMALL * 2>::launch(p, stream, bytes);
 }
 template <int DT, bool F8>
 int launch_type(const Params& p, cudaStream_t stream, int64_t* bytes) {
   switch (padded_dim(p.D)) {
-    case 64: return launch_dp<DT, F8, 64>(p, stream, bytes);
-    case 128: return launch_dp<DT, F8, 128>(p, stream, bytes);
-    default: return launch_dp<DT, F8, 256>(p, stream, bytes);
+    case 64: return launch_heads<DT, F8, 64>(p, stream, bytes);
+    case 128: return launch_heads<DT, F8, 128>(p, stream, bytes);
+    default: return launch_heads<DT, F8, 256>(p, stream, bytes);
   }
 }
 int launch(const Params& p, cudaStream_t stream, int64_t* bytes) {
