@@ -94,13 +94,10 @@ struct Logit {
     cap = p.logit_softcap * kLog2e;
     k = p.logit_softcap > 0.f ? 2.f * kLog2e * scale / p.logit_softcap : kLog2e * scale;
   }
-  __device__ __forceinline__ float of(float x) const {
-    if (cap > 0.f) {
-      float r;
-      asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ex2(x * k) + 1.f));
-      return fmaf(-2.f * cap, r, cap);
-    }
-    return x * k;
+  __device__ __forceinline__ float capped(float x) const {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ex2(x * k) + 1.f));
+    return fmaf(-2.f * cap, r, cap);
   }
 };
 
@@ -292,79 +289,129 @@ __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, S
   return true;
 }
 
-// Asynchronous copies of a warp's keys into its ring.  Lane `key` looks up a key's page two rounds ahead of its copies and shares
-// out where its rows begin; a row that is not attended is sixteen zero bytes a piece (what lies there may be anything, NaN too).
+__device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_addr), "l"(gmem));
+}
+// A table entry as it lies: its low word, and the high word of an int64.
+struct Entry {
+  uint32_t lo = 0, hi = 0;
+};
+// Asynchronous copies of a warp's keys into its ring; a row that is not attended is sixteen zero bytes a piece (what lies there may be
+// anything, NaN too).  Lane `key` has a key's table entry fetched two rounds before its rows, into shared memory: a register that a load is
+// to fill stalls the warp when it is as much as moved (pages of one token: 206 us for 1.1 GB with entries in registers, XX so).
 template <class G, class Place>
 struct Feeder {
   const Params& p;
   const Segment& g;
   const char *kb, *vb;            // the KV head's rows
-  int64_t page = 0, page2 = 0;    // of this lane's key in the next round to be copied, and in the one after it
+  const char* table;              // the sequence's row of the table
+  uint32_t ring, entries;         // shared-memory addresses: [STAGES] stages, [4][KEYS] entries
   int page_size, page_shift, warp, lane, npc, most;
-  bool same;                      // K and V pools are laid out alike
-  __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_) : p(p_), g(g_), warp(warp_), lane(lane_) {
+  bool wide;                      // int64 entries
+  bool same, fast;                // K and V pools are laid out alike; and rows are whole and begin within 64 GB of the pool's beginning
+  __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_, const unsigned char* ring_, const unsigned char* entries_)
+      : p(p_), g(g_), warp(warp_), lane(lane_) {
+    ring = (uint32_t)__cvta_generic_to_shared(ring_);
+    entries = (uint32_t)__cvta_generic_to_shared(entries_) + (uint32_t)lane * 8;
     page_size = p.k.page_size;
     page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
     npc = p.D * G::EB / 16;
     most = (int)min((int64_t)p.k.table_width * page_size, (int64_t)0x7fff0000);
+    wide = p.k.table_is_i64 != 0;
+    table = (const char*)p.k.block_table + g.seq.row * p.k.table_stride_b * (wide ? 8 : 4);
     kb = (const char*)p.k.cache + (int64_t)g.hkv * p.k.stride_ch * G::EB;
     vb = (const char*)p.v.cache + (int64_t)g.hkv * p.v.stride_ch * G::EB;
     same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
+    fast = same && npc == G::NPC && p.k.n_pages * p.k.stride_page * G::EB < (int64_t)1 << 36;
   }
-  // (any entry of the table may be read, so that the first are on their way before the length is known; those behind the
-  // sequence's pages are not used)
-  __device__ __forceinline__ void fetch_page(int r, int lo) {
+  // The entry of this lane's key in round r.  (Any entry of the table may be read: the first are on their way before the length is
+  // known; those behind the sequence's pages are not used.)
+  __device__ __forceinline__ const char* entry_at(int r, int lo) const {
     const int t = lo + r * G::ROUND + warp * G::KEYS + lane;
-    page = page2;
-    page2 = 0;
-    if (lane < G::KEYS && t < most)
-      page2 = load_index(p.k.block_table, p.k.table_is_i64, g.seq.row * p.k.table_stride_b + (page_shift >= 0 ? t >> page_shift : t / page_size));
+    if (lane >= G::KEYS || t >= most) return nullptr;
+    return table + (int64_t)(page_shift >= 0 ? t >> page_shift : t / page_size) * (wide ? 8 : 4);
   }
-  __device__ __forceinline__ void copy(int r, unsigned char* stage) {
-    if (r < g.r1) {
-      const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS, live_keys = g.seq.hi - t0;
-      if (page < 0 || page >= p.k.n_pages) {
-        if (lane < live_keys) atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
-        page = 0;
-      }
-      const int t = t0 + lane, off = page_shift >= 0 ? t & (page_size - 1) : t % page_size;
-      const int64_t ko = (page * p.k.stride_page + (int64_t)off * p.k.stride_off) * G::EB;
-      const int64_t vo = same ? ko : (page * p.v.stride_page + (int64_t)off * p.v.stride_off) * G::EB;
-      const uint32_t ks = (uint32_t)__cvta_generic_to_shared(stage), vs = ks + G::KEYS * G::RB;
+  __device__ __forceinline__ Entry load_entry(int r, int lo) const {
+    Entry e;
+    if (const char* at = entry_at(r, lo)) {
+      e.lo = __ldg((const uint32_t*)at);
+      if (wide) e.hi = __ldg((const uint32_t*)at + 1);
+    }
+    return e;
+  }
+  __device__ __forceinline__ void fetch_entry(int r) const {
+    if (const char* at = entry_at(r, g.seq.lo)) {
+      const uint32_t to = entries + (uint32_t)(r & 3) * (G::KEYS * 8);
+      if (wide) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(at));
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(at));
+    }
+  }
+  __device__ __forceinline__ Entry fetched_entry(int r) const {
+    Entry e;
+    if (lane < G::KEYS) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(e.lo), "=r"(e.hi) : "r"(entries + (uint32_t)(r & 3) * (G::KEYS * 8)) : "memory");
+    return e;
+  }
+  __device__ __forceinline__ void copy(int r, int slot, const Entry& e) const {
+    if (r >= g.r1) return;
+    const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS, live_keys = g.seq.hi - t0;
+    uint32_t page = e.lo;
+    if (page >= (uint32_t)p.k.n_pages || (wide && e.hi != 0)) {
+      if (lane < min(live_keys, G::KEYS)) atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
+      page = 0;
+    }
+    const int t = t0 + lane, off = page_shift >= 0 ? t & (page_size - 1) : t % page_size;
+    const uint32_t ks = ring + (uint32_t)slot * G::STAGE_BYTES;
+    if (fast && live_keys >= G::KEYS) {      // most rounds: no row to leave out, offsets in units of 16 bytes
+      const uint32_t at = page * (uint32_t)(p.k.stride_page * G::EB / 16) + (uint32_t)off * (uint32_t)(p.k.stride_off * G::EB / 16);
 #pragma unroll
       for (int i = 0; i < G::KEYS * G::NPC / 32; ++i) {
         const int idx = i * 32 + lane, key = idx / G::NPC, pc = idx % G::NPC;
-        const int64_t k0 = __shfl_sync(0xffffffffu, ko, key);
-        const int64_t v0 = same ? k0 : __shfl_sync(0xffffffffu, vo, key);
-        // (a key that is not attended has the address of a row of page 0, which is not read)
-        const bool live = key < live_keys && pc < npc;
-        const int at = pc < npc ? pc * 16 : 0;
-        cp_async16_zfill(ks + Place::at(key, pc), kb + at + k0, live);
-        cp_async16_zfill(vs + Place::at(key, pc), vb + at + v0, live);
+        const uint64_t row = (uint64_t)__shfl_sync(0xffffffffu, at, key) * 16;
+        const uint32_t to = ks + Place::at(key, pc);
+        cp_async16(to, kb + pc * 16 + row);
+        cp_async16(to + G::KEYS * G::RB, vb + pc * 16 + row);
       }
+      return;
     }
+    const int64_t ko = ((int64_t)page * p.k.stride_page + (int64_t)off * p.k.stride_off) * G::EB;
+    const int64_t vo = same ? ko : ((int64_t)page * p.v.stride_page + (int64_t)off * p.v.stride_off) * G::EB;
+#pragma unroll
+    for (int i = 0; i < G::KEYS * G::NPC / 32; ++i) {
+      const int idx = i * 32 + lane, key = idx / G::NPC, pc = idx % G::NPC;
+      const int64_t k0 = __shfl_sync(0xffffffffu, ko, key);
+      const int64_t v0 = same ? k0 : __shfl_sync(0xffffffffu, vo, key);
+      // (a key that is not attended has the address of a row of page 0, which is not read)
+      const bool live = key < live_keys && pc < npc;
+      const int piece = pc < npc ? pc * 16 : 0;
+      const uint32_t to = ks + Place::at(key, pc);
+      cp_async16_zfill(to, kb + piece + k0, live);
+      cp_async16_zfill(to + G::KEYS * G::RB, vb + piece + v0, live);
+    }
+  }
+  // the first two rounds of a segment on their way, and the entries of the two after them
+  __device__ __forceinline__ void begin() const {
+    static_assert(G::STAGES == 3, "two rounds of rows in flight, entries for two more");
+    Entry e0, e1;
+    if (p.window > 0) {
+      e0 = load_entry(g.r0, g.seq.lo);
+      e1 = load_entry(g.r0 + 1, g.seq.lo);
+    } else {
+      e0 = load_entry(g.r0, 0);
+      e1 = load_entry(g.r0 + 1, 0);
+    }
+    fetch_entry(g.r0 + 2);
+    fetch_entry(g.r0 + 3);
+    copy(g.r0, 0, e0);
+    cp_async_commit();
+    copy(g.r0 + 1, 1, e1);
     cp_async_commit();
   }
-  // the first rounds of a segment on their way
-  __device__ __forceinline__ void begin(unsigned char* ring) {
-    if (p.window > 0) {
-      fetch_page(g.r0, g.seq.lo);
-      fetch_page(g.r0 + 1, g.seq.lo);
-    } else {
-      fetch_page(g.r0, 0);
-      fetch_page(g.r0 + 1, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < G::STAGES - 1; ++i) {
-      copy(g.r0 + i, ring + i * G::STAGE_BYTES);
-      fetch_page(g.r0 + i + 2, g.seq.lo);
-    }
-  }
-  // round r is done: its place in the ring goes to round r + STAGES - 1
-  __device__ __forceinline__ void next(int r, unsigned char* ring, int& slot) {
-    copy(r + G::STAGES - 1, ring + (slot == 0 ? G::STAGES - 1 : slot - 1) * G::STAGE_BYTES);
-    fetch_page(r + G::STAGES + 1, g.seq.lo);
-    slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+  // round r, in place `slot` of the ring, is done: the place before it goes to round r + 2
+  __device__ __forceinline__ void next(int r, int& slot) const {
+    copy(r + 2, slot == 0 ? 2 : slot - 1, fetched_entry(r + 2));
+    fetch_entry(r + 4);
+    cp_async_commit();
+    slot = slot == 2 ? 0 : slot + 1;
   }
 };
 
@@ -395,6 +442,13 @@ __device__ __forceinline__ float upper(uint32_t w) {
   return MT == HIPATTN_BF16 ? __uint_as_float(w & 0xffff0000u) : __high2float(*reinterpret_cast<const __half2*>(&w));
 }
 
+__device__ __forceinline__ void ldsm_x4_at(uint32_t* r, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm_x4_t_at(uint32_t* r, uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+
 template <int RB>
 struct MmaPlace {   // the eight rows that ldmatrix reads at once lie in eight different groups of banks
   __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ (RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1))) << 4); }
@@ -408,11 +462,12 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   constexpr int MT = F8 ? HIPATTN_F16 : DT;          // type of the products
   constexpr int KEYS = G::KEYS, MS = DP + 2, KS = DP / 16, NT = DP / 8, AR = GT / 4;   // AR: registers of an A fragment that are not padding
   constexpr float kShift = MT == HIPATTN_F16 ? 14.f : 0.f;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, jq = lane & 3;
   unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
   float* s_merge = reinterpret_cast<float*>(smem);                       // over the rings when they are empty
   uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + G::RING_BYTES);     // [KS][32][AR]: A fragments
+  const unsigned char* entries = smem + G::RING_BYTES + 2 * GT * DP + warp * (4 * KEYS * 8);
   __shared__ float s_up[16];                                             // power of two that a head's queries were multiplied by
   const int units = p.HKV * plan.tiles;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // (the merge waits for the whole of this grid)
@@ -420,12 +475,15 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
   if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
   const int64_t share_first = sh.first;
+  // rows and pieces of ldmatrix: 16-bit K eight keys by two pieces twice, fp8 K a piece of all keys or two of sixteen, V sixteen keys by two
+  const uint32_t k_lane = F8 ? (KEYS == 32 ? P::at(lane, 0) : P::at(lane & 15, lane >> 4)) : P::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
+  const uint32_t v_lane = KEYS * G::RB + P::at(lane & 15, lane >> 4);
 
   for (bool more = true; more;) {
     const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
-    Feeder<G, P> feed(p, g, warp, lane);
+    const Feeder<G, P> feed(p, g, warp, lane, ring, entries);
     __syncthreads();
-    feed.begin(ring);
+    feed.begin();
 
     // ---- the unit's queries ----
     const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)sh.b * p.q_stride_b + (int64_t)g.h0 * p.q_stride_h;
@@ -470,8 +528,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       for (int r = g.r0; r < g.r1; ++r) {
         cp_async_wait<G::STAGES - 2>();
         __syncwarp();
-        const unsigned char* ks = ring + slot * G::STAGE_BYTES;
-        const unsigned char* vs = ks + KEYS * G::RB;
+        // this lane's row and first piece in K and in V; piece j further is the address xor 16 j (a row begins on a multiple of its size)
+        const uint32_t ks = feed.ring + slot * G::STAGE_BYTES + k_lane, vs = feed.ring + slot * G::STAGE_BYTES + v_lane;
         // ---- S = Q K^T ----
         uint32_t kept[4];
         float s[KEYS / 8][4];
@@ -490,9 +548,9 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           if constexpr (F8) {
             uint32_t b[4];
             if constexpr (KEYS == 32) {
-              ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(lane, k));
+              ldsm_x4_at(b, ks ^ (k << 4));
             } else {                                   // two pieces of 16 keys
-              if ((k & 1) == 0) ldsm_x4(kept[0], kept[1], kept[2], kept[3], ks + P::at(lane & 15, k + (lane >> 4)));
+              if ((k & 1) == 0) ldsm_x4_at(kept, ks ^ (k << 4));
               b[0] = kept[(k & 1) * 2];
               b[1] = kept[(k & 1) * 2 + 1];
             }
@@ -502,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
             for (int n = 0; n < KEYS / 8; n += 2) {
               uint32_t b[4];
-              ldsm_x4(b[0], b[1], b[2], b[3], ks + P::at(n * 8 + (lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)));
+              ldsm_x4_at(b, (ks ^ (k << 5)) + n * 8 * G::RB);
               mma16816<MT>(s[n], a, b[0], b[1]);
               mma16816<MT>(s[n + 1], a, b[2], b[3]);
             }
@@ -516,16 +574,28 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         float alpha[GT / 8];
 #pragma unroll
         for (int i = 0; i < GT / 8; ++i) {
-          float mx = -INFINITY;
+          const Logit& logit = i ? logit1 : logit0;
+          if (logit.cap > 0.f) {
 #pragma unroll
-          for (int n = 0; n < KEYS / 8; ++n)
+            for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = (i ? logit1 : logit0).of(s[n][2 * i + e]);
-              if (tail && t0 + n * 8 + e >= g.seq.hi) x = -INFINITY;
-              s[n][2 * i + e] = x;
-              mx = fmaxf(mx, x);
-            }
+              for (int e = 0; e < 2; ++e) s[n][2 * i + e] = logit.capped(s[n][2 * i + e]);
+          } else {
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) s[n][2 * i + e] *= logit.k;
+          }
+          if (tail) {
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (t0 + n * 8 + e >= g.seq.hi) s[n][2 * i + e] = -INFINITY;
+          }
+          float mx = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+          for (int n = 1; n < KEYS / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float m_new = fmaxf(m_run[i], mx), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
@@ -562,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
           for (int pc = 0; pc < G::NPC; pc += 2) {
             uint32_t b[4];
-            ldsm_x4_t(b[0], b[1], b[2], b[3], vs + P::at(c * 16 + (lane & 15), pc + (lane >> 4)));
+            ldsm_x4_t_at(b, (vs ^ (pc << 4)) + c * 16 * G::RB);
             if constexpr (F8) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -576,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           }
         }
         __syncwarp();
-        feed.next(r, ring, slot);
+        feed.next(r, slot);
       }
       cp_async_wait<0>();
       if constexpr (GT == 8) {
@@ -595,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           for (int e = 0; e < 4; ++e) nan |= o[n][e] != o[n][e];
         if (!two || !__any_sync(0xffffffffu, nan)) break;
         __syncwarp();
-        feed.begin(ring);
+        feed.begin();
       }
     }
     __syncthreads();
@@ -633,11 +703,12 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   using G = FmaGeo<DP>;
   using P = FmaPlace<G::RB, G::LPK>;
   constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, MS = DP + 2;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
   float* s_merge = reinterpret_cast<float*>(smem);                   // over the rings when they are empty
   float* s_q = reinterpret_cast<float*>(smem + G::RING_BYTES);       // [GT][DP]
+  const unsigned char* entries = smem + G::RING_BYTES + 4 * GT * DP + warp * (4 * KEYS * 8);
   const int units = p.HKV * plan.tiles;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
@@ -648,9 +719,9 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
 
   for (bool more = true; more;) {
     const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
-    Feeder<G, P> feed(p, g, warp, lane);
+    const Feeder<G, P> feed(p, g, warp, lane, ring, entries);
     __syncthreads();
-    feed.begin(ring);
+    feed.begin();
     for (int i = tid; i < GT * DP; i += kThreads) {
       const int h = i / DP, e = i % DP;
       float x = 0.f;
@@ -694,7 +765,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
       for (int h = 0; h < GT; ++h) {
 #pragma unroll
         for (int o = LPK >> 1; o > 0; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-        s[h] = in ? logit.of(s[h]) : -INFINITY;
+        s[h] = in ? (logit.cap > 0.f ? logit.capped(s[h]) : s[h] * logit.k) : -INFINITY;
         float mx = s[h];
 #pragma unroll
         for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -726,7 +797,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
         }
       }
       __syncwarp();
-      feed.next(r, ring, slot);
+      feed.next(r, slot);
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -823,13 +894,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
 constexpr int kLeastRounds = 2;       // rounds of a share
 constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
 constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
+constexpr int kWholeRounds = 32;      // most rounds of a unit that is a CTA's
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
 template <int DT, bool F8, int DP, int GT>
 struct Kernel {
   using G = Geo<DT, F8, DP>;
-  static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP;
+  static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP + kWarps * 4 * G::KEYS * 8;
   static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 2) <= G::RING_BYTES, "the join of the warps lies over the rings");
   static void (*kern())(const Params, const Plan) {
     if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT>;
@@ -854,7 +926,7 @@ struct Kernel {
       while (c > 1 && resident_clusters((const void*)kern(), (int)c, kThreads, smem) < units) --c;
       if (c > 1 && rounds <= c * kClusterRounds) l.cluster = (int)c;
     }
-    if (l.cluster == 1) l.split = rounds > l.least;
+    if (l.cluster == 1) l.split = rounds > kWholeRounds;
     *ctas = l.split ? kSMs * G::CTAS : units * l.cluster;
     return l;
   }
