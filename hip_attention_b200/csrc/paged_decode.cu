@@ -89,16 +89,18 @@ __device__ __forceinline__ float ex2(float x) {
 // off by a few 2^-24 everywhere, which is what counts in a logit, in five instructions (tanhf, whose relative error is as small
 // near zero, and a division by the cap: 12 fp8 sequences with a soft-cap 268 us, XX so).
 struct Logit {
-  float k, cap;      // cap 0: none; else k = 2 log2 e scale / cap, cap = log2 e cap
+  float k, cap;      // cap 0: none; else k = 2 log2 e scale / cap, cap = log2 e cap.  k is positive: queries are multiplied by `sign` before
   __device__ __forceinline__ Logit(const Params& p, float scale) {
+    const float size = scale == 0.f ? 1.f : fabsf(scale);
     cap = p.logit_softcap * kLog2e;
-    k = p.logit_softcap > 0.f ? 2.f * kLog2e * scale / p.logit_softcap : kLog2e * scale;
+    k = p.logit_softcap > 0.f ? 2.f * kLog2e * size / p.logit_softcap : kLog2e * size;
   }
   __device__ __forceinline__ float capped(float x) const {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ex2(x * k) + 1.f));
     return fmaf(-2.f * cap, r, cap);
   }
+  __device__ static __forceinline__ float sign(const Params& p) { return p.sm_scale > 0.f ? 1.f : (p.sm_scale < 0.f ? -1.f : 0.f); }
 };
 
 // element e of the output row of head h, from the joined maximum (base 2), numerator and denominator
@@ -116,12 +118,12 @@ struct Geo {
   static constexpr int EB = F8 ? 1 : Elem<DT>::bytes;
   static constexpr int RB = DP * EB;
   static constexpr int NPC = RB / 16;                         // pieces of a row
-  static constexpr int KEYS = DT == HIPATTN_F32 ? 4096 / RB : (RB == 64 ? 32 : 16);
+  static constexpr int KEYS = DT == HIPATTN_F32 ? 4096 / RB : (RB <= 128 ? 32 : 16);
   static constexpr int STAGES = 3;
   static constexpr int ROUND = KEYS * kWarps;
   static constexpr int STAGE_BYTES = 2 * KEYS * RB;
   static constexpr int RING_BYTES = STAGES * STAGE_BYTES * kWarps;
-  static constexpr int CTAS = 200 * 1024 / RING_BYTES;        // per multiprocessor: 4, 2 or 1
+  static constexpr int CTAS = RB == 64 ? 3 : 200 * 1024 / RING_BYTES;        // per multiprocessor: 3, 2 or 1
 };
 template <int DP>
 struct FmaGeo : Geo<HIPATTN_F32, false, DP> {
@@ -296,14 +298,21 @@ __device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void* gmem)
 struct Entry {
   uint32_t lo = 0, hi = 0;
 };
+// Where piece `pc` of row `key` of a tile lies: rows of RB bytes, their pieces turned by Kind::turn(key), which is an xor of its bits
+template <int RB, class Kind>
+struct Place {
+  __device__ static __forceinline__ constexpr int at(int key, int pc) { return key * RB + ((pc ^ Kind::turn(key)) << 4); }
+};
 // Asynchronous copies of a warp's keys into its ring; a row that is not attended is sixteen zero bytes a piece (what lies there may be
 // anything, NaN too).  Lane `key` has a key's table entry fetched two rounds before its rows, into shared memory: a register that a load is
 // to fill stalls the warp when it is as much as moved (pages of one token: 206 us for 1.1 GB with entries in registers, XX so).
-template <class G, class Place>
+template <class G, class At>
 struct Feeder {
   const Params& p;
   const Segment& g;
   const char *kb, *vb;            // the KV head's rows
+  const char *k_piece, *v_piece;  // and this lane's piece of them
+  uint32_t lane_at;               // where this lane's piece of a stage's first rows lies
   const char* table;              // the sequence's row of the table
   uint32_t ring, entries;         // shared-memory addresses: [STAGES] stages, [4][KEYS] entries
   int page_size, page_shift, warp, lane, npc, most;
@@ -321,6 +330,9 @@ struct Feeder {
     table = (const char*)p.k.block_table + g.seq.row * p.k.table_stride_b * (wide ? 8 : 4);
     kb = (const char*)p.k.cache + (int64_t)g.hkv * p.k.stride_ch * G::EB;
     vb = (const char*)p.v.cache + (int64_t)g.hkv * p.v.stride_ch * G::EB;
+    k_piece = kb + lane % G::NPC * 16;
+    v_piece = vb + lane % G::NPC * 16;
+    lane_at = At::at(G::NPC < 32 ? lane / G::NPC : 0, lane % G::NPC);
     same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
     fast = same && npc == G::NPC && p.k.n_pages * p.k.stride_page * G::EB < (int64_t)1 << 36;
   }
@@ -365,11 +377,13 @@ struct Feeder {
       const uint32_t at = page * (uint32_t)(p.k.stride_page * G::EB / 16) + (uint32_t)off * (uint32_t)(p.k.stride_off * G::EB / 16);
 #pragma unroll
       for (int i = 0; i < G::KEYS * G::NPC / 32; ++i) {
-        const int idx = i * 32 + lane, key = idx / G::NPC, pc = idx % G::NPC;
-        const uint64_t row = (uint64_t)__shfl_sync(0xffffffffu, at, key) * 16;
-        const uint32_t to = ks + Place::at(key, pc);
-        cp_async16(to, kb + pc * 16 + row);
-        cp_async16(to + G::KEYS * G::RB, vb + pc * 16 + row);
+        // lane's row and piece of the first copy; those of copy i are `first` rows further
+        constexpr int ROWS = G::NPC < 32 ? 32 / G::NPC : 1;
+        const int first = G::NPC > 32 ? i / (G::NPC / 32) : i * ROWS, pc0 = G::NPC > 32 ? i % (G::NPC / 32) * 32 : 0;
+        const uint64_t row = (uint64_t)__shfl_sync(0xffffffffu, at, first + (G::NPC < 32 ? lane / G::NPC : 0)) * 16 + pc0 * 16;
+        const uint32_t to = ((ks + lane_at) ^ (At::turn(first) << 4)) + first * G::RB + pc0 * 16;
+        cp_async16(to, k_piece + row);
+        cp_async16(to + G::KEYS * G::RB, v_piece + row);
       }
       return;
     }
@@ -383,7 +397,7 @@ struct Feeder {
       // (a key that is not attended has the address of a row of page 0, which is not read)
       const bool live = key < live_keys && pc < npc;
       const int piece = pc < npc ? pc * 16 : 0;
-      const uint32_t to = ks + Place::at(key, pc);
+      const uint32_t to = ks + At::at(key, pc);
       cp_async16_zfill(to, kb + piece + k0, live);
       cp_async16_zfill(to + G::KEYS * G::RB, vb + piece + v0, live);
     }
@@ -450,8 +464,8 @@ __device__ __forceinline__ void ldsm_x4_t_at(uint32_t* r, uint32_t a) {
 }
 
 template <int RB>
-struct MmaPlace {   // the eight rows that ldmatrix reads at once lie in eight different groups of banks
-  __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ (RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1))) << 4); }
+struct MmaPlace : Place<RB, MmaPlace<RB>> {   // the eight rows that ldmatrix reads at once lie in eight different groups of banks
+  __device__ static __forceinline__ constexpr int turn(int key) { return RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1); }
 };
 
 template <int DT, bool F8, int DP, int GT>
@@ -501,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       }
       __syncthreads();
     }
+    const float sign = Logit::sign(p);
     for (int i = tid; i < KS * 32 * AR; i += kThreads) {
       // register r of lane l: row l / 4 (+ 8), elements 2 (l % 4) .. (+ 8) of a step; with fp8 rows 4 (l % 4) .. (+ 2)
       const int r = i % AR, l = i / AR % 32, ks = i / AR / 32;
@@ -510,7 +525,10 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       if (row < g.live_heads) {
         if (e < p.D) lo = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e]);
         if (e + 1 < p.D) hi = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e + 1]);
-        if constexpr (F8 && DT == HIPATTN_BF16) { lo *= s_up[row]; hi *= s_up[row]; }
+        float up = sign;
+        if constexpr (F8 && DT == HIPATTN_BF16) up *= s_up[row];
+        lo *= up;
+        hi *= up;
       }
       s_q[i] = pack2<MT>(lo, hi);
     }
@@ -575,16 +593,13 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
         for (int i = 0; i < GT / 8; ++i) {
           const Logit& logit = i ? logit1 : logit0;
+          float k = logit.k;      // logits are s k
           if (logit.cap > 0.f) {
 #pragma unroll
             for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) s[n][2 * i + e] = logit.capped(s[n][2 * i + e]);
-          } else {
-#pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) s[n][2 * i + e] *= logit.k;
+            k = 1.f;
           }
           if (tail) {
 #pragma unroll
@@ -598,12 +613,12 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           for (int n = 1; n < KEYS / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m_run[i], mx), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
+          const float m_new = fmaxf(m_run[i], mx * k), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
           alpha[i] = ex2(m_run[i] - base - kShift);
           float sum = 0.f;
 #pragma unroll
           for (int n = 0; n < KEYS / 8; ++n) {
-            const float x = ex2(s[n][2 * i] - base), y = ex2(s[n][2 * i + 1] - base);
+            const float x = ex2(fmaf(s[n][2 * i], k, -base)), y = ex2(fmaf(s[n][2 * i + 1], k, -base));
             sum += x + y;
             const uint32_t hi = pack2<MT>(x, y), lo = pack2<MT>(x - lower<MT>(hi), y - upper<MT>(hi));
             pa[n / 2][(n & 1) * 2 + i] = hi;
@@ -694,8 +709,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 // fp32: FMA.  LPK lanes to a key for the logits, a lane owns columns of the output.
 // ---------------------------------------------------------------------------------------------------
 template <int RB, int LPK>
-struct FmaPlace {   // the lanes of a quarter warp, LPK to a row, reach eight different groups of banks
-  __device__ static __forceinline__ int at(int key, int pc) { return key * RB + ((pc ^ ((key * LPK) & 7)) << 4); }
+struct FmaPlace : Place<RB, FmaPlace<RB, LPK>> {   // the lanes of a quarter warp, LPK to a row, reach eight different groups of banks
+  __device__ static __forceinline__ constexpr int turn(int key) { return (key * LPK) & 7; }
 };
 
 template <int DP, int GT>
@@ -725,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
     for (int i = tid; i < GT * DP; i += kThreads) {
       const int h = i / DP, e = i % DP;
       float x = 0.f;
-      if (h < g.live_heads && e < p.D) x = reinterpret_cast<const float*>(p.q)[(int64_t)sh.b * p.q_stride_b + (int64_t)(g.h0 + h) * p.q_stride_h + e];
+      if (h < g.live_heads && e < p.D) x = reinterpret_cast<const float*>(p.q)[(int64_t)sh.b * p.q_stride_b + (int64_t)(g.h0 + h) * p.q_stride_h + e] * Logit::sign(p);
       s_q[i] = x;
     }
     __syncthreads();
