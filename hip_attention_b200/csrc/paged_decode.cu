@@ -28,21 +28,30 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
 // sequence of entry b: its row of the table and the positions [lo, hi) it attends
 struct Sequence {
   int64_t row;
+  bool there;     // the row is in the table (else it is read as row 0, and empty)
   int lo, hi;
 };
-__device__ __forceinline__ Sequence sequence_of(const Params& p, int b, bool report) {
-  Sequence s{0, 0, 0};
+__device__ __forceinline__ Sequence row_of(const Params& p, int b, bool report) {
+  Sequence s{0, true, 0, 0};
   s.row = p.rows ? load_index(p.rows, p.rows_is_i64, b) : b;
   if (s.row < 0 || s.row >= p.n_rows) {
     if (report && s.row >= p.n_rows) atomicOr(p.status, HIPATTN_STATUS_SEQUENCE);
     s.row = 0;
-    return s;
+    s.there = false;
   }
+  return s;
+}
+__device__ __forceinline__ void read_length(const Params& p, Sequence& s, bool report) {
   const int64_t n = load_index(p.k.cache_seq_lens, p.k.seq_lens_is_i64, s.row);
   const int64_t most = min((int64_t)p.k.table_width * p.k.page_size, (int64_t)0x7fff0000);
+  if (!s.there) return;
   if (report && n > most) atomicOr(p.status, HIPATTN_STATUS_TOKEN_RANGE);
   s.hi = (int)max((int64_t)0, min(n, most));
   s.lo = p.window > 0 ? max(0, s.hi - p.window) : 0;
+}
+__device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
+  Sequence s = row_of(p, b, false);
+  read_length(p, s, false);
   return s;
 }
 // rounds of a unit; an empty sequence has one, which writes its zeros
@@ -53,7 +62,7 @@ template <int THREADS>
 __device__ __forceinline__ void sum_rounds(const Params& p, int b, int round, int64_t* s_sum, int64_t& total, int64_t& before) {
   int64_t t = 0, f = 0;
   for (int i = threadIdx.x; i < p.B; i += THREADS) {
-    const int r = rounds_of(sequence_of(p, i, false), round);
+    const int r = rounds_of(sequence_of(p, i), round);
     t += r;
     if (i < b) f += r;
   }
@@ -103,13 +112,29 @@ struct Logit {
   __device__ static __forceinline__ float sign(const Params& p) { return p.sm_scale > 0.f ? 1.f : (p.sm_scale < 0.f ? -1.f : 0.f); }
 };
 
-// element e of the output row of head h, from the joined maximum (base 2), numerator and denominator
+// How a call is laid out.  split: every CTA takes a share of the row of rounds.  Else a unit is a CTA's, or a cluster's.
+struct Plan {
+  int tiles, split, least, cluster;   // head tiles of a KV head; rounds that a share has at least
+  int vector_out;                     // output rows begin where four elements can be stored at once
+};
+
+// Columns 4 v .. 4 v + 3 of the output row of head h, from the joined maximum (base 2), numerators and denominator
 template <int DT>
-__device__ __forceinline__ void finish(const Params& p, int b, int h, int e, float M, float num, float den) {
+__device__ __forceinline__ void finish(const Params& p, const Plan& plan, int b, int h, int v, float M, const float4& num, float den) {
+  using T = typename Elem<DT>::type;
   // (a denominator of exactly zero: nothing was attended.  NaN and infinite logits stay visible.)
   const bool none = den == 0.f;
-  reinterpret_cast<typename Elem<DT>::type*>(p.out)[(int64_t)b * p.o_stride_b + (int64_t)h * p.o_stride_h + e] = Elem<DT>::from_f32(none ? 0.f : num / den);
-  if (e == 0 && p.lse_out) p.lse_out[(int64_t)b * p.H + h] = none ? -INFINITY : (M > -INFINITY ? M : 0.f) + log2f(den);
+  const float r = none ? 0.f : 1.f / den;
+  T* out = reinterpret_cast<T*>(p.out) + (int64_t)b * p.o_stride_b + (int64_t)h * p.o_stride_h + v * 4;
+  const float x[4] = {none ? 0.f : num.x * r, none ? 0.f : num.y * r, none ? 0.f : num.z * r, none ? 0.f : num.w * r};
+  if (plan.vector_out) {
+    if constexpr (DT == HIPATTN_F32) *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<uint2*>(out) = make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = Elem<DT>::from_f32(x[e]);
+  }
+  if (v == 0 && p.lse_out) p.lse_out[(int64_t)b * p.H + h] = none ? -INFINITY : (M > -INFINITY ? M : 0.f) + log2f(den);
 }
 
 // Geometry of the kernels: RB = bytes of a row of DP elements, KEYS = keys a warp takes at once, STAGES = depth of its ring
@@ -133,11 +158,6 @@ struct FmaGeo : Geo<HIPATTN_F32, false, DP> {
   static constexpr int KP = B::NPC < 32 ? 32 / B::NPC : 1;          // V rows that a warp reads at once
 };
 
-// How a call is laid out.  split: every CTA takes a share of the row of rounds.  Else a unit is a CTA's, or a cluster's.
-struct Plan {
-  int tiles, split, least, cluster;   // head tiles of a KV head; rounds that a share has at least
-};
-
 // A CTA's share of the row of rounds
 struct Share {
   int64_t first, last, unit_at;   // [first, last): what is left of it; where sequence b begins in the row
@@ -152,7 +172,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int units, int round
   // rounds of sequence c + tid (x) and of those of [c, c + tid] (sum); the sum over the CTA is returned
   auto scan = [&](int c, int turn) {
     const int i = c + tid;
-    x = sum = i < p.B ? rounds_of(sequence_of(p, i, false), round) : 0;
+    x = sum = i < p.B ? rounds_of(sequence_of(p, i), round) : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
@@ -190,96 +210,103 @@ __device__ __forceinline__ bool find_share(const Params& p, int units, int round
   return true;
 }
 
-// The rounds [r0, r1) of one unit that a CTA works on next
+// What a CTA works on next: rounds [r0, r1) of one unit, `step` keys apart, round 0 beginning at key `lo`.  The CTAs of a cluster take
+// its rounds in turn.
 struct Segment {
   Sequence seq;
-  int rounds, r0, r1, hkv, h0, live_heads;
+  int rounds, r0, r1, lo, step, hkv, h0, live_heads;
 };
-__device__ __forceinline__ Segment segment_of(const Params& p, const Share& sh, const Plan& plan, int units, int round, int gt) {
-  Segment g;
-  g.seq = sequence_of(p, sh.b, threadIdx.x == 0);
-  g.rounds = rounds_of(g.seq, round);
-  const int tiles = plan.tiles, rank = blockIdx.x % plan.cluster, per = (g.rounds + plan.cluster - 1) / plan.cluster;
-  int u = blockIdx.x / plan.cluster % units;
-  g.r0 = min(g.rounds, rank * per);
-  g.r1 = min(g.rounds, g.r0 + per);
-  if (plan.split) {
-    u = (int)((sh.first - sh.unit_at) / g.rounds);
-    g.r0 = (int)((sh.first - sh.unit_at) % g.rounds);
-    g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
-  }
+__device__ __forceinline__ void set_unit(const Params& p, Segment& g, int u, int tiles, int gt) {
   const int heads = p.H / p.HKV, tile = u % tiles;
   g.hkv = u / tiles;
   g.h0 = g.hkv * heads + tile * gt;
   g.live_heads = min(gt, heads - tile * gt);
-  return g;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {   // the same shared-memory address in CTA `rank` of the cluster
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {   // the same shared-memory address in CTA `rank` of the cluster
   uint32_t a;
-  float v;
+  float4 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
 }
 
-// The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 2]: to the output, to scratch, or (a cluster) to s_cta [GT][DP + 2],
-// where the CTAs of the cluster read one another's and each finishes some of the outputs.  Returns whether more is to come.
+// The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 4]: to the output, to scratch, or (a cluster) to s_cta [GT][DP + 4],
+// which the CTAs of the cluster read together: as many lanes as there are CTAs to four columns, each finishing some of them.  Returns
+// whether more is to come.
 template <int DT, int DP, int GT>
 __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, Share& sh, int64_t share_first, int units, const Plan& plan, const float* s_merge,
                                             float* s_cta) {
-  constexpr int MS = DP + 2, PS = DP + 4;
+  constexpr int MS = DP + 4, V = DP / 4;
   const bool whole = plan.split ? g.r0 == 0 && g.r1 == g.rounds : plan.cluster == 1;
   float* part = s_cta;
-  int stride = MS;
-  if (plan.split) {
-    part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * PS;
-    stride = PS;
-  }
-  for (int i = threadIdx.x; i < g.live_heads * p.D; i += kThreads) {
-    const int h = i / p.D, e = i % p.D;
-    float M = -INFINITY;
+  if (plan.split) part = reinterpret_cast<float*>(p.scratch) + ((int64_t)blockIdx.x * 2 + (sh.first == share_first ? 0 : 1)) * GT * MS;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_merge[(w * GT + h) * MS + DP]);
-    const float base = M > -INFINITY ? M : 0.f;
-    float num = 0.f, den = 0.f;
+  for (int i0 = 0; i0 < GT * V; i0 += kThreads) {
+    const int i = i0 + threadIdx.x, h = i / V, v = i % V;
+    if (h >= g.live_heads || v * 4 >= p.D) continue;
+    float m[kWarps], M = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2(s_merge[(w * GT + h) * MS + DP] - base);
-      num += f * s_merge[(w * GT + h) * MS + e];
+      m[w] = s_merge[(w * GT + h) * MS + DP];
+      M = fmaxf(M, m[w]);
+    }
+    const float base = M > -INFINITY ? M : 0.f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(m[w] - base);
+      const float4 x = *reinterpret_cast<const float4*>(s_merge + (w * GT + h) * MS + v * 4);
+      num.x += f * x.x;
+      num.y += f * x.y;
+      num.z += f * x.z;
+      num.w += f * x.w;
       den += f * s_merge[(w * GT + h) * MS + DP + 1];
     }
     if (whole) {
-      finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
+      finish<DT>(p, plan, sh.b, g.h0 + h, v, M, num, den);
     } else {
-      part[h * stride + e] = num;
-      if (e == 0) {
-        part[h * stride + DP] = M;
-        part[h * stride + DP + 1] = den;
-      }
+      *reinterpret_cast<float4*>(part + h * MS + v * 4) = num;
+      if (v == 0) *reinterpret_cast<float4*>(part + h * MS + DP) = make_float4(M, den, 0.f, 0.f);
     }
   }
   if (plan.cluster > 1) {
-    cluster_sync();
+    const int rank = blockIdx.x % plan.cluster;
+    int lanes = 2;
+    while (lanes < plan.cluster) lanes *= 2;
+    const int sub = threadIdx.x % lanes, groups = kThreads / lanes, live_v = (p.D + 3) / 4, outputs = g.live_heads * live_v;
+    cluster_arrive();
+    cluster_wait();
     const uint32_t own = (uint32_t)__cvta_generic_to_shared(s_cta);
-    for (int i = blockIdx.x % plan.cluster * kThreads + threadIdx.x; i < g.live_heads * p.D; i += plan.cluster * kThreads) {
-      const int h = i / p.D, e = i % p.D;
-      const uint32_t at = own + (uint32_t)(h * MS) * 4;
-      float M = -INFINITY, num = 0.f, den = 0.f;
-#pragma unroll 4
-      for (int r = 0; r < plan.cluster; ++r) M = fmaxf(M, ld_cluster(at + DP * 4, r));
-      const float base = M > -INFINITY ? M : 0.f;
-#pragma unroll 4
-      for (int r = 0; r < plan.cluster; ++r) {
-        const float f = ex2(ld_cluster(at + DP * 4, r) - base);
-        num += f * ld_cluster(at + e * 4, r);
-        den += f * ld_cluster(at + (DP + 1) * 4, r);
+    for (int o0 = rank * groups; o0 < outputs; o0 += plan.cluster * groups) {
+      const int o = o0 + threadIdx.x / lanes, h = o / live_v, v = o - h * live_v;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f), ml = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      if (o < outputs && sub < plan.cluster) {
+        num = ld_cluster4(own + (uint32_t)(h * MS + v * 4) * 4, sub);
+        ml = ld_cluster4(own + (uint32_t)(h * MS + DP) * 4, sub);
       }
-      finish<DT>(p, sh.b, g.h0 + h, e, M, num, den);
+      float M = ml.x;
+      for (int s = lanes >> 1; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+      const float f = ex2(ml.x - (M > -INFINITY ? M : 0.f));
+      float den = f * ml.y;
+      num.x *= f;
+      num.y *= f;
+      num.z *= f;
+      num.w *= f;
+      for (int s = lanes >> 1; s > 0; s >>= 1) {
+        den += __shfl_xor_sync(0xffffffffu, den, s);
+        num.x += __shfl_xor_sync(0xffffffffu, num.x, s);
+        num.y += __shfl_xor_sync(0xffffffffu, num.y, s);
+        num.z += __shfl_xor_sync(0xffffffffu, num.z, s);
+        num.w += __shfl_xor_sync(0xffffffffu, num.w, s);
+      }
+      if (o < outputs && sub == 0) finish<DT>(p, plan, sh.b, g.h0 + h, v, M, num, den);
     }
-    cluster_sync();   // no CTA leaves while another reads its shared memory
+    cluster_arrive();
+    cluster_wait();   // no CTA leaves while another reads its shared memory
   }
   if (!plan.split) return false;
   sh.first += g.r1 - g.r0;
@@ -309,7 +336,7 @@ struct Place {
 template <class G, class At>
 struct Feeder {
   const Params& p;
-  const Segment& g;
+  Segment g;
   const char *kb, *vb;            // the KV head's rows
   const char *k_piece, *v_piece;  // and this lane's piece of them
   uint32_t lane_at;               // where this lane's piece of a stage's first rows lies
@@ -318,16 +345,52 @@ struct Feeder {
   int page_size, page_shift, warp, lane, npc, most;
   bool wide;                      // int64 entries
   bool same, fast;                // K and V pools are laid out alike; and rows are whole and begin within 64 GB of the pool's beginning
-  __device__ __forceinline__ Feeder(const Params& p_, const Segment& g_, int warp_, int lane_, const unsigned char* ring_, const unsigned char* entries_)
-      : p(p_), g(g_), warp(warp_), lane(lane_) {
-    ring = (uint32_t)__cvta_generic_to_shared(ring_);
-    entries = (uint32_t)__cvta_generic_to_shared(entries_) + (uint32_t)lane * 8;
+  Entry e0, e1;                   // of the segment's first two rounds
+
+  // Finds the segment: its sequence, unit and rounds.  `early` is called as soon as the unit is known.  The loads do not wait for one another
+  // where they need not: the first table entries and what `early` loads are on their way when the length is asked for (not for shares,
+  // whose unit follows from the lengths; entries of a window follow from the length too).
+  template <class Early>
+  __device__ __forceinline__ Feeder(const Params& p_, const Share& sh, const Plan& plan, int units, int gt, int warp_, int lane_, const unsigned char* ring_,
+                                    const unsigned char* entries_, Early early)
+      : p(p_), warp(warp_), lane(lane_) {
+    g.seq = row_of(p, sh.b, threadIdx.x == 0);
     page_size = p.k.page_size;
     page_shift = (page_size & (page_size - 1)) == 0 ? 31 - __clz(page_size) : -1;
-    npc = p.D * G::EB / 16;
     most = (int)min((int64_t)p.k.table_width * page_size, (int64_t)0x7fff0000);
     wide = p.k.table_is_i64 != 0;
     table = (const char*)p.k.block_table + g.seq.row * p.k.table_stride_b * (wide ? 8 : 4);
+    const int rank = blockIdx.x % plan.cluster;
+    g.step = G::ROUND * plan.cluster;
+    g.lo = rank * G::ROUND;
+    g.r0 = 0;
+    const bool ahead = !plan.split && p.window == 0;
+    if (ahead) {
+      e0 = load_entry(0);
+      e1 = load_entry(1);
+    }
+    if (!plan.split) {
+      set_unit(p, g, blockIdx.x / plan.cluster % units, plan.tiles, gt);
+      early(g);
+    }
+    read_length(p, g.seq, threadIdx.x == 0);
+    g.rounds = rounds_of(g.seq, G::ROUND);
+    g.lo += g.seq.lo;
+    if (plan.split) {
+      set_unit(p, g, (int)((sh.first - sh.unit_at) / g.rounds), plan.tiles, gt);
+      early(g);
+      g.r0 = (int)((sh.first - sh.unit_at) % g.rounds);
+      g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
+    } else {
+      g.r1 = max(0, (g.rounds - rank + plan.cluster - 1) / plan.cluster);
+    }
+    if (!ahead) {
+      e0 = load_entry(g.r0);
+      e1 = load_entry(g.r0 + 1);
+    }
+    ring = (uint32_t)__cvta_generic_to_shared(ring_);
+    entries = (uint32_t)__cvta_generic_to_shared(entries_) + (uint32_t)lane * 8;
+    npc = p.D * G::EB / 16;
     kb = (const char*)p.k.cache + (int64_t)g.hkv * p.k.stride_ch * G::EB;
     vb = (const char*)p.v.cache + (int64_t)g.hkv * p.v.stride_ch * G::EB;
     k_piece = kb + lane % G::NPC * 16;
@@ -336,23 +399,24 @@ struct Feeder {
     same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
     fast = same && npc == G::NPC && p.k.n_pages * p.k.stride_page * G::EB < (int64_t)1 << 36;
   }
-  // The entry of this lane's key in round r.  (Any entry of the table may be read: the first are on their way before the length is
-  // known; those behind the sequence's pages are not used.)
-  __device__ __forceinline__ const char* entry_at(int r, int lo) const {
-    const int t = lo + r * G::ROUND + warp * G::KEYS + lane;
+  // first key of this warp in round r
+  __device__ __forceinline__ int key_at(int r) const { return g.lo + r * g.step + warp * G::KEYS; }
+  // The entry of this lane's key in round r.  (Any entry of the table may be read, those behind the sequence's pages are not used.)
+  __device__ __forceinline__ const char* entry_at(int r) const {
+    const int t = key_at(r) + lane;
     if (lane >= G::KEYS || t >= most) return nullptr;
     return table + (int64_t)(page_shift >= 0 ? t >> page_shift : t / page_size) * (wide ? 8 : 4);
   }
-  __device__ __forceinline__ Entry load_entry(int r, int lo) const {
+  __device__ __forceinline__ Entry load_entry(int r) const {
     Entry e;
-    if (const char* at = entry_at(r, lo)) {
+    if (const char* at = entry_at(r)) {
       e.lo = __ldg((const uint32_t*)at);
       if (wide) e.hi = __ldg((const uint32_t*)at + 1);
     }
     return e;
   }
   __device__ __forceinline__ void fetch_entry(int r) const {
-    if (const char* at = entry_at(r, g.seq.lo)) {
+    if (const char* at = entry_at(r)) {
       const uint32_t to = entries + (uint32_t)(r & 3) * (G::KEYS * 8);
       if (wide) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(at));
       else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(to), "l"(at));
@@ -365,7 +429,7 @@ struct Feeder {
   }
   __device__ __forceinline__ void copy(int r, int slot, const Entry& e) const {
     if (r >= g.r1) return;
-    const int t0 = g.seq.lo + r * G::ROUND + warp * G::KEYS, live_keys = g.seq.hi - t0;
+    const int t0 = key_at(r), live_keys = g.seq.hi - t0;
     uint32_t page = e.lo;
     if (page >= (uint32_t)p.k.n_pages || (wide && e.hi != 0)) {
       if (lane < min(live_keys, G::KEYS)) atomicOr(p.status, HIPATTN_STATUS_PAGE_RANGE);
@@ -405,14 +469,6 @@ struct Feeder {
   // the first two rounds of a segment on their way, and the entries of the two after them
   __device__ __forceinline__ void begin() const {
     static_assert(G::STAGES == 3, "two rounds of rows in flight, entries for two more");
-    Entry e0, e1;
-    if (p.window > 0) {
-      e0 = load_entry(g.r0, g.seq.lo);
-      e1 = load_entry(g.r0 + 1, g.seq.lo);
-    } else {
-      e0 = load_entry(g.r0, 0);
-      e1 = load_entry(g.r0 + 1, 0);
-    }
     fetch_entry(g.r0 + 2);
     fetch_entry(g.r0 + 3);
     copy(g.r0, 0, e0);
@@ -420,12 +476,11 @@ struct Feeder {
     copy(g.r0 + 1, 1, e1);
     cp_async_commit();
   }
-  // round r, in place `slot` of the ring, is done: the place before it goes to round r + 2
-  __device__ __forceinline__ void next(int r, int& slot) const {
+  // Round r, in place `slot` of the ring, has arrived (all of the warp are done with the round before it): round r + 2 takes the place of that one.
+  __device__ __forceinline__ void next(int r, int slot) const {
     copy(r + 2, slot == 0 ? 2 : slot - 1, fetched_entry(r + 2));
     fetch_entry(r + 4);
     cp_async_commit();
-    slot = slot == 2 ? 0 : slot + 1;
   }
 };
 
@@ -474,7 +529,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   using P = MmaPlace<G::RB>;
   using T = typename Elem<DT>::type;
   constexpr int MT = F8 ? HIPATTN_F16 : DT;          // type of the products
-  constexpr int KEYS = G::KEYS, MS = DP + 2, KS = DP / 16, NT = DP / 8, AR = GT / 4;   // AR: registers of an A fragment that are not padding
+  constexpr int AHEAD = DP == 256 ? 0 : (G::NPC / 2 < 4 ? G::NPC / 2 : 4);      // loads of values before the weights are made
+  constexpr int KEYS = G::KEYS, MS = DP + 4, KS = DP / 16, NT = DP / 8, AR = GT / 4;   // AR: registers of an A fragment that are not padding
   constexpr float kShift = MT == HIPATTN_F16 ? 14.f : 0.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gr = lane >> 2, jq = lane & 3;
@@ -493,14 +549,36 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   const uint32_t k_lane = F8 ? (KEYS == 32 ? P::at(lane, 0) : P::at(lane & 15, lane >> 4)) : P::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
   const uint32_t v_lane = KEYS * G::RB + P::at(lane & 15, lane >> 4);
 
-  for (bool more = true; more;) {
-    const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
-    const Feeder<G, P> feed(p, g, warp, lane, ring, entries);
-    __syncthreads();
-    feed.begin();
+  const bool pairs = ((uintptr_t)p.q | (uintptr_t)(p.q_stride_b * 2) | (uintptr_t)(p.q_stride_h * 2)) % 4 == 0;    // two elements in one load
 
-    // ---- the unit's queries ----
-    const T* q = reinterpret_cast<const T*>(p.q) + (int64_t)sh.b * p.q_stride_b + (int64_t)g.h0 * p.q_stride_h;
+  for (bool more = true; more;) {
+    __syncthreads();
+    // ---- the segment, and its queries: register r of lane l of a fragment is row l / 4 (+ 8), elements 2 (l % 4) .. (+ 8) of a step; with
+    // fp8 rows 4 (l % 4) .. (+ 2) ----
+    uint32_t qw[KS * 32 * AR / kThreads];
+    auto row_and_element = [&](int j, int& row, int& e) {
+      const int i = j * kThreads + tid, r = i % AR, l = i / AR % 32, ks = i / AR / 32, second = GT == 16 ? r >> 1 : r;
+      row = (l >> 2) + (GT == 16 && (r & 1) ? 8 : 0);
+      e = ks * 16 + (F8 ? (l & 3) * 4 + second * 2 : (l & 3) * 2 + second * 8);
+    };
+    const T* q = nullptr;
+    auto load_queries = [&](const Segment& g) {
+      q = reinterpret_cast<const T*>(p.q) + (int64_t)sh.b * p.q_stride_b + (int64_t)g.h0 * p.q_stride_h;
+#pragma unroll
+      for (int j = 0; j < KS * 32 * AR / kThreads; ++j) {
+        int row, e;
+        row_and_element(j, row, e);
+        qw[j] = 0u;
+        if (row < g.live_heads && e < p.D) {
+          const T* at = q + (int64_t)row * p.q_stride_h + e;
+          if (pairs) qw[j] = __ldg(reinterpret_cast<const uint32_t*>(at));
+          else qw[j] = (uint32_t)*reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
+        }
+      }
+    };
+    const Feeder<G, P> feed(p, sh, plan, units, GT, warp, lane, ring, entries, load_queries);
+    const Segment& g = feed.g;
+    feed.begin();
     if constexpr (F8 && DT == HIPATTN_BF16) {
       for (int h = warp; h < GT; h += kWarps) {
         float mx = 0.f;
@@ -516,21 +594,13 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       __syncthreads();
     }
     const float sign = Logit::sign(p);
-    for (int i = tid; i < KS * 32 * AR; i += kThreads) {
-      // register r of lane l: row l / 4 (+ 8), elements 2 (l % 4) .. (+ 8) of a step; with fp8 rows 4 (l % 4) .. (+ 2)
-      const int r = i % AR, l = i / AR % 32, ks = i / AR / 32;
-      const int row = (l >> 2) + (GT == 16 && (r & 1) ? 8 : 0), second = GT == 16 ? r >> 1 : r;
-      const int e = ks * 16 + (F8 ? (l & 3) * 4 + second * 2 : (l & 3) * 2 + second * 8);
-      float lo = 0.f, hi = 0.f;
-      if (row < g.live_heads) {
-        if (e < p.D) lo = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e]);
-        if (e + 1 < p.D) hi = Elem<DT>::to_f32(q[(int64_t)row * p.q_stride_h + e + 1]);
-        float up = sign;
-        if constexpr (F8 && DT == HIPATTN_BF16) up *= s_up[row];
-        lo *= up;
-        hi *= up;
-      }
-      s_q[i] = pack2<MT>(lo, hi);
+#pragma unroll
+    for (int j = 0; j < KS * 32 * AR / kThreads; ++j) {
+      int row, e;
+      row_and_element(j, row, e);
+      float up = sign;
+      if constexpr (F8 && DT == HIPATTN_BF16) up *= s_up[row];
+      s_q[j * kThreads + tid] = pack2<MT>(lower<DT>(qw[j]) * up, upper<DT>(qw[j]) * up);
     }
     __syncthreads();
     const Logit logit0(p, F8 && DT == HIPATTN_BF16 ? p.sm_scale / s_up[gr] : p.sm_scale);
@@ -544,15 +614,18 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       for (int i = 0; i < GT / 8; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
       int slot = 0;
       for (int r = g.r0; r < g.r1; ++r) {
-        cp_async_wait<G::STAGES - 2>();
+        cp_async_wait<1>();
         __syncwarp();
+        feed.next(r, slot);
         // this lane's row and first piece in K and in V; piece j further is the address xor 16 j (a row begins on a multiple of its size)
         const uint32_t ks = feed.ring + slot * G::STAGE_BYTES + k_lane, vs = feed.ring + slot * G::STAGE_BYTES + v_lane;
         // ---- S = Q K^T ----
         uint32_t kept[4];
-        float s[KEYS / 8][4];
+        float s[KEYS / 8][4], s2[2][4];      // (sixteen keys: odd steps have sums of their own, four chains of products in all)
 #pragma unroll
         for (int i = 0; i < KEYS / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s2[i][0] = s2[i][1] = s2[i][2] = s2[i][3] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           uint32_t a[4] = {0u, 0u, 0u, 0u};
@@ -573,20 +646,30 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
               b[1] = kept[(k & 1) * 2 + 1];
             }
 #pragma unroll
-            for (int n = 0; n < KEYS / 8; ++n) mma16816<MT>(s[n], a, __byte_perm(b[n], 0, 0x1404), __byte_perm(b[n], 0, 0x3424));
+            for (int n = 0; n < KEYS / 8; ++n) mma16816<MT>(KEYS == 16 && (k & 1) ? s2[n & 1] : s[n], a, __byte_perm(b[n], 0, 0x1404), __byte_perm(b[n], 0, 0x3424));
           } else {
 #pragma unroll
             for (int n = 0; n < KEYS / 8; n += 2) {
               uint32_t b[4];
               ldsm_x4_at(b, (ks ^ (k << 5)) + n * 8 * G::RB);
-              mma16816<MT>(s[n], a, b[0], b[1]);
-              mma16816<MT>(s[n + 1], a, b[2], b[3]);
+              mma16816<MT>(KEYS == 16 && (k & 1) ? s2[0] : s[n], a, b[0], b[1]);
+              mma16816<MT>(KEYS == 16 && (k & 1) ? s2[1] : s[n + 1], a, b[2], b[3]);
             }
           }
         }
+        if constexpr (KEYS == 16) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < GT / 4; ++e) s[n][e] += s2[n][e];
+        }
+        // the first values on their way while the weights are made
+        uint32_t vf[AHEAD > 0 ? AHEAD : 1][4];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) ldsm_x4_t_at(vf[i], vs ^ (i << 5));
         // ---- online softmax ----
-        const int t0 = g.seq.lo + r * G::ROUND + warp * KEYS + 2 * jq;
-        const bool tail = g.seq.lo + r * G::ROUND + (warp + 1) * KEYS > g.seq.hi;
+        const int t0 = feed.key_at(r) + 2 * jq;
+        const bool tail = feed.key_at(r) + KEYS > g.seq.hi;
         uint32_t pa[KEYS / 16][4], pl[KEYS / 16][4];     // A fragments; of eight heads pa alone, the second terms in its rows 8 to 15
         bool moved = false;
         float alpha[GT / 8];
@@ -647,7 +730,12 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
           for (int pc = 0; pc < G::NPC; pc += 2) {
             uint32_t b[4];
-            ldsm_x4_t_at(b, (vs ^ (pc << 4)) + c * 16 * G::RB);
+            if (c == 0 && pc / 2 < AHEAD) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) b[e] = vf[pc / 2 < AHEAD ? pc / 2 : 0][e];
+            } else {
+              ldsm_x4_t_at(b, (vs ^ (pc << 4)) + c * 16 * G::RB);
+            }
             if constexpr (F8) {
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
@@ -660,8 +748,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
             }
           }
         }
-        __syncwarp();
-        feed.next(r, slot);
+        slot = slot == 2 ? 0 : slot + 1;
       }
       cp_async_wait<0>();
       if constexpr (GT == 8) {
@@ -717,7 +804,7 @@ template <int DP, int GT>
 __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_kernel(const Params p, const Plan plan) {
   using G = FmaGeo<DP>;
   using P = FmaPlace<G::RB, G::LPK>;
-  constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, MS = DP + 2;
+  constexpr int KEYS = G::KEYS, NPC = G::NPC, LPK = G::LPK, MS = DP + 4;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* ring = smem + warp * (G::STAGES * G::STAGE_BYTES);
@@ -733,16 +820,21 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   const Logit logit(p, p.sm_scale);
 
   for (bool more = true; more;) {
-    const Segment g = segment_of(p, sh, plan, units, G::ROUND, GT);
-    const Feeder<G, P> feed(p, g, warp, lane, ring, entries);
     __syncthreads();
+    float qw[GT * DP / kThreads];
+    auto load_queries = [&](const Segment& g) {
+#pragma unroll
+      for (int j = 0; j < GT * DP / kThreads; ++j) {
+        const int h = (j * kThreads + tid) / DP, e = (j * kThreads + tid) % DP;
+        qw[j] = 0.f;
+        if (h < g.live_heads && e < p.D) qw[j] = reinterpret_cast<const float*>(p.q)[(int64_t)sh.b * p.q_stride_b + (int64_t)(g.h0 + h) * p.q_stride_h + e];
+      }
+    };
+    const Feeder<G, P> feed(p, sh, plan, units, GT, warp, lane, ring, entries, load_queries);
+    const Segment& g = feed.g;
     feed.begin();
-    for (int i = tid; i < GT * DP; i += kThreads) {
-      const int h = i / DP, e = i % DP;
-      float x = 0.f;
-      if (h < g.live_heads && e < p.D) x = reinterpret_cast<const float*>(p.q)[(int64_t)sh.b * p.q_stride_b + (int64_t)(g.h0 + h) * p.q_stride_h + e] * Logit::sign(p);
-      s_q[i] = x;
-    }
+#pragma unroll
+    for (int j = 0; j < GT * DP / kThreads; ++j) s_q[j * kThreads + tid] = qw[j] * Logit::sign(p);
     __syncthreads();
 
     float m_run[GT], l_run[GT], acc[GT][G::PPL][4];
@@ -755,8 +847,9 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
     }
     int slot = 0;
     for (int r = g.r0; r < g.r1; ++r) {
-      cp_async_wait<G::STAGES - 2>();
+      cp_async_wait<1>();
       __syncwarp();
+      feed.next(r, slot);
       const unsigned char* ks = ring + slot * G::STAGE_BYTES;
       const unsigned char* vs = ks + KEYS * G::RB;
       // ---- logits ----
@@ -774,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
           s[h] = fmaf(qv.w, kv.w, fmaf(qv.z, kv.z, fmaf(qv.y, kv.y, fmaf(qv.x, kv.x, s[h]))));
         }
       }
-      const bool in = g.seq.lo + r * G::ROUND + warp * KEYS + key < g.seq.hi;
+      const bool in = feed.key_at(r) + key < g.seq.hi;
       float pr[GT];
 #pragma unroll
       for (int h = 0; h < GT; ++h) {
@@ -811,8 +904,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
           }
         }
       }
-      __syncwarp();
-      feed.next(r, slot);
+      slot = slot == 2 ? 0 : slot + 1;
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -844,16 +936,16 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
 // warps of a head (all eight of them for a single head) take the parts in turn and meet in shared memory.
 constexpr int kMergeWarps = 8;
 template <int DT, int DP, int GT>
-__global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(const Params p, int tiles, int ctas, int round, int least, int hb) {
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(const Params p, const Plan plan, int ctas, int round, int hb) {
   constexpr int PS = DP + 4, V = DP / 4, VL = V > 32 ? V / 32 : 1;       // float4s of a row, and of a lane
   __shared__ int64_t s_sum[2 * kMergeWarps];
   __shared__ __align__(16) float s_num[kMergeWarps][DP];
-  const int heads = p.H / p.HKV, units = p.HKV * tiles, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tiles = plan.tiles, heads = p.H / p.HKV, units = p.HKV * tiles, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / units, u = blockIdx.x % units;
-  const int rounds = rounds_of(sequence_of(p, b, false), round);
+  const int rounds = rounds_of(sequence_of(p, b), round);
   int64_t total, before;
   sum_rounds<kMergeWarps * 32>(p, b, round, s_sum, total, before);
-  const int64_t share = share_of(total * units, ctas, least), begin = before * units + (int64_t)u * rounds;
+  const int64_t share = share_of(total * units, ctas, plan.least), begin = before * units + (int64_t)u * rounds;
   const int c0 = (int)(begin / share), c1 = (int)((begin + rounds - 1) / share);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (every CTA: what follows on the stream waits for this grid alone)
   if (c0 == c1) return;
@@ -896,10 +988,16 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
     }
     __syncthreads();
     if (live) {
-      for (int e = sub * 32 + lane; e < p.D; e += per_head * 32) {
-        float x = 0.f;
-        for (int w = warp - sub; w < warp - sub + per_head; ++w) x += s_num[w][e];
-        finish<DT>(p, b, h0 + h, e, M, x, den);
+      for (int v = sub * 32 + lane; v * 4 < p.D; v += per_head * 32) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = warp - sub; w < warp - sub + per_head; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(&s_num[w][v * 4]);
+          x.x += y.x;
+          x.y += y.y;
+          x.z += y.z;
+          x.w += y.w;
+        }
+        finish<DT>(p, plan, b, h0 + h, v, M, x, den);
       }
     }
     __syncthreads();
@@ -917,7 +1015,7 @@ template <int DT, bool F8, int DP, int GT>
 struct Kernel {
   using G = Geo<DT, F8, DP>;
   static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP + kWarps * 4 * G::KEYS * 8;
-  static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 2) <= G::RING_BYTES, "the join of the warps lies over the rings");
+  static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 4) <= G::RING_BYTES, "the join of the warps lies over the rings");
   static void (*kern())(const Params, const Plan) {
     if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT>;
     else return paged_decode_mma_kernel<DT, F8, DP, GT>;
@@ -929,6 +1027,8 @@ struct Kernel {
     l.least = kLeastRounds;
     l.split = 0;
     l.cluster = 1;
+    constexpr int EB = Elem<DT>::bytes;
+    l.vector_out = ((uintptr_t)p.out | (uintptr_t)(p.o_stride_b * EB) | (uintptr_t)(p.o_stride_h * EB)) % (4 * EB) == 0;
     const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
     int64_t most = (int64_t)p.k.table_width * p.k.page_size;
     if (p.window > 0 && p.window < most) most = p.window;
@@ -984,7 +1084,7 @@ struct Kernel {
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 1;
-    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l.tiles, (int)ctas, (int)G::ROUND, l.least, hb));
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l, (int)ctas, (int)G::ROUND, hb));
     return check_launch("paged_decode_merge_kernel");
   }
 };
