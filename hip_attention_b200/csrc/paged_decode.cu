@@ -616,7 +616,6 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       for (int r = g.r0; r < g.r1; ++r) {
         cp_async_wait<1>();
         __syncwarp();
-        feed.next(r, slot);
         // this lane's row and first piece in K and in V; piece j further is the address xor 16 j (a row begins on a multiple of its size)
         const uint32_t ks = feed.ring + slot * G::STAGE_BYTES + k_lane, vs = feed.ring + slot * G::STAGE_BYTES + v_lane;
         // ---- S = Q K^T ----
@@ -663,6 +662,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
             for (int e = 0; e < GT / 4; ++e) s[n][e] += s2[n][e];
         }
+        feed.next(r, slot);
         // the first values on their way while the weights are made
         uint32_t vf[AHEAD > 0 ? AHEAD : 1][4];
 #pragma unroll
