@@ -2,7 +2,7 @@
 //
 // Which pages are free is read off the reference counts themselves: there is no list beside them that could disagree, and
 // "the lowest free pages in the order of the entries" does not depend on how threads are scheduled.  A call is planned by one
-// cluster (the counts are cut into a slice for each of its CTAs, whose sums are exchanged through distributed shared memory), which
+// cluster (the counts are cut into runs, whose sums its CTAs exchange through distributed shared memory), which
 // also changes the tables; pages are copied by a second launch over the whole GPU that the plan is handed to in device memory.
 #include "common.cuh"
 
@@ -66,49 +66,72 @@ __device__ __forceinline__ N scan_block(N x, N* s, N& all) {
   return sum - x + __shfl_sync(0xffffffffu, ws - w, warp);
 }
 
-// The counts are cut into runs of consecutive pages, one for each thread of the cluster in order (a multiple of four pages, so that
-// small pools are shared out as well); the pages of this thread are [begin, end).
-struct Run {
-  int64_t begin;
-  int end;
+// The reference counts are cut into runs of `loads` times 128 consecutive pages, at most kMaxRuns, which the warps of the cluster take in
+// turn (run q: CTA q % kPlanCtas), so that the pages dealt out, which lie at the front, are spread over all of them.  A lane reads four
+// consecutive pages at a time.
+constexpr int kMaxRuns = 2048;
+struct Runs {
+  int n_pages, loads, count;
 };
-__device__ __forceinline__ Run run_of(int n, int rank) {
-  const int per = (int)(((int64_t)n + (int64_t)kPlanCtas * kPlanThreads * 4 - 1) / ((int64_t)kPlanCtas * kPlanThreads * 4)) * 4;
-  Run r;
-  r.begin = ((int64_t)rank * kPlanThreads + threadIdx.x) * per;
-  r.end = (int)min((int64_t)n, r.begin + per);
+__device__ __forceinline__ Runs runs_of(int n_pages) {
+  Runs r;
+  r.n_pages = n_pages;
+  r.loads = (int)(((int64_t)n_pages + 128 * kMaxRuns - 1) / (128 * kMaxRuns));
+  r.count = (int)(((int64_t)n_pages + 128 * r.loads - 1) / (128 * r.loads));
   return r;
 }
-// bit i: page `at` + i exists (below `end`)
-__device__ __forceinline__ uint32_t range_mask(int64_t at, int end) {
-  return at >= end ? 0u : (at + 32 <= end ? 0xffffffffu : (1u << (int)(end - at)) - 1u);
-}
-// bit i: page `at` + i (below `end`) is in use
-__device__ __forceinline__ uint32_t live_mask(const int32_t* refs, int64_t at, int end) {
-  uint32_t m = 0;
-  const bool aligned = ((uintptr_t)(refs + at) & 15) == 0;
-#pragma unroll
-  for (int i = 0; i < 32; i += 4) {
-    if (at + i >= end) continue;
-    int4 r = make_int4(0, 0, 0, 0);
-    if (aligned && at + i + 4 <= end) {
-      r = *reinterpret_cast<const int4*>(refs + at + i);
-    } else {
-      r.x = refs[at + i];
-      if (at + i + 1 < end) r.y = refs[at + i + 1];
-      if (at + i + 2 < end) r.z = refs[at + i + 2];
-      if (at + i + 3 < end) r.w = refs[at + i + 3];
-    }
-    m |= (uint32_t)((r.x > 0) | (r.y > 0) << 1 | (r.z > 0) << 2 | (r.w > 0) << 3) << i;
+// bit i: page `at` + i is in use / is there
+__device__ __forceinline__ uint32_t live_pages(const int32_t* refs, int64_t at, int n) {
+  if (at + 4 <= n && ((uintptr_t)(refs + at) & 15) == 0) {
+    const int4 r = *reinterpret_cast<const int4*>(refs + at);
+    return (uint32_t)((r.x > 0) | (r.y > 0) << 1 | (r.z > 0) << 2 | (r.w > 0) << 3);
   }
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i < n && refs[at + i] > 0) m |= 1u << i;
   return m;
+}
+__device__ __forceinline__ uint32_t there_pages(int64_t at, int64_t n) { return at >= n ? 0u : (at + 4 <= n ? 15u : (1u << (int)(n - at)) - 1u); }
+
+// Live pages of this warp's runs into s_count [kMaxRuns / kPlanCtas]
+__device__ __forceinline__ void count_runs(const int32_t* refs, const Runs& runs, int rank, int* s_count) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+    int n = 0;
+    for (int j = 0; j < runs.loads; ++j) n += __popc(live_pages(refs, ((int64_t)q * runs.loads + j) * 128 + lane * 4, runs.n_pages));
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s_count[q / kPlanCtas] = n;
+  }
+}
+// Between two cluster barriers (the counts are written; nobody leaves before they are read): the live pages before every run, and in all
+__device__ __forceinline__ int gather_runs(const Runs& runs, const int* s_count, int* s_before, int* s_scan) {
+  const int q = threadIdx.x * 2;
+  const int x = q < runs.count ? ld_cluster_int(s_count + q / kPlanCtas, q % kPlanCtas) : 0;
+  const int y = q + 1 < runs.count ? ld_cluster_int(s_count + (q + 1) / kPlanCtas, (q + 1) % kPlanCtas) : 0;
+  int all;
+  const int before = scan_block(x + y, s_scan, all);
+  s_before[q] = before;
+  s_before[q + 1] = before + x;
+  __syncthreads();
+  return all;
+}
+static_assert(kMaxRuns == 2 * kPlanThreads, "two runs to a thread");
+
+// Sum over the lanes before this one
+__device__ __forceinline__ int scan_warp(int x) {
+  int sum = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) >= o) sum += y;
+  }
+  return sum - x;
 }
 
 // ---------------------------------------------------------------------------------------------------
 // extend and fork
 // ---------------------------------------------------------------------------------------------------
-constexpr int kDealt = 8192;   // pages that a CTA deals out at a time
-
 // A copied page: source, destination, tokens
 struct PageCopy {
   int src, dst, tokens;
@@ -127,20 +150,13 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   uint32_t* s_named = reinterpret_cast<uint32_t*>(s_before + n);   // rows that the call names
   __shared__ long long s_scan64[kPlanWarps];
   __shared__ int s_scan[kPlanWarps];
-  __shared__ int s_free, s_longest;
-  __shared__ int s_dealt[kDealt];
+  __shared__ int s_longest, s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_dealt[kPlanWarps][128];
   const int tid = threadIdx.x, rank = cluster_rank(), P = pool.page_size;
   if (FORK) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  // ---- this thread's free pages (on their way while the entries are read) ----
-  const Run run = run_of(pool.n_pages, rank);
-  int in_run = 0;
-  uint32_t free0 = 0;                   // of the first 32 pages of the run, most often all of it
-  for (int64_t at = run.begin; at < run.end; at += 32) {
-    const uint32_t f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
-    if (at == run.begin) free0 = f;
-    in_run += __popc(f);
-  }
+  const Runs runs = runs_of(pool.n_pages);
+  count_runs(pool.refs, runs, rank, s_count);
+
   for (int i = tid; i < (pool.n_seqs + 31) / 32; i += kPlanThreads) s_named[i] = 0;
   if (tid == 0) s_longest = 0;
   __syncthreads();
@@ -183,18 +199,9 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   }
   bad = __syncthreads_or(bad);
 
-  // ---- free pages before this thread's run, and in all ----
-  int in_slice;
-  const int before_run = scan_block(in_run, s_scan, in_slice);
-  if (tid == 0) s_free = in_slice;
+  // ---- free pages, and those before every run ----
   cluster_sync();
-  int base = 0;
-  long long free_pages = 0;
-  for (int r = 0; r < kPlanCtas; ++r) {
-    const int f = ld_cluster_int(&s_free, r);
-    if (r < rank) base += f;
-    free_pages += f;
-  }
+  const int free_pages = pool.n_pages - gather_runs(runs, s_count, s_live, s_scan);
   cluster_sync();   // (everybody has read the lengths and the sums: from here on they may change, and CTAs may leave)
   if (bad || total > free_pages) {
     if (rank == 0 && tid == 0) {
@@ -204,51 +211,51 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
     return;
   }
 
-  // ---- deal out the free pages: in order into shared memory, then to the entries, consecutive pages to consecutive threads ----
-  // (written by the threads that find them, 40000 pages of 262144 took 32 us, three multiprocessors storing word by word)
-  const long long stop = min(total, (long long)base + in_slice);
-  long long nth = (long long)base + before_run;
-  int64_t at = run.begin;
-  uint32_t f = free0;
-  for (long long from = base; from < stop; from += kDealt) {
-    const int count = (int)min((long long)kDealt, stop - from);
-    __syncthreads();
-    while (at < run.end && nth < from + count) {
-      if (f == 0) {
-        at += 32;
-        if (at < run.end) f = ~live_mask(pool.refs, at, run.end) & range_mask(at, run.end);
-        continue;
-      }
-      s_dealt[nth - from] = (int)at + __ffs(f) - 1;
-      f &= f - 1;
-      ++nth;
-    }
-    __syncthreads();
-    for (int k = tid; k < count; k += kPlanThreads) {
-      const int page = s_dealt[k], j = (int)(from + k);
-      int lo = 0, hi = n - 1;                // the last entry that begins at or before j
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_before[mid] <= j) lo = mid;
-        else hi = mid - 1;
-      }
-      pool.refs[page] = 1;
-      pool.table[(int64_t)s_row[lo] * pool.width + s_had[lo] + (j - s_before[lo])] = page;
-      if (FORK) {
-        int src = pool.table[(int64_t)a[lo] * pool.width + s_had[lo]];
-        int tokens = s_new[lo] - s_had[lo] * P;
-        if (src < 0 || src >= pool.n_pages) {
-          atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
-          src = page;
-          tokens = 0;
+  // ---- deal out the free pages of the runs: a warp brings 128 pages' free ones into order, then consecutive lanes take consecutive ones.
+  // (a million pages of which 36000 are dealt out: 325 us, frees included, with a thread to consecutive pages, 24 so) ----
+  const int warp = tid >> 5, lane = tid & 31;
+  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+    int64_t at = (int64_t)q * runs.loads * 128;
+    int64_t nth = at - s_live[q];             // free pages before
+    for (int j = 0; j < runs.loads && nth < total; ++j, at += 128) {
+      uint32_t f = ~live_pages(pool.refs, at + lane * 4, pool.n_pages) & there_pages(at + lane * 4, pool.n_pages);
+      int k = scan_warp(__popc(f));
+      const int found = __shfl_sync(0xffffffffu, k + __popc(f), 31), count = (int)min((long long)found, total - (long long)nth);
+      for (; f; f &= f - 1) s_dealt[warp][k++] = (int)at + lane * 4 + __ffs(f) - 1;
+      __syncwarp();
+      int entry = 0, end = 0;                 // the entry of the warp's last page, and where it ends: the next pages are most often its too
+      for (int i = lane; i < count; i += 32) {
+        const int page = s_dealt[warp][i], to = (int)nth + i;
+        if (to >= end) {
+          int lo = entry, hi = n - 1;         // the last entry that begins at or before `to`
+          while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_before[mid] <= to) lo = mid;
+            else hi = mid - 1;
+          }
+          entry = lo;
+          end = lo + 1 < n ? s_before[lo + 1] : 0x7fffffff;
         }
-        reinterpret_cast<PageCopy*>(plan + 1)[j] = PageCopy{src, page, tokens};
+        pool.refs[page] = 1;
+        pool.table[(int64_t)s_row[entry] * pool.width + s_had[entry] + (to - s_before[entry])] = page;
+        if (FORK) {
+          int src = pool.table[(int64_t)a[entry] * pool.width + s_had[entry]];
+          int tokens = s_new[entry] - s_had[entry] * P;
+          if (src < 0 || src >= pool.n_pages) {
+            atomicOr(pool.status, HIPATTN_STATUS_PAGE_RANGE);
+            src = page;
+            tokens = 0;
+          }
+          reinterpret_cast<PageCopy*>(plan + 1)[to] = PageCopy{src, page, tokens};
+        }
       }
+      __syncwarp();
+      nth += found;
     }
   }
   if (FORK) {
     // ---- full pages are shared: 128 entries of a table at a time ----
-    const int warp = tid >> 5, lane = tid & 31, chunks = (s_longest + 127) / 128;
+    const int chunks = (s_longest + 127) / 128;
     for (int64_t it = rank * kPlanWarps + warp; it < (int64_t)chunks * n; it += kPlanCtas * kPlanWarps) {
       const int i = (int)(it % n), j0 = (int)(it / n) * 128 + lane;
       if (s_row[i] < 0) continue;
@@ -358,60 +365,52 @@ __host__ __device__ __forceinline__ CompactPlan compact_plan(int32_t* scratch, i
 
 __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Pool pool, int32_t* scratch, int32_t* in_use) {
   __shared__ int s_scan[kPlanWarps];
-  __shared__ int s_live, s_below;
-  const int tid = threadIdx.x, rank = cluster_rank();
+  __shared__ int s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_part;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
   const CompactPlan plan = compact_plan(scratch, pool.n_pages);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  const Run run = run_of(pool.n_pages, rank);
-  int in_run = 0, live;
-  uint32_t live0 = 0;                // of the first 32 pages of the run, most often all of it
-  for (int64_t at = run.begin; at < run.end; at += 32) {
-    const uint32_t f = live_mask(pool.refs, at, run.end);
-    if (at == run.begin) live0 = f;
-    in_run += __popc(f);
+  const Runs runs = runs_of(pool.n_pages);
+  count_runs(pool.refs, runs, rank, s_count);
+  cluster_sync();
+  const int m = gather_runs(runs, s_count, s_live, s_scan);     // pages in use
+  cluster_sync();
+  // ---- of them, numbered below m: those before m's run, and those of the run ----
+  const int run_pages = runs.loads * 128, qm = min(m / run_pages, runs.count - 1);
+  if (warp == 0) {
+    int n = 0;
+    for (int j = 0; j < runs.loads; ++j) {
+      const int64_t at = (int64_t)qm * run_pages + j * 128 + lane * 4;
+      n += __popc(live_pages(pool.refs, at, pool.n_pages) & there_pages(at, m));
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) s_part = n;
   }
-  const int before_run = scan_block(in_run, s_scan, live);
-  if (tid == 0) s_live = live;
-  cluster_sync();
-  int base = 0, m = 0;               // pages in use before the slice, and in all
-  for (int r = 0; r < kPlanCtas; ++r) {
-    const int f = ld_cluster_int(&s_live, r);
-    if (r < rank) base += f;
-    m += f;
-  }
-  int below = 0;                     // of them, numbered below m
-  for (int64_t at = run.begin; at < min(run.end, m); at += 32)
-    below += __popc((at == run.begin ? live0 : live_mask(pool.refs, at, run.end)) & range_mask(at, m));
-  int all_below;
-  scan_block(below, s_scan, all_below);
-  if (tid == 0) s_below = all_below;
-  cluster_sync();
-  int stay = 0;
-  for (int r = 0; r < kPlanCtas; ++r) stay += ld_cluster_int(&s_below, r);
-  cluster_sync();
+  __syncthreads();
+  const int stay = s_live[qm] + s_part;
   if (rank == 0 && tid == 0) {
     plan.count[0] = m - stay;
     plan.count[1] = m;
     if (in_use) *in_use = m;
   }
   if (stay == m) return;
-  int lower = base + before_run;     // pages in use below the next one
-  for (int64_t at = run.begin; at < run.end; at += 32) {
-    const uint32_t f = at == run.begin ? live0 : live_mask(pool.refs, at, run.end);
-    // holes below m, movers at m and beyond: the page's number less the pages in use below it, or that less those that stay
-    uint32_t pick = (~f & range_mask(at, min(run.end, m))) | (f & ~range_mask(at, m));
-    while (pick) {
-      const int i = __ffs(pick) - 1, page = (int)at + i;
-      pick &= pick - 1;
-      const int k = lower + __popc(f & ((1u << i) - 1u));
-      if (page < m) {
-        plan.holes[page - k] = page;
-      } else {
-        plan.movers[k - stay] = page;
-        plan.nth[page] = k - stay;
+  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+    int lower = s_live[q];           // pages in use below the next 128
+    for (int j = 0; j < runs.loads; ++j) {
+      const int64_t at = (int64_t)q * run_pages + j * 128 + lane * 4;
+      const uint32_t live = live_pages(pool.refs, at, pool.n_pages), below = there_pages(at, m);
+      const int before = lower + scan_warp(__popc(live));
+      // holes below m: the page's number less the pages in use below it; movers at m and beyond: that less those that stay
+      for (uint32_t pick = (~live & below) | (live & ~below); pick; pick &= pick - 1) {
+        const int i = __ffs(pick) - 1, page = (int)at + i, k = before + __popc(live & ((1u << i) - 1u));
+        if (page < m) {
+          plan.holes[page - k] = page;
+        } else {
+          plan.movers[k - stay] = page;
+          plan.nth[page] = k - stay;
+        }
       }
+      lower += __reduce_add_sync(0xffffffffu, __popc(live));
     }
-    lower += __popc(f);
   }
 }
 
