@@ -2,7 +2,7 @@
 //
 // Which pages are free is read off the reference counts themselves: there is no list beside them that could disagree, and
 // "the lowest free pages in the order of the entries" does not depend on how threads are scheduled.  A call is planned by one
-// cluster (the counts are cut into runs, whose sums its CTAs exchange through distributed shared memory), which
+// CTA, or a cluster (the counts are cut into runs, whose sums its CTAs exchange through distributed shared memory), which
 // also changes the tables; pages are copied by a second launch over the whole GPU that the plan is handed to in device memory.
 #include "common.cuh"
 
@@ -10,7 +10,8 @@ namespace hipattn {
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kPlanCtas = 8;
+constexpr int kPlanCtas = 8;           // of a cluster; one CTA plans for pools of up to kSmallPool pages
+constexpr int kSmallPool = 8192;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxCachesPerLaunch = 128;
@@ -29,6 +30,10 @@ struct CacheList {
 
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void plan_sync(int ctas) {
+  if (ctas > 1) cluster_sync();
+  else __syncthreads();
 }
 __device__ __forceinline__ int cluster_rank() {
   uint32_t r;
@@ -67,7 +72,7 @@ __device__ __forceinline__ N scan_block(N x, N* s, N& all) {
 }
 
 // The reference counts are cut into runs of `loads` times 128 consecutive pages, at most kMaxRuns, which the warps of the cluster take in
-// turn (run q: CTA q % kPlanCtas), so that the pages dealt out, which lie at the front, are spread over all of them.  A lane reads four
+// turn (run q: CTA q % ctas), so that the pages dealt out, which lie at the front, are spread over all of them.  A lane reads four
 // consecutive pages at a time.
 constexpr int kMaxRuns = 2048;
 struct Runs {
@@ -94,21 +99,21 @@ __device__ __forceinline__ uint32_t live_pages(const int32_t* refs, int64_t at, 
 }
 __device__ __forceinline__ uint32_t there_pages(int64_t at, int64_t n) { return at >= n ? 0u : (at + 4 <= n ? 15u : (1u << (int)(n - at)) - 1u); }
 
-// Live pages of this warp's runs into s_count [kMaxRuns / kPlanCtas]
-__device__ __forceinline__ void count_runs(const int32_t* refs, const Runs& runs, int rank, int* s_count) {
+// Live pages of this warp's runs into s_count
+__device__ __forceinline__ void count_runs(const int32_t* refs, const Runs& runs, int rank, int ctas, int* s_count) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+  for (int q = rank + warp * ctas; q < runs.count; q += ctas * kPlanWarps) {
     int n = 0;
     for (int j = 0; j < runs.loads; ++j) n += __popc(live_pages(refs, ((int64_t)q * runs.loads + j) * 128 + lane * 4, runs.n_pages));
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) s_count[q / kPlanCtas] = n;
+    if (lane == 0) s_count[q / ctas] = n;
   }
 }
-// Between two cluster barriers (the counts are written; nobody leaves before they are read): the live pages before every run, and in all
-__device__ __forceinline__ int gather_runs(const Runs& runs, const int* s_count, int* s_before, int* s_scan) {
+// Between two barriers (the counts are written; nobody leaves before they are read): the live pages before every run, and in all
+__device__ __forceinline__ int gather_runs(const Runs& runs, int ctas, const int* s_count, int* s_before, int* s_scan) {
   const int q = threadIdx.x * 2;
-  const int x = q < runs.count ? ld_cluster_int(s_count + q / kPlanCtas, q % kPlanCtas) : 0;
-  const int y = q + 1 < runs.count ? ld_cluster_int(s_count + (q + 1) / kPlanCtas, (q + 1) % kPlanCtas) : 0;
+  auto count = [&](int i) { return i >= runs.count ? 0 : (ctas > 1 ? ld_cluster_int(s_count + i / ctas, i % ctas) : s_count[i]); };
+  const int x = count(q), y = count(q + 1);
   int all;
   const int before = scan_block(x + y, s_scan, all);
   s_before[q] = before;
@@ -117,6 +122,7 @@ __device__ __forceinline__ int gather_runs(const Runs& runs, const int* s_count,
   return all;
 }
 static_assert(kMaxRuns == 2 * kPlanThreads, "two runs to a thread");
+static_assert(kSmallPool / 128 <= kMaxRuns / kPlanCtas, "the runs of a small pool fit into one CTA's counts");
 
 // Sum over the lanes before this one
 __device__ __forceinline__ int scan_warp(int x) {
@@ -140,8 +146,8 @@ struct PageCopy {
 // extend: a[i] = row, b[i] (b null: every) = tokens that it grows by.  fork: a[i] = parent, b[i] = child.
 // plan (fork): [0] = number of copies, then PageCopy[].
 template <bool FORK>
-__global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
-    deal_pages_kernel(const Pool pool, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int every, int n, int32_t* plan) {
+__global__ void __launch_bounds__(kPlanThreads, 1)
+    deal_pages_kernel(const Pool pool, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int every, int n, int32_t* plan, int ctas) {
   extern __shared__ __align__(16) unsigned char smem[];
   int* s_row = reinterpret_cast<int*>(smem);        // row that gets pages, -1: none
   int* s_had = s_row + n;                           // pages that it has (fork: full pages of the parent)
@@ -151,21 +157,21 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   __shared__ long long s_scan64[kPlanWarps];
   __shared__ int s_scan[kPlanWarps];
   __shared__ int s_longest, s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_dealt[kPlanWarps][128];
-  const int tid = threadIdx.x, rank = cluster_rank(), P = pool.page_size;
+  const int tid = threadIdx.x, rank = blockIdx.x, P = pool.page_size;
   if (FORK) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
   const Runs runs = runs_of(pool.n_pages);
-  count_runs(pool.refs, runs, rank, s_count);
-
+  const int per = (n + kPlanThreads - 1) / kPlanThreads;   // consecutive entries of a thread
+  const int x0 = tid * per < n ? a[tid * per] : -1, y0 = tid * per < n && b ? b[tid * per] : every;     // (on their way with the counts)
   for (int i = tid; i < (pool.n_seqs + 31) / 32; i += kPlanThreads) s_named[i] = 0;
   if (tid == 0) s_longest = 0;
+  count_runs(pool.refs, runs, rank, ctas, s_count);
   __syncthreads();
   // ---- the entries: every CTA goes through all of them ----
   bool bad = false;
   long long mine = 0;
-  const int per = (n + kPlanThreads - 1) / kPlanThreads;   // consecutive entries of a thread
   for (int i = tid * per; i < min(n, (tid + 1) * per); ++i) {
-    const int x = a[i], y = b ? b[i] : every, row = FORK ? y : x;
+    const int x = i == tid * per ? x0 : a[i], y = i == tid * per ? y0 : (b ? b[i] : every), row = FORK ? y : x;
     int had = 0, len = 0, need = 0, at = -1;
     if (x >= 0 && row >= 0) {
       if (x >= pool.n_seqs || row >= pool.n_seqs || (!FORK && y < 0) || (atomicOr(&s_named[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u)) {
@@ -200,9 +206,9 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   bad = __syncthreads_or(bad);
 
   // ---- free pages, and those before every run ----
-  cluster_sync();
-  const int free_pages = pool.n_pages - gather_runs(runs, s_count, s_live, s_scan);
-  cluster_sync();   // (everybody has read the lengths and the sums: from here on they may change, and CTAs may leave)
+  plan_sync(ctas);
+  const int free_pages = pool.n_pages - gather_runs(runs, ctas, s_count, s_live, s_scan);
+  plan_sync(ctas);   // (everybody has read the lengths and the sums: from here on they may change, and CTAs may leave)
   if (bad || total > free_pages) {
     if (rank == 0 && tid == 0) {
       atomicOr(pool.status, bad ? HIPATTN_STATUS_SEQUENCE : HIPATTN_STATUS_NO_PAGES);
@@ -214,7 +220,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   // ---- deal out the free pages of the runs: a warp brings 128 pages' free ones into order, then consecutive lanes take consecutive ones.
   // (a million pages of which 36000 are dealt out: 325 us, frees included, with a thread to consecutive pages, 24 so) ----
   const int warp = tid >> 5, lane = tid & 31;
-  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+  for (int q = rank + warp * ctas; q < runs.count; q += ctas * kPlanWarps) {
     int64_t at = (int64_t)q * runs.loads * 128;
     int64_t nth = at - s_live[q];             // free pages before
     for (int j = 0; j < runs.loads && nth < total; ++j, at += 128) {
@@ -256,7 +262,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1)
   if (FORK) {
     // ---- full pages are shared: 128 entries of a table at a time ----
     const int chunks = (s_longest + 127) / 128;
-    for (int64_t it = rank * kPlanWarps + warp; it < (int64_t)chunks * n; it += kPlanCtas * kPlanWarps) {
+    for (int64_t it = rank * kPlanWarps + warp; it < (int64_t)chunks * n; it += ctas * kPlanWarps) {
       const int i = (int)(it % n), j0 = (int)(it / n) * 128 + lane;
       if (s_row[i] < 0) continue;
       const int32_t* from = pool.table + (int64_t)a[i] * pool.width;
@@ -363,17 +369,17 @@ __host__ __device__ __forceinline__ CompactPlan compact_plan(int32_t* scratch, i
   return c;
 }
 
-__global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Pool pool, int32_t* scratch, int32_t* in_use) {
+__global__ void __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Pool pool, int32_t* scratch, int32_t* in_use, int ctas) {
   __shared__ int s_scan[kPlanWarps];
   __shared__ int s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_part;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = cluster_rank();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x;
   const CompactPlan plan = compact_plan(scratch, pool.n_pages);
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const Runs runs = runs_of(pool.n_pages);
-  count_runs(pool.refs, runs, rank, s_count);
-  cluster_sync();
-  const int m = gather_runs(runs, s_count, s_live, s_scan);     // pages in use
-  cluster_sync();
+  count_runs(pool.refs, runs, rank, ctas, s_count);
+  plan_sync(ctas);
+  const int m = gather_runs(runs, ctas, s_count, s_live, s_scan);     // pages in use
+  plan_sync(ctas);
   // ---- of them, numbered below m: those before m's run, and those of the run ----
   const int run_pages = runs.loads * 128, qm = min(m / run_pages, runs.count - 1);
   if (warp == 0) {
@@ -393,7 +399,7 @@ __global__ void __cluster_dims__(kPlanCtas) __launch_bounds__(kPlanThreads, 1) p
     if (in_use) *in_use = m;
   }
   if (stay == m) return;
-  for (int q = rank + warp * kPlanCtas; q < runs.count; q += kPlanCtas * kPlanWarps) {
+  for (int q = rank + warp * ctas; q < runs.count; q += ctas * kPlanWarps) {
     int lower = s_live[q];           // pages in use below the next 128
     for (int j = 0; j < runs.loads; ++j) {
       const int64_t at = (int64_t)q * run_pages + j * 128 + lane * 4;
@@ -602,13 +608,33 @@ Pool device_pool(const hipattn_page_pool_t& p) {
   return Pool{p.ref_counts, p.seq_lens, p.block_table, p.status, p.n_pages, p.page_size, p.n_sequences, p.table_width};
 }
 
+// `ctas` CTAs, a cluster when there are several
+struct PlanLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  PlanLaunch(int64_t grid, int ctas, int threads, size_t smem, cudaStream_t stream) {
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)ctas;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
+  }
+};
+int plan_ctas(const hipattn_page_pool_t& p) { return p.n_pages <= kSmallPool ? 1 : kPlanCtas; }
+
 template <bool FORK>
 int deal_pages(const hipattn_page_pool_t& p, const int32_t* a, const int32_t* b, int every, int n, int32_t* plan, cudaStream_t stream, const char* what) {
   HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "%s: %d entries outside [1, %d]", what, n, HIPATTN_POOL_MAX_ENTRIES);
   HIPATTN_REQUIRE(a && (b || !FORK), HIPATTN_ERR_INVALID, "%s: null pointer", what);
   const size_t smem = 4 * sizeof(int) * (size_t)n + sizeof(uint32_t) * (size_t)((p.n_sequences + 31) / 32);
   HIPATTN_CUDA_OK(allow_smem((const void*)deal_pages_kernel<FORK>, smem));
-  deal_pages_kernel<FORK><<<kPlanCtas, kPlanThreads, smem, stream>>>(device_pool(p), a, b, every, n, plan);
+  const int ctas = plan_ctas(p);
+  PlanLaunch launch(ctas, ctas, kPlanThreads, smem, stream);
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, deal_pages_kernel<FORK>, device_pool(p), a, b, every, n, plan, ctas));
   return check_launch("deal_pages_kernel");
 }
 
@@ -672,17 +698,8 @@ extern "C" int hipattn_pool_free(const hipattn_page_pool_t* p, const int32_t* ro
   HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "pool_free: %d entries outside [1, %d]", n, HIPATTN_POOL_MAX_ENTRIES);
   HIPATTN_REQUIRE(rows != nullptr, HIPATTN_ERR_INVALID, "pool_free: null pointer");
   const int ctas = p->table_width > 1024 ? 8 : 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n * ctas));
-  cfg.blockDim = dim3(256);
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)ctas;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, free_rows_kernel, device_pool(*p), rows, ctas));
+  PlanLaunch launch((int64_t)n * ctas, ctas, 256, 0, (cudaStream_t)stream);
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, free_rows_kernel, device_pool(*p), rows, ctas));
   return check_launch("free_rows_kernel");
 }
 
@@ -690,7 +707,9 @@ extern "C" int hipattn_pool_compact(const hipattn_page_pool_t* p, int32_t* pages
   int rc = validate_pool(p, "pool_compact", true);
   if (rc) return rc;
   HIPATTN_REQUIRE(p->scratch != nullptr, HIPATTN_ERR_INVALID, "pool_compact: scratch is null");
-  plan_compact_kernel<<<kPlanCtas, kPlanThreads, 0, (cudaStream_t)stream>>>(device_pool(*p), (int32_t*)p->scratch, pages_in_use);
+  const int ctas = plan_ctas(*p);
+  PlanLaunch plan(ctas, ctas, kPlanThreads, 0, (cudaStream_t)stream);
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&plan.cfg, plan_compact_kernel, device_pool(*p), (int32_t*)p->scratch, pages_in_use, ctas));
   rc = check_launch("plan_compact_kernel");
   if (rc) return rc;
   const int pieces = (int)((p->page_bytes + kCopyBytes - 1) / kCopyBytes);
