@@ -251,7 +251,29 @@ std::unordered_map<int, at::Tensor> g_status;
 at::Tensor status_word(int index) {
   std::lock_guard<std::mutex> lock(g_status_mutex);
   at::Tensor& t = g_status[index];
-  if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, index));
+  if (t.defined()) return t;
+  const auto options = at::TensorOptions().dtype(at::kInt).device(at::kCUDA, index);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(index).stream();
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  cuda_ok(cudaStreamIsCapturing(stream, &capturing), "cudaStreamIsCapturing");
+  if (capturing == cudaStreamCaptureStatusNone) {
+    t = at::zeros({1}, options);
+  } else {
+    // the first call of the process is being captured: the word must neither come from the graph's memory nor be zeroed by its replays
+    const c10::cuda::CUDAGuard guard(c10::Device(at::kCUDA, index));
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cuda_ok(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+    void* word = nullptr;
+    cudaStream_t side = nullptr;
+    cudaError_t e = cudaMalloc(&word, sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&side, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int32_t), side);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(side);
+    if (side) cudaStreamDestroy(side);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cuda_ok(e, "device status word");
+    t = at::from_blob(word, {1}, options);
+  }
   return t;
 }
 
@@ -1474,7 +1496,7 @@ PyObject* page_pool(PyObject* const* argv) {
       VALUE_ERROR("the caches of a pool must have one shape, type, layout and device");
     if (dtype_of(c.scalar_type()) < 0 && !is_fp8(c.scalar_type())) VALUE_ERROR("caches must be float32, float16, bfloat16 or float8_e5m2 (or its uint8 view)");
     if (c.numel() == 0) VALUE_ERROR("caches %s have no elements", shape_text(c).c_str());
-    if (c.stride(3) != 1 || c.stride(2) != c.size(3) || (c.size(1) > 1 && c.stride(1) != c.size(2) * c.size(3)))
+    if (c.stride(3) != 1 || (c.size(2) > 1 && c.stride(2) != c.size(3)) || (c.size(1) > 1 && c.stride(1) != c.size(2) * c.size(3)))
       VALUE_ERROR("the tokens of a page must be contiguous (the pages may lie anywhere)");
     if (c.size(0) > 1 && c.stride(0) < c.size(1) * c.size(2) * c.size(3)) VALUE_ERROR("pages overlap");
     h->keep.push_back(c);

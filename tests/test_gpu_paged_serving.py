@@ -224,3 +224,35 @@ def test_calls_of_the_c_interface():
     vals = [v[:1111].double(), v[1111:].double()]
     none = torch.zeros((0, HKV, D), dtype=torch.float64, device="cuda")
     check(out, lse, reference(q, [keys[0], keys[1], none, none, keys[0]], [vals[0], vals[1], none, none, vals[0]], 0.2), q.dtype)
+
+
+def test_first_call_of_a_process_captured():
+    """A process whose first call is captured: the status word is not part of the graph, neither its memory nor its zeros."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from hip_attention_b200 import paged_decode_attention, read_status
+kc, vc = (torch.randn((4, 4, 2, 64), device='cuda') for _ in range(2))
+q, table, lens = torch.randn((1, 4, 64), device='cuda'), torch.tensor([[2, 9]], device='cuda'), torch.tensor([3], device='cuda')
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = paged_decode_attention(q, kc, vc, table, lens)
+graph.replay()
+assert read_status('cuda') == 0
+want = paged_decode_attention(q, kc, vc, table, lens)
+assert torch.equal(out, want)
+lens.fill_(6)                      # the second page is out of range
+graph.replay()
+assert read_status('cuda') == 1 and read_status('cuda') == 0
+del out, graph
+torch.cuda.empty_cache()
+lens.fill_(3)
+assert torch.equal(paged_decode_attention(q, kc, vc, table, lens), want) and read_status('cuda') == 0
+print('fine')
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
