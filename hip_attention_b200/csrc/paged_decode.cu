@@ -84,8 +84,12 @@ __device__ __forceinline__ void sum_rounds(const Params& p, int b, int round, in
   }
 }
 
+// a / b of numbers that are not negative: in 32 bits wherever they fit (a division of 64 bits is a hundred instructions)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
 __device__ __forceinline__ int64_t share_of(int64_t total, int ctas, int least) {
-  const int64_t s = (total + ctas - 1) / ctas;
+  const int64_t s = quotient(total + ctas - 1, ctas);
   return s < least ? least : s;
 }
 
@@ -377,9 +381,10 @@ struct Feeder {
     g.rounds = rounds_of(g.seq, G::ROUND);
     g.lo += g.seq.lo;
     if (plan.split) {
-      set_unit(p, g, (int)((sh.first - sh.unit_at) / g.rounds), plan.tiles, gt);
+      const int64_t from = sh.first - sh.unit_at, u = quotient(from, g.rounds);
+      set_unit(p, g, (int)u, plan.tiles, gt);
       early(g);
-      g.r0 = (int)((sh.first - sh.unit_at) % g.rounds);
+      g.r0 = (int)(from - u * g.rounds);
       g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
     } else {
       g.r1 = max(0, (g.rounds - rank + plan.cluster - 1) / plan.cluster);
@@ -946,7 +951,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   int64_t total, before;
   sum_rounds<kMergeWarps * 32>(p, b, round, s_sum, total, before);
   const int64_t share = share_of(total * units, ctas, plan.least), begin = before * units + (int64_t)u * rounds;
-  const int c0 = (int)(begin / share), c1 = (int)((begin + rounds - 1) / share);
+  const int c0 = (int)quotient(begin, share), c1 = (int)quotient(begin + rounds - 1, share);
   asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (every CTA: what follows on the stream waits for this grid alone)
   if (c0 == c1) return;
   const int tile = u % tiles, h0 = u / tiles * heads + tile * GT, live_heads = min(GT, heads - tile * GT);
@@ -1007,7 +1012,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
 constexpr int kLeastRounds = 2;       // rounds of a share
 constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
 constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
-constexpr int kWholeRounds = 32;      // most rounds of a unit that is a CTA's
+constexpr int kWholeRounds = 64;      // most rounds of a unit that is a CTA's
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
