@@ -4,7 +4,7 @@
 // "the lowest free pages in the order of the entries" does not depend on how threads are scheduled.  A call is planned by one
 // CTA, or a cluster (the counts are cut into runs, whose sums its CTAs exchange through distributed shared memory), which
 // also changes the tables; pages are copied by a second launch over the whole GPU that the plan is handed to in device memory.
-#include "common.cuh"
+#include "in_turn.cuh"
 
 namespace hipattn {
 namespace {
@@ -147,7 +147,7 @@ struct PageCopy {
 // plan (fork): [0] = number of copies, then PageCopy[].
 template <bool FORK>
 __global__ void __launch_bounds__(kPlanThreads, 1)
-    deal_pages_kernel(const Pool pool, const int32_t* __restrict__ a, const int32_t* __restrict__ b, int every, int n, int32_t* plan, int ctas) {
+    deal_pages_kernel(const Pool pool, const int32_t* a, const int32_t* b, int every, int n, int32_t* plan, int ctas) {
   extern __shared__ __align__(16) unsigned char smem[];
   int* s_row = reinterpret_cast<int*>(smem);        // row that gets pages, -1: none
   int* s_had = s_row + n;                           // pages that it has (fork: full pages of the parent)
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   __shared__ int s_scan[kPlanWarps];
   __shared__ int s_longest, s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_dealt[kPlanWarps][128];
   const int tid = threadIdx.x, rank = blockIdx.x, P = pool.page_size;
-  if (FORK) asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  in_turn();
 
   const Runs runs = runs_of(pool.n_pages);
   const int per = (n + kPlanThreads - 1) / kPlanThreads;   // consecutive entries of a thread
@@ -310,7 +310,7 @@ __device__ __forceinline__ void copy_piece(const char* src, char* dst, int64_t b
 // The begun pages of a fork
 __global__ void __launch_bounds__(kCopyThreads) copy_begun_pages_kernel(const CacheList caches, const int32_t* plan, int64_t page_stride, int64_t token_bytes,
                                                                         int pieces) {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  in_turn();
   const int count = plan[0];
   const PageCopy* copies = reinterpret_cast<const PageCopy*>(plan + 1);
   for (int64_t it = blockIdx.x; it < (int64_t)count * caches.n * pieces; it += gridDim.x) {
@@ -326,8 +326,9 @@ __global__ void __launch_bounds__(kCopyThreads) copy_begun_pages_kernel(const Ca
 // free
 // ---------------------------------------------------------------------------------------------------
 // One cluster per row.  Its first CTA takes the length and leaves 0, so that a row that is named twice is freed once.
-__global__ void __launch_bounds__(256) free_rows_kernel(const Pool pool, const int32_t* __restrict__ rows, int ctas) {
+__global__ void __launch_bounds__(256) free_rows_kernel(const Pool pool, const int32_t* rows, int ctas) {
   __shared__ int s_len;
+  in_turn();
   const int rank = ctas > 1 ? cluster_rank() : 0;
   const int row = rows[blockIdx.x / ctas];
   const bool there = row >= 0 && row < pool.n_seqs;
@@ -372,9 +373,9 @@ __host__ __device__ __forceinline__ CompactPlan compact_plan(int32_t* scratch, i
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Pool pool, int32_t* scratch, int32_t* in_use, int ctas) {
   __shared__ int s_scan[kPlanWarps];
   __shared__ int s_count[kMaxRuns / kPlanCtas], s_live[kMaxRuns], s_part;
+  in_turn();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = blockIdx.x;
   const CompactPlan plan = compact_plan(scratch, pool.n_pages);
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const Runs runs = runs_of(pool.n_pages);
   count_runs(pool.refs, runs, rank, ctas, s_count);
   plan_sync(ctas);
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_compact_kernel(const Poo
 // Pages, counts and (first launch) tables
 __global__ void __launch_bounds__(kCopyThreads) move_pages_kernel(const Pool pool, const CacheList caches, int32_t* scratch, int64_t page_stride, int64_t page_bytes,
                                                                   int pieces, int tables) {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  in_turn();
   const CompactPlan plan = compact_plan(scratch, pool.n_pages);
   const int moves = plan.count[0], m = plan.count[1];
   if (moves == 0) return;
@@ -491,6 +492,7 @@ template <int DT, bool F8>
 __global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_write_kv_params_t p, int span, int lanes) {
   constexpr int EB = Elem<DT>::bytes, VEC = 16 / EB, CB = F8 ? 1 : EB;
   __shared__ int s_page[kMaxSpan], s_off[kMaxSpan];
+  in_turn();
   const int row_pieces = p.D / VEC, pieces = p.HKV * row_pieces;       // of a token, keys or values
   const int64_t tok0 = (int64_t)blockIdx.x * span;
   const int tokens = (int)min((int64_t)span, p.N - tok0);
@@ -517,7 +519,7 @@ __global__ void __launch_bounds__(kWriteThreads) write_kv_kernel(const hipattn_w
   for (int k = 0; k < kWriteAhead; ++k) load(group + k * groups, x[k]);
 
   if (threadIdx.x < tokens) {
-    auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldg((const long long*)q + i) : (int64_t)__ldg((const int*)q + i); };
+    auto index = [](const void* q, int is64, int64_t i) { return is64 ? (int64_t)__ldcg((const long long*)q + i) : (int64_t)__ldcg((const int*)q + i); };
     const int64_t tok = tok0 + threadIdx.x;
     int page = -1, off = 0;                  // -1: not written
     // the token's sequence and place in it
@@ -608,22 +610,6 @@ Pool device_pool(const hipattn_page_pool_t& p) {
   return Pool{p.ref_counts, p.seq_lens, p.block_table, p.status, p.n_pages, p.page_size, p.n_sequences, p.table_width};
 }
 
-// `ctas` CTAs, a cluster when there are several
-struct PlanLaunch {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  PlanLaunch(int64_t grid, int ctas, int threads, size_t smem, cudaStream_t stream) {
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)ctas;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = ctas > 1 ? 1 : 0;
-  }
-};
 int plan_ctas(const hipattn_page_pool_t& p) { return p.n_pages <= kSmallPool ? 1 : kPlanCtas; }
 
 template <bool FORK>
@@ -633,25 +619,11 @@ int deal_pages(const hipattn_page_pool_t& p, const int32_t* a, const int32_t* b,
   const size_t smem = 4 * sizeof(int) * (size_t)n + sizeof(uint32_t) * (size_t)((p.n_sequences + 31) / 32);
   HIPATTN_CUDA_OK(allow_smem((const void*)deal_pages_kernel<FORK>, smem));
   const int ctas = plan_ctas(p);
-  PlanLaunch launch(ctas, ctas, kPlanThreads, smem, stream);
+  InTurn launch(ctas, kPlanThreads, smem, stream, ctas);
   HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, deal_pages_kernel<FORK>, device_pool(p), a, b, every, n, plan, ctas));
   return check_launch("deal_pages_kernel");
 }
 
-// a launch that may begin while the one before it, which it waits for, is still running
-struct AfterPlan {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  AfterPlan(int64_t grid, int threads, cudaStream_t stream) {
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.stream = stream;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-  }
-};
 int64_t copy_grid(int64_t items) {
   const int64_t most = kSMs * 8;
   return items < 1 ? 1 : (items < most ? items : most);
@@ -684,7 +656,7 @@ extern "C" int hipattn_pool_fork(const hipattn_page_pool_t* p, const int32_t* pa
     CacheList list;
     list.n = p->n_caches - c0 < kMaxCachesPerLaunch ? p->n_caches - c0 : kMaxCachesPerLaunch;
     for (int i = 0; i < list.n; ++i) list.at[i] = (char*)p->caches[c0 + i];
-    AfterPlan launch(copy_grid((int64_t)n * list.n * pieces), kCopyThreads, (cudaStream_t)stream);
+    InTurn launch(copy_grid((int64_t)n * list.n * pieces), kCopyThreads, 0, (cudaStream_t)stream);
     HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, copy_begun_pages_kernel, list, (const int32_t*)p->scratch, p->page_stride, p->page_bytes / p->page_size, pieces));
     rc = check_launch("copy_begun_pages_kernel");
     if (rc) return rc;
@@ -698,7 +670,7 @@ extern "C" int hipattn_pool_free(const hipattn_page_pool_t* p, const int32_t* ro
   HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "pool_free: %d entries outside [1, %d]", n, HIPATTN_POOL_MAX_ENTRIES);
   HIPATTN_REQUIRE(rows != nullptr, HIPATTN_ERR_INVALID, "pool_free: null pointer");
   const int ctas = p->table_width > 1024 ? 8 : 1;
-  PlanLaunch launch((int64_t)n * ctas, ctas, 256, 0, (cudaStream_t)stream);
+  InTurn launch((int64_t)n * ctas, 256, 0, (cudaStream_t)stream, ctas);
   HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, free_rows_kernel, device_pool(*p), rows, ctas));
   return check_launch("free_rows_kernel");
 }
@@ -708,7 +680,7 @@ extern "C" int hipattn_pool_compact(const hipattn_page_pool_t* p, int32_t* pages
   if (rc) return rc;
   HIPATTN_REQUIRE(p->scratch != nullptr, HIPATTN_ERR_INVALID, "pool_compact: scratch is null");
   const int ctas = plan_ctas(*p);
-  PlanLaunch plan(ctas, ctas, kPlanThreads, 0, (cudaStream_t)stream);
+  InTurn plan(ctas, kPlanThreads, 0, (cudaStream_t)stream, ctas);
   HIPATTN_CUDA_OK(cudaLaunchKernelEx(&plan.cfg, plan_compact_kernel, device_pool(*p), (int32_t*)p->scratch, pages_in_use, ctas));
   rc = check_launch("plan_compact_kernel");
   if (rc) return rc;
@@ -717,7 +689,7 @@ extern "C" int hipattn_pool_compact(const hipattn_page_pool_t* p, int32_t* pages
     CacheList list;
     list.n = p->n_caches - c0 < kMaxCachesPerLaunch ? p->n_caches - c0 : kMaxCachesPerLaunch;
     for (int i = 0; i < list.n; ++i) list.at[i] = (char*)p->caches[c0 + i];
-    AfterPlan launch(copy_grid((int64_t)half_of(p->n_pages) * list.n * pieces + (int64_t)p->n_sequences * ((p->table_width + 31) / 32) / 8), kCopyThreads, (cudaStream_t)stream);
+    InTurn launch(copy_grid((int64_t)half_of(p->n_pages) * list.n * pieces + (int64_t)p->n_sequences * ((p->table_width + 31) / 32) / 8), kCopyThreads, 0, (cudaStream_t)stream);
     HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, move_pages_kernel, device_pool(*p), list, (int32_t*)p->scratch, p->page_stride, p->page_bytes, pieces, c0 == 0 ? 1 : 0));
     rc = check_launch("move_pages_kernel");
     if (rc) return rc;
@@ -753,18 +725,13 @@ extern "C" int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream
   int lanes = 32;      // threads to a token: a power of two that its pieces fill
   while (lanes < kWriteThreads && lanes < pieces) lanes *= 2;
   HIPATTN_REQUIRE(blocks < 0x7fffffffLL, HIPATTN_ERR_INVALID, "write_kv: grid of %lld blocks", (long long)blocks);
-  const cudaStream_t s = (cudaStream_t)stream;
-  switch (p->dtype) {
-    case HIPATTN_F32: write_kv_kernel<HIPATTN_F32, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes); break;
-    case HIPATTN_F16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_F16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
-      else write_kv_kernel<HIPATTN_F16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
-      break;
-    case HIPATTN_BF16:
-      if (p->k_pool.fp8_e5m2) write_kv_kernel<HIPATTN_BF16, true><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
-      else write_kv_kernel<HIPATTN_BF16, false><<<(unsigned)blocks, kWriteThreads, 0, s>>>(*p, (int)span, lanes);
-      break;
-    default: set_error("write_kv: unknown dtype %d", p->dtype); return HIPATTN_ERR_INVALID;
-  }
+  const bool f8 = p->k_pool.fp8_e5m2 != 0;
+  void (*kern)(const hipattn_write_kv_params_t, int, int) = nullptr;
+  if (p->dtype == HIPATTN_F32) kern = write_kv_kernel<HIPATTN_F32, false>;
+  if (p->dtype == HIPATTN_F16) kern = f8 ? write_kv_kernel<HIPATTN_F16, true> : write_kv_kernel<HIPATTN_F16, false>;
+  if (p->dtype == HIPATTN_BF16) kern = f8 ? write_kv_kernel<HIPATTN_BF16, true> : write_kv_kernel<HIPATTN_BF16, false>;
+  HIPATTN_REQUIRE(kern != nullptr, HIPATTN_ERR_INVALID, "write_kv: unknown dtype %d", p->dtype);
+  InTurn launch(blocks, kWriteThreads, 0, (cudaStream_t)stream);
+  HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, kern, *p, (int)span, lanes));
   return check_launch("write_kv_kernel");
 }

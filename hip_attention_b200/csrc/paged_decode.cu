@@ -9,6 +9,7 @@
 // A warp takes KEYS keys at a time from a ring of its own in shared memory, filled with 16-byte asynchronous copies, and keeps
 // its own running maximum, sum and output: nothing in the loop waits for another warp.  paged_decode_mma_kernel: 16-bit and fp8
 // rows; paged_decode_fma_kernel: fp32.
+#include "in_turn.cuh"
 #include "mma_common.cuh"
 
 namespace hipattn {
@@ -22,7 +23,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 using Params = hipattn_paged_decode_params_t;
 
 __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i) {
-  return is64 ? __ldg((const long long*)p + i) : (int64_t)__ldg((const int*)p + i);
+  return is64 ? __ldcg((const long long*)p + i) : (int64_t)__ldcg((const int*)p + i);
 }
 
 // sequence of entry b: its row of the table and the positions [lo, hi) it attends
@@ -100,7 +101,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // A product q.k as a logit to base 2: scale log2 e x, or with a soft-cap log2 e cap tanh(scale x / cap).  tanh(y) = 1 - 2 / (e^2y + 1) is
 // off by a few 2^-24 everywhere, which is what counts in a logit, in five instructions (tanhf, whose relative error is as small
-// near zero, and a division by the cap: 12 fp8 sequences with a soft-cap 268 us, XX so).
+// near zero, and a division by the cap: 12 fp8 sequences with a soft-cap 268 us a call, 138 so).
 struct Logit {
   float k, cap;      // cap 0: none; else k = 2 log2 e scale / cap, cap = log2 e cap.  k is positive: queries are multiplied by `sign` before
   __device__ __forceinline__ Logit(const Params& p, float scale) {
@@ -336,7 +337,7 @@ struct Place {
 };
 // Asynchronous copies of a warp's keys into its ring; a row that is not attended is sixteen zero bytes a piece (what lies there may be
 // anything, NaN too).  Lane `key` has a key's table entry fetched two rounds before its rows, into shared memory: a register that a load is
-// to fill stalls the warp when it is as much as moved (pages of one token: 206 us for 1.1 GB with entries in registers, XX so).
+// to fill stalls the warp when it is as much as moved (pages of one token, 1.1 GB of rows: 206 us with entries in registers, 192 so).
 template <class G, class At>
 struct Feeder {
   const Params& p;
@@ -415,8 +416,8 @@ struct Feeder {
   __device__ __forceinline__ Entry load_entry(int r) const {
     Entry e;
     if (const char* at = entry_at(r)) {
-      e.lo = __ldg((const uint32_t*)at);
-      if (wide) e.hi = __ldg((const uint32_t*)at + 1);
+      e.lo = __ldcg((const uint32_t*)at);
+      if (wide) e.hi = __ldcg((const uint32_t*)at + 1);
     }
     return e;
   }
@@ -545,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   const unsigned char* entries = smem + G::RING_BYTES + 2 * GT * DP + warp * (4 * KEYS * 8);
   __shared__ float s_up[16];                                             // power of two that a head's queries were multiplied by
   const int units = p.HKV * plan.tiles;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");      // (the merge waits for the whole of this grid)
+  in_turn();
 
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
   if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         qw[j] = 0u;
         if (row < g.live_heads && e < p.D) {
           const T* at = q + (int64_t)row * p.q_stride_h + e;
-          if (pairs) qw[j] = __ldg(reinterpret_cast<const uint32_t*>(at));
+          if (pairs) qw[j] = __ldcg(reinterpret_cast<const uint32_t*>(at));
           else qw[j] = (uint32_t)*reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + 1) << 16;
         }
       }
@@ -817,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   float* s_q = reinterpret_cast<float*>(smem + G::RING_BYTES);       // [GT][DP]
   const unsigned char* entries = smem + G::RING_BYTES + 4 * GT * DP + warp * (4 * KEYS * 8);
   const int units = p.HKV * plan.tiles;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  in_turn();
 
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
   if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
@@ -952,7 +953,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   sum_rounds<kMergeWarps * 32>(p, b, round, s_sum, total, before);
   const int64_t share = share_of(total * units, ctas, plan.least), begin = before * units + (int64_t)u * rounds;
   const int c0 = (int)quotient(begin, share), c1 = (int)quotient(begin + rounds - 1, share);
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");   // (every CTA: what follows on the stream waits for this grid alone)
+  in_turn();    // (the lengths do not change under the launch before)
   if (c0 == c1) return;
   const int tile = u % tiles, h0 = u / tiles * heads + tile * GT, live_heads = min(GT, heads - tile * GT);
   const float* parts = reinterpret_cast<const float*>(p.scratch) + ((int64_t)c0 * 2 + (begin == c0 * share ? 0 : 1)) * GT * PS;   // of share c0
@@ -1065,31 +1066,15 @@ struct Kernel {
     const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
     HIPATTN_REQUIRE(ctas < 0x7fffffffLL && units < 0x7fffffffLL, HIPATTN_ERR_INVALID, "paged_decode: grid of %lld blocks", (long long)ctas);
     HIPATTN_CUDA_OK(allow_smem((const void*)kern(), smem));
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cfg.attrs = at;
-    if (l.cluster > 1) {
-      at[0].id = cudaLaunchAttributeClusterDimension;
-      at[0].val.clusterDim.x = (unsigned)l.cluster;
-      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.numAttrs = 1;
-    }
-    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, kern(), p, l));
+    InTurn main(ctas, kThreads, smem, stream, l.cluster);
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&main.cfg, kern(), p, l));
     const int rc = check_launch("paged_decode_kernel");
     if (rc || !l.split) return rc;
     // few units have many parts each: one CTA per head then
     const int hb = units < kSMs ? 1 : GT, heads = p.H / p.HKV;
-    cfg.gridDim = dim3((unsigned)units, (unsigned)cdiv(heads < GT ? heads : GT, hb));
-    cfg.blockDim = dim3(kMergeWarps * 32);
-    cfg.dynamicSmemBytes = 0;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l, (int)ctas, (int)G::ROUND, hb));
+    InTurn merge(units, kMergeWarps * 32, 0, stream);
+    merge.cfg.gridDim.y = (unsigned)cdiv(heads < GT ? heads : GT, hb);
+    HIPATTN_CUDA_OK(cudaLaunchKernelEx(&merge.cfg, paged_decode_merge_kernel<DT, DP, GT>, p, l, (int)ctas, (int)G::ROUND, hb));
     return check_launch("paged_decode_merge_kernel");
   }
 };
