@@ -349,7 +349,7 @@ struct Feeder {
   uint32_t ring, entries;         // shared-memory addresses: [STAGES] stages, [4][KEYS] entries
   int page_size, page_shift, warp, lane, npc, most;
   bool wide;                      // int64 entries
-  bool same, fast;                // K and V pools are laid out alike; and rows are whole and begin within 64 GB of the pool's beginning
+  bool same, fast;                // K and V pools are laid out alike; and rows have all DP columns and begin within 64 GB of the pool's beginning
   Entry e0, e1;                   // of the segment's first two rounds
 
   // Finds the segment: its sequence, unit and rounds.  `early` is called as soon as the unit is known.  The loads do not wait for one another
@@ -403,7 +403,7 @@ struct Feeder {
     v_piece = vb + lane % G::NPC * 16;
     lane_at = At::at(G::NPC < 32 ? lane / G::NPC : 0, lane % G::NPC);
     same = p.k.stride_page == p.v.stride_page && p.k.stride_off == p.v.stride_off;
-    fast = same && npc == G::NPC && p.k.n_pages * p.k.stride_page * G::EB < (int64_t)1 << 36;
+    fast = same && npc == G::NPC && (p.k.n_pages * p.k.stride_page + page_size * p.k.stride_off) * G::EB < (int64_t)1 << 36;
   }
   // first key of this warp in round r
   __device__ __forceinline__ int key_at(int r) const { return g.lo + r * g.step + warp * G::KEYS; }

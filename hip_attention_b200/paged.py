@@ -7,7 +7,7 @@ cache_seq_lens``) and, with pages of one token, ``forward_paged_hip`` (``req_to_
 inference server around it; its configuration only says which layers and steps are dense (``hip_config.py:97-102``).
 
 Every call is stream-ordered on the current stream of the caches' device, synchronises nothing and can be captured into a
-CUDA graph.  What the device finds wrong is recorded in the status word (``read_status``): HIPATTN_STATUS_NO_PAGES (16), a
+CUDA graph.  They are calls of a server: no gradient passes through them.  What the device finds wrong is recorded in the status word (``read_status``): HIPATTN_STATUS_NO_PAGES (16), a
 pool had too few free pages; HIPATTN_STATUS_SEQUENCE (32), a call named a sequence it cannot take; pages and positions out
 of range as in the rest of the package.
 """
@@ -47,7 +47,7 @@ def write_paged_kv(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block
     (``HiPPagePool.extend``).  Sequence b (row rows[b] of the table; None: b; negative: its tokens are left out) has tokens
     token_offsets[b] : token_offsets[b + 1], or N / B of them each; tokens outside the offsets are not written.  A
     float8_e5m2 pool (or its uint8 view) receives the nearest values (ties to even, beyond the range infinity).  The rows of a
-    call must differ."""
+    call must differ: of two that are the same, which values stay is not defined."""
     host().write_kv(k, v, k_cache, v_cache, block_table, cache_seq_lens, rows, token_offsets)
 
 

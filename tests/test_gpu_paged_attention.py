@@ -334,3 +334,18 @@ def test_captured_and_replayed_on_other_lengths():
         torch.cuda.synchronize()
         for _, out in graphs:
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("D", [64, 96])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_pools_whose_tokens_lie_further_apart_than_their_pages(dtype, D):
+    """[page_size, n_pages, kv_heads, head_dim] seen as pages."""
+    from hip_attention_b200 import paged_decode_attention
+    lens = [300, 1, 77]
+    kc, vc, table, sl, keys, vals = make_pool(lens, 16, 2, D, dtype)
+    turned = [c.transpose(0, 1).contiguous().transpose(0, 1) for c in (kc, vc)]
+    assert turned[0].stride(1) > turned[0].stride(0)
+    q = torch.randn((3, 4, D), device="cuda").to(DT[dtype])
+    got, lse = paged_decode_attention(q, *turned, table, sl, sm_scale=0.1, return_lse=True)
+    check(got, lse, reference(q, keys, vals, 0.1, sixteen=dtype != "fp32"), q.dtype)
+    assert torch.equal(got, paged_decode_attention(q, kc, vc, table, sl, sm_scale=0.1))

@@ -256,3 +256,60 @@ print('fine')
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("width,n", [(64, 900), (4096, 900)])
+def test_first_launch_of_a_kernel_captured(width, n):
+    """The first call that joins parts (in a cluster; over shares, with a second launch) may be a captured one."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = f"""
+import torch
+from hip_attention_b200 import paged_decode_attention, read_status
+kc, vc = (torch.randn((64, 16, 2, 64), device='cuda').half() for _ in range(2))
+table = torch.zeros((1, {width}), dtype=torch.int32, device='cuda')
+table[0, :64] = torch.randperm(64, device='cuda')
+q, lens = torch.randn((1, 4, 64), device='cuda').half(), torch.tensor([{n}], device='cuda')
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = paged_decode_attention(q, kc, vc, table, lens)
+graph.replay()
+assert torch.equal(out, paged_decode_attention(q, kc, vc, table, lens)) and out.abs().sum() > 0 and read_status('cuda') == 0
+print('fine')
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("before", ["copy", "fill", "other stream", "kernel", "nothing"])
+def test_captured_behind_anything(before):
+    """What a captured call reads may come from a copy, a fill, a kernel or another stream."""
+    from hip_attention_b200 import paged_decode_attention
+    g = torch.Generator(device="cuda").manual_seed(0)
+    kc, vc = (torch.randn((64, 16, 2, 64), generator=g, device="cuda") for _ in range(2))
+    q, table, lens = torch.randn((1, 4, 64), generator=g, device="cuda"), torch.randperm(64, generator=g, device="cuda")[None], torch.tensor([900], device="cuda")
+    want = paged_decode_attention(q, kc, vc, table, lens)
+    host, q2, side = q.cpu().pin_memory(), torch.zeros_like(q), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cur = torch.cuda.current_stream()
+        if before == "copy":
+            q2.copy_(host, non_blocking=True)
+        elif before == "other stream":
+            side.wait_stream(cur)
+            with torch.cuda.stream(side):
+                q2.copy_(q)
+            cur.wait_stream(side)
+        elif before != "nothing":
+            torch.mul(q, 1.0, out=q2)
+            if before == "fill":
+                torch.zeros(4096, device="cuda")
+        outs = [paged_decode_attention(q if before == "nothing" else q2, kc, vc, table, lens) for _ in range(2)]
+    q2.zero_()
+    for _ in range(10):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
