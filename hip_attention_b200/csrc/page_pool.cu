@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
 // copies of pages
 // ---------------------------------------------------------------------------------------------------
 constexpr int kCopyThreads = 256;
-constexpr int kCopyBytes = 16384;     // of a page, to a CTA at a time: four 16-byte pieces a thread in flight
+constexpr int kCopyBytes = 16384;     // of a page, to a CTA at a time: four 16-byte pieces a thread in flight (begun pages of 96 beams in
+                                      // 32 caches, 768 MB in and out: 121 us, 6.35 TB/s; 398 MB moved: 137 us, 5.8)
 
 __device__ __forceinline__ void copy_piece(const char* src, char* dst, int64_t bytes) {
   uint4 v[kCopyBytes / 16 / kCopyThreads];
@@ -485,6 +486,8 @@ __device__ __forceinline__ uint2 narrow_e5m2(const uint4& w) {
 
 // A CTA writes `span` consecutive tokens: their slots are looked up once, by one thread each, while the first rows are on their way.  A
 // thread keeps its place in the row (keys or values, head, elements) and goes from token to token, `lanes` threads to a token.
+// Bound: HBM; 17600 tokens of 8 KV heads into an fp8 pool (108 MB): 109 us with a thread to a piece, which looked everything up for itself
+// and rounded by way of the library's conversion, 22 so.  A step's 32 tokens: 2.6 us.
 constexpr int kWriteThreads = 256;
 constexpr int kMaxSpan = 32;
 constexpr int kWriteAhead = 4;    // 16-byte pieces of a thread in flight

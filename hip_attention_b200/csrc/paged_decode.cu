@@ -9,6 +9,9 @@
 // A warp takes KEYS keys at a time from a ring of its own in shared memory, filled with 16-byte asynchronous copies, and keeps
 // its own running maximum, sum and output: nothing in the loop waits for another warp.  paged_decode_mma_kernel: 16-bit and fp8
 // rows; paged_decode_fma_kernel: fp32.
+//
+// Measured: one sequence of 1048571 tokens, bf16, 8 KV heads of dimension 128 (4.3 GB) 620 us, 6.9 TB/s; 32 sequences of up to 16384
+// tokens (1.18 GB) 180 us, 6.5 TB/s; 12 fp8 sequences in pages of one token, soft-capped (0.56 GB) 111 us, 5.0 TB/s; one sequence of 389 tokens 5.0 us.
 #include "in_turn.cuh"
 #include "mma_common.cuh"
 
@@ -1010,6 +1013,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   }
 }
 
+// The layout's bounds, in rounds.  A cluster whose CTAs have more than sixteen each gains less from its missing second launch (3 to 4 us)
+// than it loses where lengths differ.  Units to a CTA each: 32 sequences of up to 800 tokens 16 us, in shares 29; 64 of up to 2000 73 and 80;
+// 40 of up to 3000 (48 rounds) 53 and 59.
 constexpr int kLeastRounds = 2;       // rounds of a share
 constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
 constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster

@@ -336,7 +336,7 @@ typedef struct hipattn_paged_decode_params {
   float sm_scale, logit_softcap;
 } hipattn_paged_decode_params_t;
 
-int64_t hipattn_paged_decode_scratch(const hipattn_paged_decode_params_t* p);  /* reads shapes only; 0: none needed */
+int64_t hipattn_paged_decode_scratch(const hipattn_paged_decode_params_t* p);  /* for the current device; reads shapes only; 0: none needed */
 int hipattn_paged_decode(const hipattn_paged_decode_params_t* p, void* stream);
 
 /*
