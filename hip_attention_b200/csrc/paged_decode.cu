@@ -671,7 +671,6 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
             for (int e = 0; e < GT / 4; ++e) s[n][e] += s2[n][e];
         }
-        feed.next(r, slot);
         // the first values on their way while the weights are made
         uint32_t vf[AHEAD > 0 ? AHEAD : 1][4];
 #pragma unroll
@@ -727,6 +726,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[n][e] *= alpha[GT == 16 ? e >> 1 : 0];
         }
+        feed.next(r, slot);
         // ---- O += P V ----
         auto product = [&](int n, int c, uint32_t b0, uint32_t b1) {
           mma16816<MT>(o[n], pa[c], b0, b1);
