@@ -61,12 +61,12 @@ __device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
 // rounds of a unit; an empty sequence has one, which writes its zeros
 __device__ __forceinline__ int rounds_of(const Sequence& s, int round) { return max(1, (s.hi - s.lo + round - 1) / round); }
 
-// Sum of rounds over all sequences (`total`) and over those before sequence b (`before`), for the merge kernel; all threads.
+// Sum of rounds (and `extra` each) over all sequences (`total`) and over those before sequence b (`before`), for the merge kernel; all threads.
 template <int THREADS>
-__device__ __forceinline__ void sum_rounds(const Params& p, int b, int round, int64_t* s_sum, int64_t& total, int64_t& before) {
+__device__ __forceinline__ void sum_rounds(const Params& p, int b, int round, int extra, int64_t* s_sum, int64_t& total, int64_t& before) {
   int64_t t = 0, f = 0;
   for (int i = threadIdx.x; i < p.B; i += THREADS) {
-    const int r = rounds_of(sequence_of(p, i), round);
+    const int r = rounds_of(sequence_of(p, i), round) + extra;
     t += r;
     if (i < b) f += r;
   }
@@ -123,6 +123,7 @@ struct Logit {
 // How a call is laid out.  split: every CTA takes a share of the row of rounds.  Else a unit is a CTA's, or a cluster's.
 struct Plan {
   int tiles, split, least, cluster;   // head tiles of a KV head; rounds that a share has at least
+  int extra;                          // rounds that beginning and ending a unit counts for in a share
   int vector_out;                     // output rows begin where four elements can be stored at once
 };
 
@@ -172,15 +173,15 @@ struct Share {
   int b;
 };
 // false: the share is empty.  All threads.
-__device__ __forceinline__ bool find_share(const Params& p, int units, int round, int least, Share& sh) {
+__device__ __forceinline__ bool find_share(const Params& p, int units, int round, const Plan& plan, Share& sh) {
   __shared__ int64_t s_scan[2][kWarps];
   __shared__ int64_t s_found[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int64_t total = 0, x = 0, sum = 0;
-  // rounds of sequence c + tid (x) and of those of [c, c + tid] (sum); the sum over the CTA is returned
+  // rounds (and extra) of sequence c + tid (x) and of those of [c, c + tid] (sum); the sum over the CTA is returned
   auto scan = [&](int c, int turn) {
     const int i = c + tid;
-    x = sum = i < p.B ? rounds_of(sequence_of(p, i), round) : 0;
+    x = sum = i < p.B ? rounds_of(sequence_of(p, i), round) + plan.extra : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
@@ -198,7 +199,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int units, int round
   };
   int turn = 0;
   for (int c = 0; c < p.B; c += kThreads) total += scan(c, turn++);
-  const int64_t share = share_of(total * units, gridDim.x, least);
+  const int64_t share = share_of(total * units, gridDim.x, plan.least);
   sh.first = share * blockIdx.x;
   sh.last = min(sh.first + share, total * units);
   if (sh.first >= sh.last) return false;
@@ -222,7 +223,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int units, int round
 // its rounds in turn.
 struct Segment {
   Sequence seq;
-  int rounds, r0, r1, lo, step, hkv, h0, live_heads;
+  int rounds, r0, r1, lo, step, hkv, h0, live_heads, used;      // used: what it takes of the share
 };
 __device__ __forceinline__ void set_unit(const Params& p, Segment& g, int u, int tiles, int gt) {
   const int heads = p.H / p.HKV, tile = u % tiles;
@@ -239,6 +240,17 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, int rank) {   // th
   asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
   return v;
+}
+
+// The share moves on behind a segment; false: that was the last
+__device__ __forceinline__ bool next_segment(const Segment& g, Share& sh, int units, const Plan& plan) {
+  sh.first += g.used;
+  if (sh.first >= sh.last) return false;
+  if (sh.first == sh.unit_at + (int64_t)(g.rounds + plan.extra) * units) {
+    sh.unit_at = sh.first;
+    ++sh.b;
+  }
+  return true;
 }
 
 // The segment's result from the warps' parts, s_merge [kWarps][GT][DP + 4]: to the output, to scratch, or (a cluster) to s_cta [GT][DP + 4],
@@ -316,14 +328,7 @@ __device__ __forceinline__ bool end_segment(const Params& p, const Segment& g, S
     cluster_arrive();
     cluster_wait();   // no CTA leaves while another reads its shared memory
   }
-  if (!plan.split) return false;
-  sh.first += g.r1 - g.r0;
-  if (sh.first >= sh.last) return false;
-  if (sh.first == sh.unit_at + (int64_t)g.rounds * units) {
-    sh.unit_at = sh.first;
-    ++sh.b;
-  }
-  return true;
+  return plan.split && next_segment(g, sh, units, plan);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t smem_addr, const void* gmem) {
@@ -385,11 +390,14 @@ struct Feeder {
     g.rounds = rounds_of(g.seq, G::ROUND);
     g.lo += g.seq.lo;
     if (plan.split) {
-      const int64_t from = sh.first - sh.unit_at, u = quotient(from, g.rounds);
+      const int size = g.rounds + plan.extra;      // of a unit: what it takes to begin it, then its rounds
+      const int64_t from = sh.first - sh.unit_at, u = quotient(from, size);
       set_unit(p, g, (int)u, plan.tiles, gt);
       early(g);
-      g.r0 = (int)(from - u * g.rounds);
-      g.r1 = (int)min((int64_t)g.rounds, g.r0 + (sh.last - sh.first));
+      const int begin = (int)(from - u * size), end = (int)min((int64_t)size, begin + (sh.last - sh.first));
+      g.used = end - begin;
+      g.r0 = max(0, begin - plan.extra);
+      g.r1 = max(0, end - plan.extra);
     } else {
       g.r1 = max(0, (g.rounds - rank + plan.cluster - 1) / plan.cluster);
     }
@@ -552,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   in_turn();
 
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
-  if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
+  if (plan.split && !find_share(p, units, G::ROUND, plan, sh)) return;
   const int64_t share_first = sh.first;
   // rows and pieces of ldmatrix: 16-bit K eight keys by two pieces twice, fp8 K a piece of all keys or two of sixteen, V sixteen keys by two
   const uint32_t k_lane = F8 ? (KEYS == 32 ? P::at(lane, 0) : P::at(lane & 15, lane >> 4)) : P::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
@@ -587,6 +595,10 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
     };
     const Feeder<G, P> feed(p, sh, plan, units, GT, warp, lane, ring, entries, load_queries);
     const Segment& g = feed.g;
+    if (plan.split && g.r0 == g.r1) {      // (the share has no round of the unit, only its beginning)
+      more = next_segment(g, sh, units, plan);
+      continue;
+    }
     feed.begin();
     if constexpr (F8 && DT == HIPATTN_BF16) {
       for (int h = warp; h < GT; h += kWarps) {
@@ -824,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   in_turn();
 
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
-  if (plan.split && !find_share(p, units, G::ROUND, plan.least, sh)) return;
+  if (plan.split && !find_share(p, units, G::ROUND, plan, sh)) return;
   const int64_t share_first = sh.first;
   const Logit logit(p, p.sm_scale);
 
@@ -841,6 +853,10 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
     };
     const Feeder<G, P> feed(p, sh, plan, units, GT, warp, lane, ring, entries, load_queries);
     const Segment& g = feed.g;
+    if (plan.split && g.r0 == g.r1) {      // (the share has no round of the unit, only its beginning)
+      more = next_segment(g, sh, units, plan);
+      continue;
+    }
     feed.begin();
 #pragma unroll
     for (int j = 0; j < GT * DP / kThreads; ++j) s_q[j * kThreads + tid] = qw[j] * Logit::sign(p);
@@ -953,13 +969,13 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   const int b = blockIdx.x / units, u = blockIdx.x % units;
   const int rounds = rounds_of(sequence_of(p, b), round);
   int64_t total, before;
-  sum_rounds<kMergeWarps * 32>(p, b, round, s_sum, total, before);
-  const int64_t share = share_of(total * units, ctas, plan.least), begin = before * units + (int64_t)u * rounds;
-  const int c0 = (int)quotient(begin, share), c1 = (int)quotient(begin + rounds - 1, share);
+  sum_rounds<kMergeWarps * 32>(p, b, round, plan.extra, s_sum, total, before);
+  const int64_t share = share_of(total * units, ctas, plan.least), begin = before * units + (int64_t)u * (rounds + plan.extra);
+  const int c0 = (int)quotient(begin + plan.extra, share), c1 = (int)quotient(begin + plan.extra + rounds - 1, share);
   in_turn();    // (the lengths do not change under the launch before)
   if (c0 == c1) return;
   const int tile = u % tiles, h0 = u / tiles * heads + tile * GT, live_heads = min(GT, heads - tile * GT);
-  const float* parts = reinterpret_cast<const float*>(p.scratch) + ((int64_t)c0 * 2 + (begin == c0 * share ? 0 : 1)) * GT * PS;   // of share c0
+  const float* parts = reinterpret_cast<const float*>(p.scratch) + ((int64_t)c0 * 2 + (begin <= c0 * share ? 0 : 1)) * GT * PS;   // of share c0
   const float* later = reinterpret_cast<const float*>(p.scratch);                                                               // of share c: c * 2 * GT * PS
   const int per_head = hb < kMergeWarps ? kMergeWarps / hb : 1;           // warps of a head
   for (int i0 = 0; i0 < hb; i0 += kMergeWarps / per_head) {
@@ -1017,6 +1033,10 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
 // than it loses where lengths differ.  Units to a CTA each: 32 sequences of up to 800 tokens 16 us, in shares 29; 64 of up to 2000 73 and 80;
 // 40 of up to 3000 (48 rounds) 53 and 59.
 constexpr int kLeastRounds = 2;       // rounds of a share
+// Beginning and ending a unit takes as long as some four rounds (2.5 us); without them in the shares' sizes a CTA that got a dozen short or
+// empty sequences ended last by far (64 sequences of up to 1000 tokens behind a wide table: 50 us, 34 so).  Few units are cut as small as they may be.
+constexpr int kUnitRounds = 4;
+constexpr int kManyUnits = 64;
 constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
 constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
 constexpr int kWholeRounds = 64;      // most rounds of a unit that is a CTA's
@@ -1036,12 +1056,13 @@ struct Kernel {
   static Plan plan(const Params& p, int64_t* ctas) {
     Plan l;
     l.tiles = cdiv(p.H / p.HKV, GT);
-    l.least = kLeastRounds;
     l.split = 0;
     l.cluster = 1;
     constexpr int EB = Elem<DT>::bytes;
     l.vector_out = ((uintptr_t)p.out | (uintptr_t)(p.o_stride_b * EB) | (uintptr_t)(p.o_stride_h * EB)) % (4 * EB) == 0;
     const int64_t units = (int64_t)p.B * p.HKV * l.tiles;
+    l.extra = units >= kManyUnits ? kUnitRounds : 0;
+    l.least = kLeastRounds + l.extra;
     int64_t most = (int64_t)p.k.table_width * p.k.page_size;
     if (p.window > 0 && p.window < most) most = p.window;
     const int64_t rounds = (most + G::ROUND - 1) / G::ROUND;      // a unit has at most
