@@ -1525,6 +1525,11 @@ PyObject* page_pool(PyObject* const* argv) {
   h->keep.push_back(lens);
   h->keep.push_back(table);
   p.status = (uint32_t*)status_word(h->dev.index()).data_ptr();
+  // the plans of forks and compactions: calls on one pool are ordered, so one buffer serves all of them
+  const c10::cuda::CUDAGuard guard(h->dev);
+  const at::Tensor scratch = Device{h->dev}.empty({std::max(hipattn_pool_scratch(&p, HIPATTN_POOL_MAX_ENTRIES), hipattn_pool_scratch(&p, 0))}, at::kByte);
+  p.scratch = scratch.data_ptr();
+  h->keep.push_back(scratch);
   PyObject* o = PyCapsule_New(h.get(), kPoolName, drop_pool);
   if (o) h.release();
   return o;
@@ -1564,10 +1569,7 @@ PyObject* pool_fork(PyObject* const* argv) {
   if (parents.size(0) != children.size(0)) VALUE_ERROR("%lld parents, but %lld children", (long long)parents.size(0), (long long)children.size(0));
   const int n = (int)parents.size(0);
   if (n == 0) Py_RETURN_NONE;
-  hipattn_page_pool_t p = h->pool;
-  const at::Tensor scratch = Device{h->dev}.empty({hipattn_pool_scratch(&p, n)}, at::kByte);
-  p.scratch = scratch.data_ptr();
-  check(hipattn_pool_fork(&p, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), n, c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "fork");
+  check(hipattn_pool_fork(&h->pool, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), n, c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "fork");
   Py_RETURN_NONE;
 }
 // pool_free(handle, rows)
@@ -1583,11 +1585,8 @@ PyObject* pool_free(PyObject* const* argv) {
 PyObject* pool_compact(PyObject* const* argv) {
   PoolHandle* h = pool_of(argv[0]);
   const c10::cuda::CUDAGuard guard(h->dev);
-  const Device mem{h->dev};
-  hipattn_page_pool_t p = h->pool;
-  const at::Tensor scratch = mem.empty({hipattn_pool_scratch(&p, 0)}, at::kByte), in_use = mem.empty({1}, at::kInt);
-  p.scratch = scratch.data_ptr();
-  check(hipattn_pool_compact(&p, in_use.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "compact");
+  const at::Tensor in_use = Device{h->dev}.empty({1}, at::kInt);
+  check(hipattn_pool_compact(&h->pool, in_use.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "compact");
   return wrap(in_use);
 }
 

@@ -1030,8 +1030,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
 }
 
 // The layout's bounds, in rounds.  A cluster whose CTAs have more than sixteen each gains less from its missing second launch (3 to 4 us)
-// than it loses where lengths differ.  Units to a CTA each: 32 sequences of up to 800 tokens 16 us, in shares 29; 64 of up to 2000 73 and 80;
-// 40 of up to 3000 (48 rounds) 53 and 59.
+// than it loses where lengths differ.  Units to a CTA each: 32 sequences of up to 800 tokens (13 rounds) 16 us, in shares 19; 64 of 600 tokens 32
+// and 37; 64 of 2000 (32 rounds) 87 and 90, of up to 2000 60 and 55; 40 of 3000 (47 rounds) 107 and 84.
 constexpr int kLeastRounds = 2;       // rounds of a share
 // Beginning and ending a unit takes as long as some four rounds (2.5 us); without them in the shares' sizes a CTA that got a dozen short or
 // empty sequences ended last by far (64 sequences of up to 1000 tokens behind a wide table: 50 us, 34 so).  Few units are cut as small as they may be.
@@ -1039,7 +1039,7 @@ constexpr int kUnitRounds = 4;
 constexpr int kManyUnits = 64;
 constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
 constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
-constexpr int kWholeRounds = 64;      // most rounds of a unit that is a CTA's
+constexpr int kWholeRounds = 24;      // most rounds of a unit that is a CTA's
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
@@ -1137,7 +1137,8 @@ int validate(const Params* p) {
                   HIPATTN_ERR_INVALID, "paged_decode: k and v must be pools of the same pages and type");
   HIPATTN_REQUIRE(p->rows || p->n_rows >= p->B, HIPATTN_ERR_INVALID, "paged_decode: %d entries, but a table of %d rows", p->B, p->n_rows);
   HIPATTN_REQUIRE(p->window >= 0, HIPATTN_ERR_INVALID, "paged_decode: window %d is negative", p->window);
-  HIPATTN_REQUIRE(p->logit_softcap >= 0.f && p->sm_scale == p->sm_scale, HIPATTN_ERR_INVALID, "paged_decode: bad scale or soft-cap");
+  HIPATTN_REQUIRE(p->logit_softcap >= 0.f && p->logit_softcap < INFINITY && fabsf(p->sm_scale) < INFINITY, HIPATTN_ERR_INVALID,
+                  "paged_decode: scale %g and soft-cap %g must be finite, the cap not negative", p->sm_scale, p->logit_softcap);
   const int eb = p->dtype == HIPATTN_F32 ? 4 : 2;
   int rc = validate_tokens(p->k, eb, p->D, "k");
   if (rc) return rc;

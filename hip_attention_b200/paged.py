@@ -34,6 +34,10 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     ``sliding_window`` only the last so many positions are attended.  Keys are used as they lie in the pool: rotate them
     before they are written.
 
+    How the work is laid out follows from the width of ``block_table``, which is all the host knows of the lengths: give the
+    columns that the longest sequence can need (``block_table[:, :w]``; one sequence of 389 tokens takes 7 us behind a table of 400 and 12 us
+    behind one of 131072).
+
     Returns the context [B, H, D] (in ``out`` when given) and, with ``return_lse``, the base-2 log-sum-exp [B, H] (float32).
     A sequence without tokens gives zeros and -inf."""
     return host().paged_decode(q, k_cache, v_cache, block_table, cache_seq_lens, rows, sm_scale, sliding_window, logit_softcap, return_lse, out)

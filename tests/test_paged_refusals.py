@@ -30,7 +30,7 @@ def _decode(tok=None, **kw):
 @pytest.mark.parametrize("kw, tok, code", [
     (dict(B=0), {}, 1), (dict(H=5), {}, 1), (dict(D=0), {}, 1), (dict(dtype=7), {}, 1), (dict(D=264), {}, 2), (dict(D=68), {}, 1),
     (dict(n_rows=1), {}, 1), (dict(window=-1), {}, 1), (dict(logit_softcap=-1.0), {}, 1), (dict(logit_softcap=float("nan")), {}, 1),
-    (dict(sm_scale=float("nan")), {}, 1), (dict(q=None), {}, 1), (dict(out=None), {}, 1), (dict(status=None), {}, 1),
+    (dict(sm_scale=float("nan")), {}, 1), (dict(sm_scale=float("-inf")), {}, 1), (dict(logit_softcap=float("inf")), {}, 1), (dict(q=None), {}, 1), (dict(out=None), {}, 1), (dict(status=None), {}, 1),
     ({}, dict(cache=None), 1), ({}, dict(block_table=None), 1), ({}, dict(page_size=0), 1), ({}, dict(table_width=0), 1),
     ({}, dict(stride_off=129), 1), ({}, dict(cache=4100), 1), (dict(dtype=0), dict(fp8_e5m2=1), 2), (dict(D=72), dict(fp8_e5m2=1), 2),
     ({}, dict(fp8_e5m2=1, stride_ch=136), 2),
