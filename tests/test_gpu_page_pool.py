@@ -109,7 +109,7 @@ def same(pool, model, caches, contents=True):
 
 
 @pytest.mark.parametrize("seed", range(6))
-@pytest.mark.parametrize("n_pages,P,R,W,layout", [(61, 4, 9, 12, "plain"), (40, 1, 6, 30, "plain"), (500, 16, 33, 40, "interleaved"), (17, 5, 5, 7, "interleaved")])
+@pytest.mark.parametrize("n_pages,P,R,W,layout", [(61, 4, 9, 12, "plain"), (40, 1, 6, 30, "plain"), (500, 16, 33, 40, "interleaved"), (17, 5, 5, 7, "interleaved"), (9000, 2, 20, 900, "plain")])
 def test_random_calls_equal_the_model(seed, n_pages, P, R, W, layout):
     """Any calls in any order, among them calls that cannot be carried out."""
     from hip_attention_b200 import read_status
