@@ -627,12 +627,15 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
     const Logit logit0(p, F8 && DT == HIPATTN_BF16 ? p.sm_scale / s_up[gr] : p.sm_scale);
     const Logit logit1(p, F8 && DT == HIPATTN_BF16 && GT == 16 ? p.sm_scale / s_up[gr + 8] : p.sm_scale);
 
-    float o[NT][4], m_run[GT / 8], l_run[GT / 8];
+    // b_run: what the logits are lowered by before they become weights, the running maximum less kShift.  It is this base that a round keeps or
+    // moves, so that sums of rounds with one maximum stay as they are: the factor to them has to be exactly 1 there (from the maxima, with
+    // the shift subtracted again, it is off by up to 2^-16 for logits near -256, in every round alike: 3e-3 of the output after 1024 rounds).
+    float o[NT][4], b_run[GT / 8], l_run[GT / 8];
     for (bool two = true;; two = false) {      // (a second time only for sixteen heads, and where there is NaN)
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < GT / 8; ++i) { m_run[i] = -INFINITY; l_run[i] = 0.f; }
+      for (int i = 0; i < GT / 8; ++i) { b_run[i] = -INFINITY; l_run[i] = 0.f; }
       int slot = 0;
       for (int r = g.r0; r < g.r1; ++r) {
         cp_async_wait<1>();
@@ -716,8 +719,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           for (int n = 1; n < KEYS / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float m_new = fmaxf(m_run[i], mx * k), base = (m_new > -INFINITY ? m_new : 0.f) - kShift;
-          alpha[i] = ex2(m_run[i] - base - kShift);
+          const float b_new = fmaxf(b_run[i], fmaf(mx, k, -kShift)), base = b_new > -INFINITY ? b_new : 0.f;
+          alpha[i] = ex2(b_run[i] - base);
           float sum = 0.f;
 #pragma unroll
           for (int n = 0; n < KEYS / 8; ++n) {
@@ -729,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
             else pl[n / 2][(n & 1) * 2 + i] = lo;
           }
           l_run[i] = l_run[i] * alpha[i] + sum;      // (this lane's keys; the four lanes of a row are added up at the end)
-          m_run[i] = m_new;
+          b_run[i] = b_new;
           moved |= alpha[i] != 1.f;
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
 #pragma unroll
         for (int e = 0; e < 2; ++e) dst[F8 ? (n >> 1) * 16 + (2 * jq + e) * 2 + (n & 1) : n * 8 + 2 * jq + e] = o[n][2 * i + e];
       if (jq == 0) {
-        dst[DP] = m_run[i] - kShift;       // (numerator and denominator are 2^kShift times as large)
+        dst[DP] = b_run[i];
         dst[DP + 1] = l_run[i];
       }
     }

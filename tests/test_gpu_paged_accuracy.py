@@ -1,0 +1,77 @@
+"""Exact decode attention where errors could pile up or be hidden: long sequences far from zero, caps of any size, values that are not
+finite beside others that are.  Pools whose logits are exact in 32 bits, against 64 bits.
+
+What the kernels may be off by, from their arithmetic (u = 2^-24; T: rounds of a warp, of `keys` keys each; S parts of a unit):
+* a weight exp2(s k - base), s exact: k = log2 e rounded moves it by |s - s_max| u relative (the base is common to all); the
+  difference, within [-4, 16), is rounded by 2^-21, exp2 is off by 2 ulp: together below W = 2^-20;
+* 16-bit products take a weight in two terms; what is left out is 2^-22 of it in half precision;
+* the denominator: one rounding a round, 16 within it, S parts: (T + 16 + S) u;
+* a numerator: a tensor core's step adds 16 products to the sum so far and may cut each of the 17 at the last bit of the largest:
+  17 u of that sum, which grows in equal steps, so that T keys / 16 steps (twice as many where the second term is a product of its own)
+  have half of 17 u each of the end; and S parts: 2 u each;
+* the log-sum-exp adds the base and the logarithm of a denominator below 2^36, off by one ulp of 36: 2^-18; log2 e a itself is off by u."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_paged_attention import DT, FP8
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+SMS = 148
+
+
+def offset_pool(n, page, HKV, D, cache_type, seed):
+    """Keys (1, x_t, 0, ...) with x_t a quarter's multiple in [-1, 0]: q = (a, 1, 0, ...) gives the logit a + x_t without a rounding.  Values: even
+    columns 1 in the first half of the sequence and 0 behind it, odd ones N(0, 1)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    n_pages = -(-n // page)
+    table = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)[None]
+    t = torch.arange(n, device="cuda")
+    x = torch.randint(-4, 1, (n,), generator=g, device="cuda") / 4.0
+    x[n // 3] = 0.0
+    v = torch.randn((n, HKV, D), generator=g, device="cuda")
+    v[:, :, ::2] = (t < n // 2).float()[:, None, None]
+    k = torch.zeros((n, HKV, D), device="cuda")
+    k[:, :, 0], k[:, :, 1] = 1.0, x[:, None]
+    caches = []
+    for rows in (k, v):
+        c = torch.zeros((n_pages * page, HKV, D), device="cuda")
+        c[table[0, t // page].long() * page + t % page] = rows
+        caches.append(c.to(cache_type).view(n_pages, page, HKV, D))
+    return caches[0], caches[1], table, x.double(), v.to(cache_type).double()
+
+
+@pytest.mark.parametrize("B,n", [(40, 32768), (1, 131072)])
+@pytest.mark.parametrize("G", [8, 16])
+@pytest.mark.parametrize("dtype,fp8,D", [("fp16", False, 64), ("fp16", False, 128), ("bf16", True, 64), ("fp16", True, 128), ("bf16", False, 128)])
+def test_an_offset_of_all_logits_changes_nothing(dtype, fp8, D, G, B, n):
+    """A constant added to all logits leaves the softmax as it is and the log-sum-exp moves by it, however many rounds a sequence takes."""
+    from hip_attention_b200 import paged_decode_attention
+    HKV = 2
+    kc, vc, table, x, v = offset_pool(n, 64, HKV, D, FP8 if fp8 else DT[dtype], seed=G + D)
+    H = HKV * G
+    i = torch.arange(B * H, device="cuda")
+    low = torch.tensor([-16.0, -64.0, -256.0], device="cuda")[i % 3]        # largest logit to base 2: fourteen below a power of two, where the shift rounds
+    a = ((low + 14.0 * ((i * 0.6180339887498949) % 1.0)) * math.log(2)).view(B, H).to(DT[dtype])
+    q = torch.zeros((B, H, D), dtype=DT[dtype], device="cuda")
+    q[:, :, 0], q[:, :, 1] = a, 1.0
+    out, lse = paged_decode_attention(q, kc, vc, table, torch.tensor([n], device="cuda"), rows=torch.zeros(B, dtype=torch.int32, device="cuda"), return_lse=True)
+    p = torch.softmax(x, 0)
+    want, size = (torch.einsum("t,thd->hd", p, w).repeat_interleave(G, 0) for w in (v, v.abs()))
+    want_lse = (a.double() + torch.logsumexp(x, 0)) / math.log(2)
+    row = D * (1 if fp8 else 2)
+    keys = 32 if row <= 128 else 16
+    T = math.ceil(B * HKV * math.ceil(n / (4 * keys)) / SMS) + 1            # (at least one CTA to a multiprocessor)
+    S = 4 + 3 * SMS
+    weight = 2.0 ** -20
+    steps = T * (keys // 16) * (1 if G == 8 else 2)
+    den = (T + 16 + S) * U + weight
+    two_terms = 2.0 ** -16 if dtype == "bf16" and not fp8 else 2.0 ** -22
+    tol = size * (weight + two_terms + den + steps * 17 * U / 2 + 2 * S * U) + torch.finfo(q.dtype).eps / 2 * want.abs()
+    err = (out.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by {(err / tol).max().item():.3g} of the bound"
+    tol = (want_lse.abs() + a.double().abs() / math.log(2)) * 2 * U + den / math.log(2) + 2.0 ** -18
+    err = (lse.double() - want_lse).abs()
+    assert bool((err <= tol).all()), f"lse off by {(err / tol).max().item():.3g} of the bound"
