@@ -12,6 +12,8 @@
 //
 // Measured: one sequence of 1048571 tokens, bf16, 8 KV heads of dimension 128 (4.3 GB) 620 us, 6.9 TB/s; 32 sequences of up to 16384
 // tokens (1.18 GB) 180 us, 6.5 TB/s; 12 fp8 sequences in pages of one token, soft-capped (0.56 GB) 111 us, 5.0 TB/s; one sequence of 389 tokens 5.0 us.
+#include <cfloat>
+
 #include "in_turn.cuh"
 #include "mma_common.cuh"
 
@@ -102,20 +104,30 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
-// A product q.k as a logit to base 2: scale log2 e x, or with a soft-cap log2 e cap tanh(scale x / cap).  tanh(y) = 1 - 2 / (e^2y + 1) is
-// off by a few 2^-24 everywhere, which is what counts in a logit, in five instructions (tanhf, whose relative error is as small
-// near zero, and a division by the cap: 12 fp8 sequences with a soft-cap 268 us a call, 138 so).
+// A product q.k as a logit to base 2: scale log2 e x, or with a soft-cap log2 e cap tanh(scale x / cap), in one of two forms.
+// Short: tanh(y) = 1 - 2 / (e^2y + 1), off by a few 2^-24 of the cap, in five instructions.  For 16-bit products and caps up to kShortCap, where that
+// is below 2^-16, what the two 16-bit terms of a weight keep.
+// Else (fp32 products, larger caps): tanhf, off by a few 2^-24 of the logit itself, and the plain logit where the cap changes less than 2^-25 of it, so
+// that a cap far above the logits changes nothing.  Kernels of their own: 12 fp8 sequences with a cap of 30 115 us in the short form, 124 in this one, and
+// with both in one kernel others lose 4 % to it that have no cap at all.  fp32, 16 sequences of up to 16384: 247 us in the short form, 260 in this one.
+constexpr float kShortCap = 64.f;
 struct Logit {
-  float k, cap;      // cap 0: none; else k = 2 log2 e scale / cap, cap = log2 e cap.  k is positive: queries are multiplied by `sign` before
-  __device__ __forceinline__ Logit(const Params& p, float scale) {
+  float k, cap;      // cap 0: none, else log2 e cap.  k = log2 e scale, short form 2 log2 e scale / cap.  k is positive: queries are multiplied by `sign` before
+  __device__ __forceinline__ Logit(const Params& p, float scale, bool is_short) {
     const float size = scale == 0.f ? 1.f : fabsf(scale);
-    cap = p.logit_softcap * kLog2e;
-    k = p.logit_softcap > 0.f ? 2.f * kLog2e * size / p.logit_softcap : kLog2e * size;
+    cap = fminf(p.logit_softcap * kLog2e, FLT_MAX);
+    k = kLog2e * size;
+    if (p.logit_softcap > 0.f && is_short) k = fminf(2.f * kLog2e * size / p.logit_softcap, FLT_MAX);
   }
-  __device__ __forceinline__ float capped(float x) const {
+  __device__ __forceinline__ float capped_short(float x) const {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(ex2(x * k) + 1.f));
     return fmaf(-2.f * cap, r, cap);
+  }
+  __device__ __forceinline__ float per_cap() const { return fminf(k / cap, FLT_MAX); }     // scale / cap
+  __device__ __forceinline__ float capped(float x, float per_cap) const {
+    const float y = x * per_cap;
+    return fabsf(y) < 0x1p-12f ? x * k : cap * tanhf(y);
   }
   __device__ static __forceinline__ float sign(const Params& p) { return p.sm_scale > 0.f ? 1.f : (p.sm_scale < 0.f ? -1.f : 0.f); }
 };
@@ -540,7 +552,7 @@ struct MmaPlace : Place<RB, MmaPlace<RB>> {   // the eight rows that ldmatrix re
   __device__ static __forceinline__ constexpr int turn(int key) { return RB >= 128 ? key & 7 : (key >> 1) & (RB / 16 - 1); }
 };
 
-template <int DT, bool F8, int DP, int GT>
+template <int DT, bool F8, int DP, int GT, bool LONG_CAP>
 __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_mma_kernel(const Params p, const Plan plan) {
   using G = Geo<DT, F8, DP>;
   using P = MmaPlace<G::RB>;
@@ -624,8 +636,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
       s_q[j * kThreads + tid] = pack2<MT>(lower<DT>(qw[j]) * up, upper<DT>(qw[j]) * up);
     }
     __syncthreads();
-    const Logit logit0(p, F8 && DT == HIPATTN_BF16 ? p.sm_scale / s_up[gr] : p.sm_scale);
-    const Logit logit1(p, F8 && DT == HIPATTN_BF16 && GT == 16 ? p.sm_scale / s_up[gr + 8] : p.sm_scale);
+    const Logit logit0(p, F8 && DT == HIPATTN_BF16 ? p.sm_scale / s_up[gr] : p.sm_scale, !LONG_CAP);
+    const Logit logit1(p, F8 && DT == HIPATTN_BF16 && GT == 16 ? p.sm_scale / s_up[gr + 8] : p.sm_scale, !LONG_CAP);
 
     // b_run: what the logits are lowered by before they become weights, the running maximum less kShift.  It is this base that a round keeps or
     // moves, so that sums of rounds with one maximum stay as they are: the factor to them has to be exactly 1 there (from the maxima, with
@@ -701,10 +713,11 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           const Logit& logit = i ? logit1 : logit0;
           float k = logit.k;      // logits are s k
           if (logit.cap > 0.f) {
+            const float per_cap = LONG_CAP ? logit.per_cap() : 0.f;
 #pragma unroll
             for (int n = 0; n < KEYS / 8; ++n)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) s[n][2 * i + e] = logit.capped(s[n][2 * i + e]);
+              for (int e = 0; e < 2; ++e) s[n][2 * i + e] = LONG_CAP ? logit.capped(s[n][2 * i + e], per_cap) : logit.capped_short(s[n][2 * i + e]);
             k = 1.f;
           }
           if (tail) {
@@ -841,7 +854,8 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   Share sh{0, 0, 0, (int)(blockIdx.x / plan.cluster / units)};
   if (plan.split && !find_share(p, units, G::ROUND, plan, sh)) return;
   const int64_t share_first = sh.first;
-  const Logit logit(p, p.sm_scale);
+  const Logit logit(p, p.sm_scale, false);
+  const float per_cap = logit.per_cap();
 
   for (bool more = true; more;) {
     __syncthreads();
@@ -901,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
       for (int h = 0; h < GT; ++h) {
 #pragma unroll
         for (int o = LPK >> 1; o > 0; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-        s[h] = in ? (logit.cap > 0.f ? logit.capped(s[h]) : s[h] * logit.k) : -INFINITY;
+        s[h] = in ? (logit.cap > 0.f ? logit.capped(s[h], per_cap) : s[h] * logit.k) : -INFINITY;
         float mx = s[h];
 #pragma unroll
         for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -1046,14 +1060,14 @@ constexpr int kWholeRounds = 24;      // most rounds of a unit that is a CTA's
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 
-template <int DT, bool F8, int DP, int GT>
+template <int DT, bool F8, int DP, int GT, bool LONG_CAP>
 struct Kernel {
   using G = Geo<DT, F8, DP>;
   static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP + kWarps * 4 * G::KEYS * 8;
   static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 4) <= G::RING_BYTES, "the join of the warps lies over the rings");
   static void (*kern())(const Params, const Plan) {
     if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT>;
-    else return paged_decode_mma_kernel<DT, F8, DP, GT>;
+    else return paged_decode_mma_kernel<DT, F8, DP, GT, LONG_CAP>;
   }
   // How the call is laid out, and its CTAs.  Reads shapes and what the device holds.
   static Plan plan(const Params& p, int64_t* ctas) {
@@ -1110,17 +1124,23 @@ struct Kernel {
 };
 
 // `bytes`: only the scratch of the call
-template <int DT, bool F8, int DP>
+template <int DT, bool F8, int DP, bool LONG_CAP>
 int launch_heads(const Params& p, cudaStream_t stream, int64_t* bytes) {
   constexpr int SMALL = DT == HIPATTN_F32 ? 4 : 8;
-  return p.H / p.HKV <= SMALL ? Kernel<DT, F8, DP, SMALL>::launch(p, stream, bytes) : Kernel<DT, F8, DP, SMALL * 2>::launch(p, stream, bytes);
+  return p.H / p.HKV <= SMALL ? Kernel<DT, F8, DP, SMALL, LONG_CAP>::launch(p, stream, bytes) : Kernel<DT, F8, DP, SMALL * 2, LONG_CAP>::launch(p, stream, bytes);
+}
+template <int DT, bool F8, int DP>
+int launch_dim(const Params& p, cudaStream_t stream, int64_t* bytes) {
+  if constexpr (DT != HIPATTN_F32)      // (the kernel of 32-bit products knows one form)
+    if (p.logit_softcap > kShortCap) return launch_heads<DT, F8, DP, true>(p, stream, bytes);
+  return launch_heads<DT, F8, DP, false>(p, stream, bytes);
 }
 template <int DT, bool F8>
 int launch_type(const Params& p, cudaStream_t stream, int64_t* bytes) {
   switch (padded_dim(p.D)) {
-    case 64: return launch_heads<DT, F8, 64>(p, stream, bytes);
-    case 128: return launch_heads<DT, F8, 128>(p, stream, bytes);
-    default: return launch_heads<DT, F8, 256>(p, stream, bytes);
+    case 64: return launch_dim<DT, F8, 64>(p, stream, bytes);
+    case 128: return launch_dim<DT, F8, 128>(p, stream, bytes);
+    default: return launch_dim<DT, F8, 256>(p, stream, bytes);
   }
 }
 int launch(const Params& p, cudaStream_t stream, int64_t* bytes) {

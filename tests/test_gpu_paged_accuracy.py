@@ -75,3 +75,45 @@ def test_an_offset_of_all_logits_changes_nothing(dtype, fp8, D, G, B, n):
     tol = (want_lse.abs() + a.double().abs() / math.log(2)) * 2 * U + den / math.log(2) + 2.0 ** -18
     err = (lse.double() - want_lse).abs()
     assert bool((err <= tol).all()), f"lse off by {(err / tol).max().item():.3g} of the bound"
+
+
+@pytest.mark.parametrize("cap", [1e-40, 1e-3, 0.5, 30.0, 64.0, 65.0, 200.0, 1e3, 1e5, 1e20, 3e38])
+@pytest.mark.parametrize("dtype,fp8,G", [("fp32", False, 4), ("fp32", False, 8), ("bf16", False, 4), ("fp16", False, 12), ("bf16", True, 4), ("fp16", True, 12)])
+def test_soft_caps_of_any_size(dtype, fp8, G, cap):
+    """A capped logit is off by a few roundings of itself (16-bit products with caps up to 64: of the cap); a cap far above the logits changes nothing.
+
+    z = cap tanh(s scale / cap), s exact.  scale / cap and its product with s: 6 roundings; tanhf: 2 ulp; the product with log2 e cap: 3; 13 u < 2^-20 of z, also
+    where the cap is left out (y^2 / 3 < 2^-25).  Short form: 14 u < 2^-20 of the cap besides (exp2 2 ulp, the sum, the reciprocal 1 ulp, the last product)."""
+    from hip_attention_b200 import paged_decode_attention
+    D, page, lens = 64, 16, [1, 2, 37, 300, 1]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    W = max(-(-n // page) for n in lens)
+    n_pages = W * len(lens)
+    table = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32).view(len(lens), W)
+    ct = FP8 if fp8 else DT[dtype]
+    kc, vc = torch.zeros((n_pages, page, 1, D), device="cuda"), torch.randn((n_pages, page, 1, D), generator=g, device="cuda")
+    kc[..., 0] = torch.randint(-7, 8, kc.shape[:-1], generator=g, device="cuda") / 4.0
+    kc[..., 0][kc[..., 0] == 0] = 1.0
+    if fp8:
+        kc[..., 0] = kc[..., 0].to(FP8).float()
+    kc, vc = kc.to(ct), vc.to(ct)
+    q = torch.zeros((len(lens), G, D), dtype=DT[dtype], device="cuda")
+    q[:, :, 0] = 2.0 ** (torch.arange(G, device="cuda") % 4 * 3 - 5)          # logits from 2^-8 to 14
+    out, lse = paged_decode_attention(q, kc, vc, table, torch.tensor(lens, device="cuda"), sm_scale=0.5, logit_softcap=cap, return_lse=True)
+    cap = torch.tensor(cap, dtype=torch.float32).double().item()
+    short = dtype != "fp32" and cap <= 64
+    for b, n in enumerate(lens):
+        k, v = (c[table[b].long()].view(torch.uint8 if fp8 else ct).reshape(-1, D)[:n].view(ct).double() for c in (kc, vc))
+        for h in range(G):
+            z = cap * torch.tanh(k[:, 0] * q[b, h, 0].double() * 0.5 / cap)
+            ds = z.abs().max().item() * 2.0 ** -20 + (2.0 ** -20 * cap if short else 0.0)
+            p = torch.softmax(z, 0)
+            want, size, want_lse = p @ v, p @ v.abs(), (torch.logsumexp(z, 0) / math.log(2)).item()
+            weight = 2.0 ** -20 + 2 * z.abs().max().item() * U
+            two_terms = {"fp32": 0.0, "fp16": 2.0 ** -22, "bf16": 2.0 ** -22 if fp8 else 2.0 ** -16}[dtype]
+            tol = size * (2 * (ds + weight) + two_terms + 100 * U) + torch.finfo(q.dtype).eps / 2 * want.abs()
+            err = (out[b, h].double() - want).abs()
+            assert bool((err <= tol).all()), f"{n} {h}: off by {(err / tol).max().item():.3g} of the bound"
+            top = 9.0 if dtype == "fp32" else 23.0        # log2 of the denominator: off by one ulp
+            tol = (ds + weight + 50 * U) / math.log(2) + 2 * U * (abs(want_lse) + top)
+            assert abs(lse[b, h].item() - want_lse) <= tol, f"{n} {h}: lse off by {abs(lse[b, h].item() - want_lse) / tol:.3g} of the bound"
