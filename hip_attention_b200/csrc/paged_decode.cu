@@ -13,6 +13,7 @@
 // Measured: one sequence of 1048571 tokens, bf16, 8 KV heads of dimension 128 (4.3 GB) 620 us, 6.9 TB/s; 32 sequences of up to 16384
 // tokens (1.18 GB) 180 us, 6.5 TB/s; 12 fp8 sequences in pages of one token, soft-capped (0.56 GB) 111 us, 5.0 TB/s; one sequence of 389 tokens 5.0 us.
 #include <cfloat>
+#include <type_traits>
 
 #include "in_turn.cuh"
 #include "mma_common.cuh"
@@ -528,7 +529,8 @@ struct Feeder {
 // (largest: 16384), so that a weight of 2^-28 of the largest is still a normal number: many small weights add up.  Of eight heads the
 // second terms are the rows 8 to 15 of the tile, with sums of their own, and cost nothing; of sixteen they are a second product.
 // The second term may be zero or negative, which an infinite value turns into NaN: eight heads leave it out where the first sum is
-// not finite; of sixteen a warp that finds NaN in its output goes through its keys once more with the first term alone.
+// not finite; of sixteen a warp that finds NaN in its output goes through its keys once more and leaves the second term out of those sums
+// (the others come out as they were: a value that is not finite costs its neighbours nothing).
 // ---------------------------------------------------------------------------------------------------
 // the halves of two packed 16-bit elements
 template <int MT>
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
   float* s_merge = reinterpret_cast<float*>(smem);                       // over the rings when they are empty
   uint32_t* s_q = reinterpret_cast<uint32_t*>(smem + G::RING_BYTES);     // [KS][32][AR]: A fragments
   const unsigned char* entries = smem + G::RING_BYTES + 2 * GT * DP + warp * (4 * KEYS * 8);
+  __shared__ uint32_t s_nan[GT == 16 ? NT / 8 * kThreads : 1];           // [NT / 8][kThreads]: a bit for a sum that the first pass left NaN
   __shared__ float s_up[16];                                             // power of two that a head's queries were multiplied by
   const int units = p.HKV * plan.tiles;
   in_turn();
@@ -643,7 +646,9 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
     // moves, so that sums of rounds with one maximum stay as they are: the factor to them has to be exactly 1 there (from the maxima, with
     // the shift subtracted again, it is off by up to 2^-16 for logits near -256, in every round alike: 3e-3 of the output after 1024 rounds).
     float o[NT][4], b_run[GT / 8], l_run[GT / 8];
-    for (bool two = true;; two = false) {      // (a second time only for sixteen heads, and where there is NaN)
+    // all rounds.  TWO: with both terms of the weights, else with the second one only where s_nan has no bit
+    auto pass = [&](auto both) {
+      constexpr bool TWO = decltype(both)::value;
 #pragma unroll
       for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -655,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         // this lane's row and first piece in K and in V; piece j further is the address xor 16 j (a row begins on a multiple of its size)
         const uint32_t ks = feed.ring + slot * G::STAGE_BYTES + k_lane, vs = feed.ring + slot * G::STAGE_BYTES + v_lane;
         // ---- S = Q K^T ----
-        uint32_t kept[4];
+        [[maybe_unused]] uint32_t kept[4];
         float s[KEYS / 8][4], s2[2][4];      // (sixteen keys: odd steps have sums of their own, four chains of products in all)
 #pragma unroll
         for (int i = 0; i < KEYS / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -758,8 +763,15 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         // ---- O += P V ----
         auto product = [&](int n, int c, uint32_t b0, uint32_t b1) {
           mma16816<MT>(o[n], pa[c], b0, b1);
-          if constexpr (GT == 16) {
-            if (two) mma16816<MT>(o[n], pl[c], b0, b1);
+          if constexpr (GT == 16 && TWO) {
+            mma16816<MT>(o[n], pl[c], b0, b1);
+          } else if constexpr (GT == 16) {
+            const float one[4] = {o[n][0], o[n][1], o[n][2], o[n][3]};
+            mma16816<MT>(o[n], pl[c], b0, b1);
+            const uint32_t nan = *(volatile uint32_t*)&s_nan[n / 8 * kThreads + tid] >> (n % 8 * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (nan >> e & 1u) o[n][e] = one[e];
           }
         };
 #pragma unroll
@@ -788,23 +800,29 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
         slot = slot == 2 ? 0 : slot + 1;
       }
       cp_async_wait<0>();
-      if constexpr (GT == 8) {
-        // the terms together; where the first is infinite or NaN the second says nothing (zero times infinity)
+    };
+    pass(std::true_type());
+    if constexpr (GT == 8) {
+      // the terms together; where the first is infinite or NaN the second says nothing (zero times infinity)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (fabsf(o[n][e]) < INFINITY) o[n][e] += o[n][e + 2];
-        break;
-      } else {
-        bool nan = false;
+        for (int e = 0; e < 2; ++e)
+          if (fabsf(o[n][e]) < INFINITY) o[n][e] += o[n][e + 2];
+    } else {
+      uint32_t any = 0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int w = 0; w < NT / 8; ++w) {
+        uint32_t nan = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) nan |= o[n][e] != o[n][e];
-        if (!two || !__any_sync(0xffffffffu, nan)) break;
-        __syncwarp();
+        for (int i = 0; i < 32; ++i) nan |= o[w * 8 + i / 4][i % 4] != o[w * 8 + i / 4][i % 4] ? 1u << i : 0u;
+        s_nan[w * kThreads + tid] = nan;
+        any |= nan;
+      }
+      if (__any_sync(0xffffffffu, any != 0)) {
+        __syncwarp();      // (all of the warp are done with the last rows)
         feed.begin();
+        pass(std::false_type());
       }
     }
     __syncthreads();

@@ -117,3 +117,49 @@ def test_soft_caps_of_any_size(dtype, fp8, G, cap):
             top = 9.0 if dtype == "fp32" else 23.0        # log2 of the denominator: off by one ulp
             tol = (ds + weight + 50 * U) / math.log(2) + 2 * U * (abs(want_lse) + top)
             assert abs(lse[b, h].item() - want_lse) <= tol, f"{n} {h}: lse off by {abs(lse[b, h].item() - want_lse) / tol:.3g} of the bound"
+
+
+@pytest.mark.parametrize("width", [64, 4096])
+@pytest.mark.parametrize("dtype,fp8,D", [("bf16", False, 64), ("bf16", False, 128), ("bf16", False, 256), ("fp16", False, 128), ("fp16", True, 128), ("bf16", True, 64)])
+@pytest.mark.parametrize("G", [8, 9, 16, 24])
+def test_what_is_not_finite_costs_its_neighbours_nothing(dtype, fp8, D, G, width):
+    """One infinite and one NaN value, and a NaN in one head's query: other columns and heads keep both terms of their weights.
+
+    Two kinds of keys with logits 0 and -1.25 in such numbers that values of +1 and -1 nearly cancel: the output is small, its rounding too, and
+    a weight's rounding to one term (2^-9 of exp(-1.25) in bf16, 2^-11 in half precision, the same for all its keys) would show."""
+    from hip_attention_b200 import paged_decode_attention
+    n, page, HKV, w = 4000, 64, 1, math.exp(-1.25)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n_pages = -(-n // page)
+    t = torch.arange(n, device="cuda")
+    first = (t * 0.6180339887498949) % 1.0 < w / (1 + w)
+    k, v = torch.zeros((n, HKV, D), device="cuda"), torch.empty((n, HKV, D), device="cuda")
+    k[:, 0, 0] = torch.where(first, 0.0, -1.25)
+    v[:] = torch.where(first, 1.0, -1.0)[:, None, None]
+    v[:, 0, 1::2] *= -1
+    clean = v.double()
+    v[2501, 0, 3], v[77, 0, 5] = float("inf"), float("nan")
+    table = torch.full((1, width), n_pages + 3, dtype=torch.int32, device="cuda")
+    table[0, :n_pages] = torch.randperm(n_pages, generator=g, device="cuda")
+    ct = FP8 if fp8 else DT[dtype]
+    caches = []
+    for rows in (k, v):
+        c = torch.zeros((n_pages * page, HKV, D), device="cuda")
+        c[table[0, t // page].long() * page + t % page] = rows
+        caches.append(c.to(ct).view(n_pages, page, HKV, D))
+    q = torch.zeros((1, G, D), dtype=DT[dtype], device="cuda")
+    q[..., 0] = 1.0
+    q[0, G - 2, 2] = float("nan")
+    out, lse = paged_decode_attention(q, *caches, table, torch.tensor([n], device="cuda"), return_lse=True)
+    p = torch.softmax(k[:, 0, 0].double(), 0)
+    want, size = p @ clean[:, 0], p @ clean[:, 0].abs()
+    heads, cols = [h for h in range(G) if h != G - 2], [d for d in range(D) if d not in (3, 5)]
+    assert bool(torch.isnan(out[0, G - 2]).all()) and bool(torch.isnan(lse[0, G - 2]))
+    assert bool((out[0, heads, 3] == float("inf")).all()) and bool(torch.isnan(out[0, heads, 5]).all())
+    two_terms = 2.0 ** -16 if dtype == "bf16" and not fp8 else 2.0 ** -22
+    steps = 2 * 2 * 63                                          # (a sequence in one CTA: 63 rounds of up to 32 keys a warp, both terms)
+    tol = size * (2 * 2.0 ** -20 + two_terms + (200 + steps * 17 / 2) * U) + torch.finfo(q.dtype).eps / 2 * want.abs() + 2.0 ** -25
+    err = (out[0].double() - want).abs()[heads][:, cols]
+    assert bool((err <= tol[cols]).all()), f"off by {(err / tol[cols]).max().item():.3g} of the bound"
+    want_lse = torch.logsumexp(k[:, 0, 0].double(), 0).item() / math.log(2)
+    assert bool(((lse[0, heads].double() - want_lse).abs() <= 2.0 ** -18).all())
