@@ -179,12 +179,13 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
       } else {
         const int old = pool.lens[x];
         const long long now = FORK ? old : (long long)old + y;
-        if (old < 0 || now > 0x7fff0000LL || (now + P - 1) / P > pool.width || (FORK && pool.lens[row] != 0)) {
+        const long long pages = (now + P - 1) / P;       // (the longest length and a page of more than 65537 tokens pass 2^31)
+        if (old < 0 || now > 0x7fff0000LL || pages > pool.width || (FORK && pool.lens[row] != 0)) {
           bad = true;
         } else {
           len = (int)now;
-          had = FORK ? len / P : (old + P - 1) / P;
-          need = (len + P - 1) / P - had;
+          had = FORK ? len / P : (int)(((long long)old + P - 1) / P);
+          need = (int)pages - had;
           at = row;
           if (FORK) atomicMax(&s_longest, had);
         }
