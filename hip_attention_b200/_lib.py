@@ -13,7 +13,7 @@ STATUS_PAGE_RANGE, STATUS_TOKEN_RANGE, STATUS_TIMEOUT, STATUS_CHUNK_SIZE = 1, 2,
 STATUS_NO_PAGES, STATUS_SEQUENCE = 16, 32
 MAX_CHUNKS = 16384
 NOALLOC_SCRATCH_BYTES = 16 * 1024 * 1024
-ABI_VERSION = 11
+ABI_VERSION = 12
 SCAN_AUTO, SCAN_STRICT, SCAN_CHECK = 0, 1, 2
 ROPE_NONE, ROPE_RELATIVE, ROPE_STREAMING = 0, 1, 2
 
@@ -73,7 +73,7 @@ class WriteKvParams(C.Structure):
 class PagePool(C.Structure):
     _fields_ = [("ref_counts", vp), ("seq_lens", vp), ("block_table", vp), ("caches", C.POINTER(vp)), ("page_stride", i64), ("page_bytes", i64),
                 ("status", vp), ("scratch", vp), ("n_pages", i32), ("page_size", i32), ("n_sequences", i32), ("table_width", i32),
-                ("n_caches", i32), ("reserved_", i32)]
+                ("n_caches", i32), ("reserved_", i32), ("grown", vp)]
 
 
 # name -> (restype, argtypes); every symbol include/hipattn.h declares

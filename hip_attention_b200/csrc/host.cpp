@@ -1542,7 +1542,7 @@ at::Tensor entries(PyObject* o, const PoolHandle* h, const char* what) {
   if (t.size(0) > HIPATTN_POOL_MAX_ENTRIES) VALUE_ERROR("%s names %lld sequences, a call takes %d", what, (long long)t.size(0), HIPATTN_POOL_MAX_ENTRIES);
   return t.scalar_type() == at::kInt ? t : t.clamp(-1, 0x7fffffff).to(at::kInt);   // (what does not fit is beyond any table)
 }
-// pool_extend(handle, rows, n_tokens: tensor or int)
+// pool_extend(handle, rows, n_tokens: tensor or int, grown) -> grown
 PyObject* pool_extend(PyObject* const* argv) {
   PoolHandle* h = pool_of(argv[0]);
   const c10::cuda::CUDAGuard guard(h->dev);
@@ -1556,10 +1556,15 @@ PyObject* pool_extend(PyObject* const* argv) {
     every = as_int(Ref::borrow(argv[2]));
     if (every < 0 || every > 0x7fffffff) VALUE_ERROR("n_tokens %lld must not be negative, nor beyond 2^31", (long long)every);
   }
-  if (rows.size(0) == 0) Py_RETURN_NONE;
-  check(hipattn_pool_extend(&h->pool, rows.data_ptr<int32_t>(), tokens.defined() ? tokens.data_ptr<int32_t>() : nullptr, (int32_t)every, (int32_t)rows.size(0),
+  const at::Tensor grown = tensor_of(argv[3], "grown");
+  if (grown.defined() && (grown.scalar_type() != at::kInt || grown.dim() != 1 || !grown.is_contiguous() || grown.device() != h->dev || grown.size(0) != rows.size(0)))
+    VALUE_ERROR("grown must be a contiguous int32 tensor of %lld entries on the pool's device", (long long)rows.size(0));
+  if (rows.size(0) == 0) return Py_NewRef(argv[3]);
+  hipattn_page_pool_t pool = h->pool;
+  pool.grown = grown.defined() ? grown.data_ptr<int32_t>() : nullptr;
+  check(hipattn_pool_extend(&pool, rows.data_ptr<int32_t>(), tokens.defined() ? tokens.data_ptr<int32_t>() : nullptr, (int32_t)every, (int32_t)rows.size(0),
                             c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "extend");
-  Py_RETURN_NONE;
+  return Py_NewRef(argv[3]);
 }
 // pool_fork(handle, parents, children)
 PyObject* pool_fork(PyObject* const* argv) {
@@ -1767,7 +1772,7 @@ PyMethodDef methods[] = {
     {"paged_decode", (PyCFunction)(void*)py_call<paged_decode, 11>, METH_FASTCALL, "q, k_cache, v_cache, block_table, cache_seq_lens, rows, sm_scale, sliding_window, logit_softcap, return_lse, out"},
     {"write_kv", (PyCFunction)(void*)py_call<write_kv, 8>, METH_FASTCALL, "k, v, k_cache, v_cache, block_table, cache_seq_lens, rows, token_offsets"},
     {"page_pool", (PyCFunction)(void*)py_call<page_pool, 4>, METH_FASTCALL, "[caches], ref_counts, seq_lens, block_table -> handle"},
-    {"pool_extend", (PyCFunction)(void*)py_call<pool_extend, 3>, METH_FASTCALL, "handle, rows, n_tokens"},
+    {"pool_extend", (PyCFunction)(void*)py_call<pool_extend, 4>, METH_FASTCALL, "handle, rows, n_tokens, grown -> grown"},
     {"pool_fork", (PyCFunction)(void*)py_call<pool_fork, 3>, METH_FASTCALL, "handle, parents, children"},
     {"pool_free", (PyCFunction)(void*)py_call<pool_free, 2>, METH_FASTCALL, "handle, rows"},
     {"pool_compact", (PyCFunction)(void*)py_call<pool_compact, 1>, METH_FASTCALL, "handle -> pages in use"},

@@ -21,6 +21,7 @@ struct Pool {
   int32_t* lens;
   int32_t* table;
   uint32_t* status;
+  int32_t* grown;      // extend, or null: its rows, -1 where nothing grew
   int n_pages, page_size, n_seqs, width;
 };
 struct CacheList {
@@ -215,6 +216,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
       atomicOr(pool.status, bad ? HIPATTN_STATUS_SEQUENCE : HIPATTN_STATUS_NO_PAGES);
       if (FORK) plan[0] = 0;
     }
+    if (!FORK && rank == 0 && pool.grown)
+      for (int i = tid; i < n; i += kPlanThreads) pool.grown[i] = -1;
     return;
   }
 
@@ -282,8 +285,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
     }
   }
   if (rank == 0) {
-    for (int i = tid; i < n; i += kPlanThreads)
+    for (int i = tid; i < n; i += kPlanThreads) {
       if (s_row[i] >= 0) pool.lens[s_row[i]] = s_new[i];
+      if (!FORK && pool.grown) pool.grown[i] = s_row[i];
+    }
     if (FORK && tid == 0) plan[0] = (int)total;
   }
 }
@@ -611,7 +616,7 @@ int validate_pool(const hipattn_page_pool_t* p, const char* what, bool caches) {
   return HIPATTN_OK;
 }
 Pool device_pool(const hipattn_page_pool_t& p) {
-  return Pool{p.ref_counts, p.seq_lens, p.block_table, p.status, p.n_pages, p.page_size, p.n_sequences, p.table_width};
+  return Pool{p.ref_counts, p.seq_lens, p.block_table, p.status, p.grown, p.n_pages, p.page_size, p.n_sequences, p.table_width};
 }
 
 int plan_ctas(const hipattn_page_pool_t& p) { return p.n_pages <= kSmallPool ? 1 : kPlanCtas; }

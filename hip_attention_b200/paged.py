@@ -49,7 +49,8 @@ def write_paged_kv(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, block
 
     ``k`` / ``v`` [N, HKV, D]: the last tokens of the sequences, whose lengths ``cache_seq_lens`` count them already
     (``HiPPagePool.extend``).  Sequence b (row rows[b] of the table; None: b; negative: its tokens are left out) has tokens
-    token_offsets[b] : token_offsets[b + 1], or N / B of them each; tokens outside the offsets are not written.  A
+    token_offsets[b] : token_offsets[b + 1], or N / B of them each; tokens outside the offsets are not written.  Give the rows that grew
+    (``HiPPagePool.extend``): a growth that was refused has no place for its tokens, and they would go over the last ones.  A
     float8_e5m2 pool (or its uint8 view) receives the nearest values (ties to even, beyond the range infinity).  The rows of a
     call must differ: of two that are the same, which values stay is not defined."""
     host().write_kv(k, v, k_cache, v_cache, block_table, cache_seq_lens, rows, token_offsets)
@@ -91,10 +92,14 @@ class HiPPagePool:
         self.block_table = self.state[n_pages + max_sequences:].view(max_sequences, max_pages_per_sequence)
         self._handle = host().page_pool(k_caches + v_caches, self.ref_counts, self.seq_lens, self.block_table)
 
-    def extend(self, rows: Tensor, n_tokens: Union[Tensor, int]) -> None:
-        """Sequence rows[i] grows by n_tokens[i] tokens (an int: by as many each) and gets the pages for them.  Write the
-        tokens with ``write_paged_kv``."""
-        host().pool_extend(self._handle, rows, n_tokens)
+    def extend(self, rows: Tensor, n_tokens: Union[Tensor, int], grown: Optional[Tensor] = None) -> Optional[Tensor]:
+        """Sequence rows[i] grows by n_tokens[i] tokens (an int: by as many each) and gets the pages for them.
+
+        ``grown`` (int32, as long as ``rows``) receives the rows that grew, ``rows`` or, when the call could not be carried out, -1
+        everywhere, and is returned.  It is what the ``write_paged_kv`` and ``paged_decode_attention`` that follow take as their ``rows``:
+        they leave -1 out.  With the rows that were asked for, the tokens of a refused growth would be written over the last ones
+        of their sequences, in a page that others may share."""
+        return host().pool_extend(self._handle, rows, n_tokens, grown)
 
     def fork(self, parents: Tensor, children: Tensor) -> None:
         """Sequence children[i], which is empty, becomes a copy of parents[i] (a parent may have several children).  Full

@@ -382,9 +382,12 @@ typedef struct hipattn_page_pool {
   void* scratch;             /* hipattn_pool_scratch bytes (fork: of n entries; compact: n = 0) */
   int32_t n_pages, page_size, n_sequences, table_width, n_caches;
   int32_t reserved_;
+  int32_t* grown;            /* optional, [n] of a hipattn_pool_extend call: receives rows[i], or -1 where nothing grew */
 } hipattn_page_pool_t;
 int64_t hipattn_pool_scratch(const hipattn_page_pool_t* pool, int32_t n);
-/* rows[i] grows by n_tokens[i] (>= 0; n_tokens null: by `every`) tokens and gets the pages they need. */
+/* rows[i] grows by n_tokens[i] (>= 0; n_tokens null: by `every`) tokens and gets the pages they need.  `grown` receives the rows of a call that
+ * was carried out, and -1 for entries that are left out and for all entries of one that was not: give it to hipattn_write_kv as
+ * `rows`, or tokens that have no place go over the last ones of their sequences. */
 int hipattn_pool_extend(const hipattn_page_pool_t* pool, const int32_t* rows, const int32_t* n_tokens, int32_t every, int32_t n, void* stream);
 /* children[i], an empty sequence, becomes a copy of parents[i]: full pages are shared, the tokens of a begun page are copied to a
  * page of the child's own in all caches. */

@@ -39,3 +39,85 @@ def test_the_longest_sequence_in_pages_of_many_tokens(P):
     a = ints([1])
     L.check(lib.hipattn_pool_free(C.byref(p), a.data_ptr(), 1, st), "free")
     assert read_status("cuda") == 0 and lens.tolist() == [5, 0, 0] and refs[need].item() == 1 and int(refs.sum()) == 1
+
+
+def _bits(pool):
+    return [c.view(torch.int16).clone() for c in pool.k_caches + pool.v_caches] + [pool.state.clone()]
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("n_tokens", ["int", "tensor"])
+def test_a_step_of_a_pool_that_runs_out_writes_nothing(captured, n_tokens):
+    """A growth that is refused names no rows, so the writes behind it leave the last tokens as they were, one of them in a page that
+    two sequences share; a graph of the step goes on when there are pages again."""
+    from hip_attention_b200 import HiPPagePool, paged_decode_attention, read_status, write_paged_kv
+    P, HKV, D, layers = 4, 2, 64, 2
+    g = torch.Generator(device="cuda").manual_seed(0)
+    caches = [torch.randn((5, P, HKV, D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2 * layers)]
+    pool = HiPPagePool(caches[:layers], caches[layers:], 4, 6)
+    k, v, q = (torch.randn((4, n, D), generator=g, device="cuda").to(torch.bfloat16) for n in (HKV, HKV, 4))
+    rows, one = ints([0, 1, -1, 2]), ints([1, 1, 1, 1])
+    out = torch.full((layers, 4, 4, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    pool.extend(ints([0, 1]), ints([2 * P, P - 1]))        # pages 0 to 2
+    pool.fork(ints([0]), ints([2]))                        # two full pages shared; two pages are free, a step needs two, then none
+    read_status("cuda")
+
+    def step():
+        pool.extend(rows, one if n_tokens == "tensor" else 1, grown)
+        for l in range(layers):
+            write_paged_kv(k, v, pool.k_caches[l], pool.v_caches[l], pool.block_table, pool.seq_lens, rows=grown)
+            paged_decode_attention(q, pool.k_caches[l], pool.v_caches[l], pool.block_table, pool.seq_lens, rows=grown, out=out[l])
+        return grown
+    grown = torch.zeros_like(rows)
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        run = lambda: (graph.replay(), grown)[1]   # noqa: E731
+    else:
+        run = step
+    pool.extend(ints([3]), 2 * P)                          # the last two pages
+    assert read_status("cuda") == 0
+    before = _bits(pool)
+    assert run().tolist() == [-1, -1, -1, -1] and read_status("cuda") == 16
+    assert all(torch.equal(a, b) for a, b in zip(before, _bits(pool))) and not out.any()
+    pool.free(ints([3]))
+    assert run().tolist() == [0, 1, -1, 2] and read_status("cuda") == 0
+    lens = pool.seq_lens.tolist()
+    assert lens == [2 * P + 1, P, 2 * P + 1, 0]
+    for l in range(layers):
+        for i, r in ((0, 0), (1, 1), (3, 2)):
+            page, at = pool.block_table[r, (lens[r] - 1) // P], (lens[r] - 1) % P
+            assert torch.equal(pool.k_caches[l][page, at], k[i]) and torch.equal(pool.v_caches[l][page, at], v[i])
+        assert torch.equal(pool.k_caches[l][:2].view(torch.int16), before[l][:2])       # the shared pages
+    assert out[:, [0, 1, 3]].any(-1).all() and not out[:, 2].any()
+
+
+def test_rows_that_grew():
+    """-1 for entries that are left out and for every entry of a call that is refused, whatever the reason; `rows` itself may receive them."""
+    from hip_attention_b200 import HiPPagePool, read_status
+    c = [torch.zeros((9000, 2, 1, 8), dtype=torch.float16, device="cuda") for _ in range(2)]
+    for n_pages in (12, 9000):            # planned by one CTA, and by a cluster
+        pool = HiPPagePool([c[0][:n_pages]], [c[1][:n_pages]], 5, 9)
+        read_status("cuda")
+
+        def grow(rows, tokens):
+            grown = torch.full((len(rows),), 99, dtype=torch.int32, device="cuda")
+            assert pool.extend(ints(rows), tokens, grown) is grown
+            return grown.tolist()
+        grown = torch.empty(4, dtype=torch.int32, device="cuda")
+        pool.extend(torch.tensor([3, -1, 0, -7], device="cuda"), ints([3, 5, 0, 1]), grown)
+        assert grown.tolist() == [3, -1, 0, -1] and read_status("cuda") == 0
+        for rows, tokens in (([0, 0], [1, 1]), ([0, 5], [1, 1]), ([0, 1], [1, -1]), ([0, 1], [1, 19])):
+            assert grow(rows, ints(tokens)) == [-1, -1] and read_status("cuda") == 32
+        if n_pages == 12:
+            assert grow([0, 1, 2], 8) == [-1, -1, -1] and read_status("cuda") == 16
+        assert grow([], 1) == [] and pool.extend(ints([0]), 0) is None
+        rows = ints([4, -2])
+        pool.extend(rows, 1, rows)
+        assert rows.tolist() == [4, -1] and pool.seq_lens.tolist() == [0, 0, 0, 3, 1]
+        for bad in (torch.empty(3, dtype=torch.int32, device="cuda"), torch.empty(2, dtype=torch.int64, device="cuda"), torch.empty(2, dtype=torch.int32),
+                    torch.empty(4, dtype=torch.int32, device="cuda")[::2]):
+            with pytest.raises(ValueError, match="grown"):
+                pool.extend(ints([0, 1]), 1, bad)
+        assert pool.seq_lens.tolist() == [0, 0, 0, 3, 1] and read_status("cuda") == 0
