@@ -1473,6 +1473,19 @@ struct PoolHandle {
   std::vector<void*> caches;
   hipattn_page_pool_t pool{};
   c10::Device dev{at::kCUDA, 0};
+  std::vector<at::Tensor> own;            // what the pool allocated: its state and the plans
+  std::vector<cudaStream_t> streams;      // that own's memory is known to be used on, the one it was allocated on first
+
+  // The stream of a call.  A pool may be dropped while its calls are still running on another stream than the one that it was made on: the
+  // allocator has to know of it before it gives the memory away.
+  cudaStream_t stream() {
+    const c10::cuda::CUDAStream s = c10::cuda::getCurrentCUDAStream(dev.index());
+    for (cudaStream_t known : streams)
+      if (known == s.stream()) return known;
+    for (const at::Tensor& t : own) t.record_stream(s.unwrap());
+    streams.push_back(s.stream());
+    return s.stream();
+  }
 };
 const char* kPoolName = "hip_attention_b200.page_pool";
 void drop_pool(PyObject* o) { delete (PoolHandle*)PyCapsule_GetPointer(o, kPoolName); }
@@ -1521,15 +1534,16 @@ PyObject* page_pool(PyObject* const* argv) {
   if (p.page_stride % 16) VALUE_ERROR("pages must start on 16-byte boundaries");
   for (void* c : h->caches)
     if ((uintptr_t)c % 16) VALUE_ERROR("caches must start on 16-byte boundaries");
-  h->keep.push_back(refs);
-  h->keep.push_back(lens);
-  h->keep.push_back(table);
+  h->own.push_back(refs);
+  h->own.push_back(lens);
+  h->own.push_back(table);
   p.status = (uint32_t*)status_word(h->dev.index()).data_ptr();
   // the plans of forks and compactions: calls on one pool are ordered, so one buffer serves all of them
   const c10::cuda::CUDAGuard guard(h->dev);
   const at::Tensor scratch = Device{h->dev}.empty({std::max(hipattn_pool_scratch(&p, HIPATTN_POOL_MAX_ENTRIES), hipattn_pool_scratch(&p, 0))}, at::kByte);
   p.scratch = scratch.data_ptr();
-  h->keep.push_back(scratch);
+  h->own.push_back(scratch);
+  h->streams.push_back(c10::cuda::getCurrentCUDAStream(h->dev.index()).stream());
   PyObject* o = PyCapsule_New(h.get(), kPoolName, drop_pool);
   if (o) h.release();
   return o;
@@ -1562,8 +1576,8 @@ PyObject* pool_extend(PyObject* const* argv) {
   if (rows.size(0) == 0) return Py_NewRef(argv[3]);
   hipattn_page_pool_t pool = h->pool;
   pool.grown = grown.defined() ? grown.data_ptr<int32_t>() : nullptr;
-  check(hipattn_pool_extend(&pool, rows.data_ptr<int32_t>(), tokens.defined() ? tokens.data_ptr<int32_t>() : nullptr, (int32_t)every, (int32_t)rows.size(0),
-                            c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "extend");
+  check(hipattn_pool_extend(&pool, rows.data_ptr<int32_t>(), tokens.defined() ? tokens.data_ptr<int32_t>() : nullptr, (int32_t)every, (int32_t)rows.size(0), h->stream()),
+        "extend");
   return Py_NewRef(argv[3]);
 }
 // pool_fork(handle, parents, children)
@@ -1574,7 +1588,7 @@ PyObject* pool_fork(PyObject* const* argv) {
   if (parents.size(0) != children.size(0)) VALUE_ERROR("%lld parents, but %lld children", (long long)parents.size(0), (long long)children.size(0));
   const int n = (int)parents.size(0);
   if (n == 0) Py_RETURN_NONE;
-  check(hipattn_pool_fork(&h->pool, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), n, c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "fork");
+  check(hipattn_pool_fork(&h->pool, parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), n, h->stream()), "fork");
   Py_RETURN_NONE;
 }
 // pool_free(handle, rows)
@@ -1583,7 +1597,7 @@ PyObject* pool_free(PyObject* const* argv) {
   const c10::cuda::CUDAGuard guard(h->dev);
   const at::Tensor rows = entries(argv[1], h, "rows");
   if (rows.size(0) == 0) Py_RETURN_NONE;
-  check(hipattn_pool_free(&h->pool, rows.data_ptr<int32_t>(), (int)rows.size(0), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "free");
+  check(hipattn_pool_free(&h->pool, rows.data_ptr<int32_t>(), (int)rows.size(0), h->stream()), "free");
   Py_RETURN_NONE;
 }
 // pool_compact(handle) -> pages in use, int32 [1]
@@ -1591,7 +1605,7 @@ PyObject* pool_compact(PyObject* const* argv) {
   PoolHandle* h = pool_of(argv[0]);
   const c10::cuda::CUDAGuard guard(h->dev);
   const at::Tensor in_use = Device{h->dev}.empty({1}, at::kInt);
-  check(hipattn_pool_compact(&h->pool, in_use.data_ptr<int32_t>(), c10::cuda::getCurrentCUDAStream(h->dev.index()).stream()), "compact");
+  check(hipattn_pool_compact(&h->pool, in_use.data_ptr<int32_t>(), h->stream()), "compact");
   return wrap(in_use);
 }
 

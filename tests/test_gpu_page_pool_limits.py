@@ -121,3 +121,32 @@ def test_rows_that_grew():
             with pytest.raises(ValueError, match="grown"):
                 pool.extend(ints([0, 1]), 1, bad)
         assert pool.seq_lens.tolist() == [0, 0, 0, 3, 1] and read_status("cuda") == 0
+
+
+def test_a_pool_dropped_while_its_calls_run_on_another_stream():
+    """What the pool allocated is not given to others before the stream that uses it has passed, and the calls end as they should."""
+    from hip_attention_b200 import HiPPagePool, read_status
+    n_pages, P, R, W = 300, 4, 40, 50
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn((n_pages, P, 1, 16), generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    pool = HiPPagePool([k], [v], R, W)
+    pool.extend(ints([1, 0]), ints([8 * P, 6 * P + 3]))       # pages 0 to 7, 8 to 14
+    pool.free(ints([1]))
+    parents, children = ints([0]), ints([2])
+    k0, v0 = k.clone(), v.clone()
+    read_status("cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    sizes = [pool.state.numel() * 4, 4096 * 12 + 16]
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(400_000_000)
+        pool.fork(parents, children)          # page 14's three tokens to page 0
+        pool.compact()                        # eight pages: 0, 8 .. 14; 8 .. 14 to 1 .. 7
+    del pool
+    others = [torch.zeros(n, dtype=torch.uint8, device="cuda") for n in sizes * 30]
+    assert not side.query()                   # (the calls have not begun)
+    torch.cuda.synchronize()
+    assert not any(bool(x.any()) for x in others) and read_status("cuda") == 0
+    for c, c0 in ((k, k0), (v, v0)):
+        assert torch.equal(c[1:8], c0[8:15]) and torch.equal(c[0, :3], c0[14, :3]) and torch.equal(c[0, 3], c0[0, 3]) and torch.equal(c[8:], c0[8:])
