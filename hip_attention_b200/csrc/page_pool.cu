@@ -24,6 +24,8 @@ struct Pool {
   int32_t* grown;      // extend, or null: its rows, -1 where nothing grew
   int n_pages, page_size, n_seqs, width;
 };
+// (not n + P - 1 over P: the longest length and a page of more than 65537 tokens pass 2^31)
+__device__ __forceinline__ int pages_of(int n, int P) { return n / P + (n % P != 0); }
 struct CacheList {
   char* at[kMaxCachesPerLaunch];
   int n;
@@ -180,13 +182,12 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
       } else {
         const int old = pool.lens[x];
         const long long now = FORK ? old : (long long)old + y;
-        const long long pages = (now + P - 1) / P;       // (the longest length and a page of more than 65537 tokens pass 2^31)
-        if (old < 0 || now > 0x7fff0000LL || pages > pool.width || (FORK && pool.lens[row] != 0)) {
+        if (old < 0 || now > 0x7fff0000LL || (FORK && pool.lens[row] != 0) || pages_of((int)now, P) > pool.width) {
           bad = true;
         } else {
           len = (int)now;
-          had = FORK ? len / P : (int)(((long long)old + P - 1) / P);
-          need = (int)pages - had;
+          had = FORK ? len / P : pages_of(old, P);
+          need = pages_of(len, P) - had;
           at = row;
           if (FORK) atomicMax(&s_longest, had);
         }
