@@ -737,7 +737,16 @@ __global__ void __launch_bounds__(kThreads, Geo<DT, F8, DP>::CTAS) paged_decode_
           for (int n = 1; n < KEYS / 8; ++n) mx = fmaxf(mx, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float b_new = fmaxf(b_run[i], fmaf(mx, k, -kShift)), base = b_new > -INFINITY ? b_new : 0.f;
+          float b_new = fmaxf(b_run[i], fmaf(mx, k, -kShift));
+          if (fabsf(b_new) >= 0x1p24f) {      // neighbours are two and more apart there: a logit that is not rounded itself may lie far above the largest one
+#pragma unroll
+            for (int n = 0; n < KEYS / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) s[n][2 * i + e] = __fmul_rn(s[n][2 * i + e], k);
+            b_new = fmaxf(b_run[i], __fmul_rn(mx, k));
+            k = 1.f;
+          }
+          const float base = b_new > -INFINITY ? b_new : 0.f;
           alpha[i] = ex2(b_run[i] - base);
           float sum = 0.f;
 #pragma unroll

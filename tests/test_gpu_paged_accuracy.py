@@ -163,3 +163,40 @@ def test_what_is_not_finite_costs_its_neighbours_nothing(dtype, fp8, D, G, width
     assert bool((err <= tol[cols]).all()), f"off by {(err / tol[cols]).max().item():.3g} of the bound"
     want_lse = torch.logsumexp(k[:, 0, 0].double(), 0).item() / math.log(2)
     assert bool(((lse[0, heads].double() - want_lse).abs() <= 2.0 ** -18).all())
+
+
+@pytest.mark.parametrize("width", [64, 4096])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("dtype,fp8,size", [("fp16", False, 13), ("fp16", False, 15), ("fp16", True, 13), ("bf16", True, 13), ("bf16", False, 16), ("bf16", False, 60), ("fp32", False, 60)])
+@pytest.mark.parametrize("G", [4, 12])
+def test_logits_whose_neighbours_are_far_apart(dtype, fp8, size, sign, G, width):
+    """Logits of 2^26 and beyond: the largest take all of the weight, in equal parts.  (1.25 2^size times 2^size, next to it 1 2^size times that: no
+    other key is less than 2^24 below.)"""
+    from hip_attention_b200 import paged_decode_attention
+    n, page, D = 3000, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(size)
+    n_pages = -(-n // page)
+    t = torch.arange(n, device="cuda")
+    top = torch.rand(n, generator=g, device="cuda") < 0.02
+    k = torch.zeros((n, 1, D), device="cuda")
+    k[:, 0, 0] = torch.where(top, 1.25 if sign > 0 else 1.0, 1.0 if sign > 0 else 1.25) * 2.0 ** size * sign
+    v = torch.randn((n, 1, D), generator=g, device="cuda")
+    table = torch.full((1, width), 0, dtype=torch.int32, device="cuda")
+    table[0, :n_pages] = torch.randperm(n_pages, generator=g, device="cuda")
+    ct = FP8 if fp8 else DT[dtype]
+    caches = []
+    for rows in (k, v):
+        c = torch.zeros((n_pages * page, 1, D), device="cuda")
+        c[table[0, t // page].long() * page + t % page] = rows
+        caches.append(c.to(ct).view(n_pages, page, 1, D))
+    q = torch.zeros((1, G, D), dtype=DT[dtype], device="cuda")
+    q[..., 0] = 2.0 ** size * (1 + torch.arange(G, device="cuda") / 16)
+    out, lse = paged_decode_attention(q, *caches, table, torch.tensor([n], device="cuda"), return_lse=True)
+    vt = v.to(ct).double()[top, 0]
+    want, size_ = vt.mean(0), vt.abs().mean(0)
+    # weights of the largest are equal; numerators and denominators: 24 rounds, up to 300 parts (2 u each), two terms of 16 bits or one of eight bits more
+    tol = size_ * ((24 * 2 * 17 + 600) * U + (2.0 ** -16 if dtype == "bf16" and not fp8 else 0.0) + 2.0 ** -20) + torch.finfo(q.dtype).eps / 2 * want.abs()
+    err = (out[0].double() - want).abs()
+    assert bool((err <= tol).all()), f"off by {(err / tol).max().item():.3g} of the bound"
+    want_lse = q[0, :, 0].double() * k.to(ct).double()[top, 0, 0][0] / math.log(2) + math.log2(vt.shape[0])
+    assert bool(((lse[0].double() - want_lse).abs() <= want_lse.abs() * 2.0 ** -21).all())
