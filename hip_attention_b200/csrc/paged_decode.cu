@@ -110,7 +110,8 @@ __device__ __forceinline__ float ex2(float x) {
 // is below 2^-16, what the two 16-bit terms of a weight keep.
 // Else (fp32 products, larger caps): tanhf, off by a few 2^-24 of the logit itself, and the plain logit where the cap changes less than 2^-25 of it, so
 // that a cap far above the logits changes nothing.  Kernels of their own: 12 fp8 sequences with a cap of 30 115 us in the short form, 124 in this one, and
-// with both in one kernel others lose 4 % to it that have no cap at all.  fp32, 16 sequences of up to 16384: 247 us in the short form, 260 in this one.
+// with both in one kernel others lose 4 % to it that have no cap at all.  fp32, 16 sequences of up to 16384 tokens: 222 us
+// without a cap, 224 with one; 243 and 246 with both in one kernel in the short form.
 constexpr float kShortCap = 64.f;
 struct Logit {
   float k, cap;      // cap 0: none, else log2 e cap.  k = log2 e scale, short form 2 log2 e scale / cap.  k is positive: queries are multiplied by `sign` before
@@ -864,7 +865,7 @@ struct FmaPlace : Place<RB, FmaPlace<RB, LPK>> {   // the lanes of a quarter war
   __device__ static __forceinline__ constexpr int turn(int key) { return (key * LPK) & 7; }
 };
 
-template <int DP, int GT>
+template <int DP, int GT, bool CAP>
 __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_kernel(const Params p, const Plan plan) {
   using G = FmaGeo<DP>;
   using P = FmaPlace<G::RB, G::LPK>;
@@ -882,7 +883,7 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
   if (plan.split && !find_share(p, units, G::ROUND, plan, sh)) return;
   const int64_t share_first = sh.first;
   const Logit logit(p, p.sm_scale, false);
-  const float per_cap = logit.per_cap();
+  const float per_cap = CAP ? logit.per_cap() : 0.f;
 
   for (bool more = true; more;) {
     __syncthreads();
@@ -939,10 +940,23 @@ __global__ void __launch_bounds__(kThreads, FmaGeo<DP>::CTAS) paged_decode_fma_k
       const bool in = feed.key_at(r) + key < g.seq.hi;
       float pr[GT];
 #pragma unroll
-      for (int h = 0; h < GT; ++h) {
+      for (int h = 0; h < GT; ++h)
 #pragma unroll
         for (int o = LPK >> 1; o > 0; o >>= 1) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-        s[h] = in ? (logit.cap > 0.f ? logit.capped(s[h], per_cap) : s[h] * logit.k) : -INFINITY;
+      if constexpr (CAP) {       // a key's lanes take a head each (every lane all heads: a tenth of the kernel's time)
+#pragma unroll
+        for (int h0 = 0; h0 < GT; h0 += LPK) {
+          float mine = s[h0];
+#pragma unroll
+          for (int j = 1; j < LPK && h0 + j < GT; ++j) mine = sub == j ? s[h0 + j] : mine;
+          mine = logit.capped(mine, per_cap);
+#pragma unroll
+          for (int j = 0; j < LPK && h0 + j < GT; ++j) s[h0 + j] = __shfl_sync(0xffffffffu, mine, (lane & ~(LPK - 1)) + j);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < GT; ++h) {
+        s[h] = in ? (CAP ? s[h] : s[h] * logit.k) : -INFINITY;
         float mx = s[h];
 #pragma unroll
         for (int o = 16; o >= LPK; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -1093,7 +1107,7 @@ struct Kernel {
   static constexpr size_t smem = G::RING_BYTES + (DT == HIPATTN_F32 ? sizeof(float) : sizeof(uint16_t)) * GT * DP + kWarps * 4 * G::KEYS * 8;
   static_assert(sizeof(float) * (kWarps + 1) * GT * (DP + 4) <= G::RING_BYTES, "the join of the warps lies over the rings");
   static void (*kern())(const Params, const Plan) {
-    if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT>;
+    if constexpr (DT == HIPATTN_F32) return paged_decode_fma_kernel<DP, GT, LONG_CAP>;
     else return paged_decode_mma_kernel<DT, F8, DP, GT, LONG_CAP>;
   }
   // How the call is laid out, and its CTAs.  Reads shapes and what the device holds.
@@ -1158,8 +1172,7 @@ int launch_heads(const Params& p, cudaStream_t stream, int64_t* bytes) {
 }
 template <int DT, bool F8, int DP>
 int launch_dim(const Params& p, cudaStream_t stream, int64_t* bytes) {
-  if constexpr (DT != HIPATTN_F32)      // (the kernel of 32-bit products knows one form)
-    if (p.logit_softcap > kShortCap) return launch_heads<DT, F8, DP, true>(p, stream, bytes);
+  if (p.logit_softcap > (DT == HIPATTN_F32 ? 0.f : kShortCap)) return launch_heads<DT, F8, DP, true>(p, stream, bytes);
   return launch_heads<DT, F8, DP, false>(p, stream, bytes);
 }
 template <int DT, bool F8>
