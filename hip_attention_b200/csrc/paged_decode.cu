@@ -116,9 +116,11 @@ constexpr float kShortCap = 64.f;
 struct Logit {
   float k, cap;      // cap 0: none, else log2 e cap.  k = log2 e scale, short form 2 log2 e scale / cap.  k is positive: queries are multiplied by `sign` before
   __device__ __forceinline__ Logit(const Params& p, float scale, bool is_short) {
-    const float size = scale == 0.f ? 1.f : fabsf(scale);
+    // (never zero nor infinite: the zero of a scale of zero, which the queries carry, and of an empty product has to stay one.  A tiny scale over a
+    // head's power of two may come out as zero.)
+    const float size = fmaxf(fabsf(scale), FLT_TRUE_MIN);
     cap = fminf(p.logit_softcap * kLog2e, FLT_MAX);
-    k = kLog2e * size;
+    k = fminf(kLog2e * size, FLT_MAX);
     if (p.logit_softcap > 0.f && is_short) k = fminf(2.f * kLog2e * size / p.logit_softcap, FLT_MAX);
   }
   __device__ __forceinline__ float capped_short(float x) const {

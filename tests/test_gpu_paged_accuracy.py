@@ -200,3 +200,24 @@ def test_logits_whose_neighbours_are_far_apart(dtype, fp8, size, sign, G, width)
     assert bool((err <= tol).all()), f"off by {(err / tol).max().item():.3g} of the bound"
     want_lse = q[0, :, 0].double() * k.to(ct).double()[top, 0, 0][0] / math.log(2) + math.log2(vt.shape[0])
     assert bool(((lse[0].double() - want_lse).abs() <= want_lse.abs() * 2.0 ** -21).all())
+
+
+@pytest.mark.parametrize("cap", [None, 30.0, 1000.0])
+@pytest.mark.parametrize("scale,query", [(1e-9, 2.0 ** -126), (1e-30, 2.0 ** -100), (1.4e-45, 1.0), (-1e-9, 2.0 ** -126), (3.4e38, 0.0), (0.0, 1.0)])
+@pytest.mark.parametrize("dtype,fp8", [("bf16", True), ("fp16", True), ("bf16", False), ("fp32", False)])
+def test_scales_at_the_ends_of_their_range(dtype, fp8, scale, query, cap):
+    """Logits that are zero, or nothing beside 1, give the mean of the values."""
+    from hip_attention_b200 import paged_decode_attention
+    n, D = 500, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ct = FP8 if fp8 else DT[dtype]
+    k, v = (torch.randn((n, 1, 1, D), generator=g, device="cuda").to(ct) for _ in range(2))
+    q = torch.full((1, 8, D), query, device="cuda").to(DT[dtype])
+    q[0, 1] *= -1
+    out, lse = paged_decode_attention(q, k, v, torch.arange(n, device="cuda")[None], torch.tensor([n], device="cuda"), sm_scale=scale, logit_softcap=cap, return_lse=True)
+    want, size = v.double().mean(0)[0], v.double().abs().mean(0)[0]
+    # weights are equal; the log-sum-exp: with the shift of half-precision weights, 14 + log2 500 < 23, one ulp; caps up to 64 in 16 bits: 2^-20 of the cap
+    short = 2.0 ** -20 * cap if cap and cap <= 64 and dtype != "fp32" else 0.0
+    tol = size * (100 * U + (2.0 ** -16 if dtype == "bf16" and not fp8 else 2.0 ** -22) + 2.0 ** -20 + 2 * short) + torch.finfo(q.dtype).eps / 2 * want.abs()
+    assert bool(((out[0].double() - want).abs() <= tol).all())
+    assert bool(((lse.double() - math.log2(n)).abs() <= 2.0 ** -18 + 1.5 * short).all())
