@@ -1309,6 +1309,10 @@ void need_index(const at::Tensor& t, int64_t dim, const char* what) {
   if (!t.defined() || t.dim() != dim || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || (dim == 1 && !t.is_contiguous()))
     VALUE_ERROR("%s must be a contiguous int32 or int64 tensor of %d dimension%s", what, (int)dim, dim == 1 ? "" : "s");
 }
+// sizes that the C interface takes as int32
+void need_int32(int64_t n, const char* what) {
+  if (n > 0x7fffffff) VALUE_ERROR("%s: %lld are more than 2^31 - 1", what, (long long)n);
+}
 // the pair of pools [n_pages, page_size, kv_heads, head_dim] that a call reads or writes
 void kv_pools(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table, const at::Tensor& lens, at::ScalarType elem, hipattn_tokens_t* tk,
               hipattn_tokens_t* tv) {
@@ -1316,6 +1320,12 @@ void kv_pools(const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
   if (!k.is_cuda()) VALUE_ERROR("k_cache must be a CUDA tensor: there is no CPU path");
   need_index(table, 2, "block_table");
   need_index(lens, 1, "cache_seq_lens");
+  if (k.dim() == 4) {
+    need_int32(k.size(0), "pages of k_cache");
+    need_int32(k.size(1), "tokens of a page");
+  }
+  need_int32(table.size(0), "rows of block_table");
+  need_int32(table.size(1), "columns of block_table");
   *tk = tokens(at::Tensor(), k, table, lens, "k");
   *tv = tokens(at::Tensor(), v, table, lens, "v");
   if (k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type())
@@ -1345,6 +1355,7 @@ PyObject* paged_decode(PyObject* const* argv) {
   on_device(q, dev, "q");
   if (q.stride(2) != 1) VALUE_ERROR("q must have a contiguous last dim");
   const int64_t B = q.size(0), H = q.size(1), D = q.size(2), HKV = k.size(2);
+  need_int32(B, "tokens of q");
   if (k.size(3) != D) VALUE_ERROR("q %s and the caches %s differ in head_dim", shape_text(q).c_str(), shape_text(k).c_str());
   if (HKV < 1 || H % HKV) VALUE_ERROR("%lld heads are not a multiple of %lld KV heads", (long long)H, (long long)HKV);
   if (rows.defined()) {
@@ -1436,6 +1447,7 @@ PyObject* write_kv(PyObject* const* argv) {
     on_device(rows, dev, "rows");
     B = rows.size(0);
   }
+  need_int32(B, "entries of rows");
   if (offsets.defined()) {
     need_index(offsets, 1, "token_offsets");
     on_device(offsets, dev, "token_offsets");
@@ -1508,6 +1520,8 @@ PyObject* page_pool(PyObject* const* argv) {
     if (c.sizes() != first.sizes() || c.scalar_type() != first.scalar_type() || c.strides() != first.strides() || c.device() != first.device())
       VALUE_ERROR("the caches of a pool must have one shape, type, layout and device");
     if (dtype_of(c.scalar_type()) < 0 && !is_fp8(c.scalar_type())) VALUE_ERROR("caches must be float32, float16, bfloat16 or float8_e5m2 (or its uint8 view)");
+    if (c.size(0) > 0x7fff0000) VALUE_ERROR("a pool has at most %d pages, %lld were given", 0x7fff0000, (long long)c.size(0));
+    need_int32(c.size(1), "tokens of a page");
     if (c.numel() == 0) VALUE_ERROR("caches %s have no elements", shape_text(c).c_str());
     if (c.stride(3) != 1 || (c.size(2) > 1 && c.stride(2) != c.size(3)) || (c.size(1) > 1 && c.stride(1) != c.size(2) * c.size(3)))
       VALUE_ERROR("the tokens of a page must be contiguous (the pages may lie anywhere)");

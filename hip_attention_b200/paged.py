@@ -85,6 +85,8 @@ class HiPPagePool:
         if not first.is_cuda:
             raise ValueError("the caches must be CUDA tensors: there is no CPU path")
         n_pages, self.page_size = first.shape[:2]
+        if n_pages > 0x7fff0000:
+            raise ValueError(f"a pool has at most {0x7fff0000} pages, {n_pages} were given")
         self.k_caches, self.v_caches = k_caches, v_caches
         self.state = torch.zeros(n_pages + max_sequences + max_sequences * max_pages_per_sequence, dtype=torch.int32, device=first.device)
         self.ref_counts = self.state[:n_pages]

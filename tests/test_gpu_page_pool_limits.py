@@ -150,3 +150,22 @@ def test_a_pool_dropped_while_its_calls_run_on_another_stream():
     assert not any(bool(x.any()) for x in others) and read_status("cuda") == 0
     for c, c0 in ((k, k0), (v, v0)):
         assert torch.equal(c[1:8], c0[8:15]) and torch.equal(c[0, :3], c0[14, :3]) and torch.equal(c[0, 3], c0[0, 3]) and torch.equal(c[8:], c0[8:])
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Sizes whose lower 32 bits alone would look ordinary (expanded tensors: nothing of that size is there)."""
+    from hip_attention_b200 import HiPPagePool, paged_decode_attention, write_paged_kv
+    big = 2 ** 32 + 4
+    c = torch.zeros((4, 4, 2, 64), dtype=torch.bfloat16, device="cuda")
+    pages, tokens = c[:1].expand(big, 4, 2, 64), c[:, :1].expand(4, big, 2, 64)
+    q, table, lens = torch.zeros((1, 4, 64), dtype=torch.bfloat16, device="cuda"), ints([[0, 1]]), ints([3])
+    k = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device="cuda")
+    many = q.expand(big, 4, 64)
+    for bad in (lambda: paged_decode_attention(q, pages, pages, table, lens), lambda: paged_decode_attention(q, tokens, tokens, table, lens),
+                lambda: paged_decode_attention(many, c, c, table, lens), lambda: write_paged_kv(k, k, pages, pages, table, lens),
+                lambda: write_paged_kv(k, k, tokens, tokens, table, lens), lambda: paged_decode_attention(q, c, c, table.expand(big, 2), lens),
+                lambda: HiPPagePool([tokens], [tokens], 2, 2)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            bad()
+    with pytest.raises(ValueError, match="at most"):
+        HiPPagePool([pages], [pages], 2, 2)
