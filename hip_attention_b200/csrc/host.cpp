@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -1309,6 +1310,10 @@ void need_index(const at::Tensor& t, int64_t dim, const char* what) {
   if (!t.defined() || t.dim() != dim || (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) || (dim == 1 && !t.is_contiguous()))
     VALUE_ERROR("%s must be a contiguous int32 or int64 tensor of %d dimension%s", what, (int)dim, dim == 1 ? "" : "s");
 }
+// a tensor that a call writes: an expanded one has several elements in one place
+void need_own_elements(const at::Tensor& t, const char* what) {
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes) VALUE_ERROR("%s is expanded: its elements share memory", what);
+}
 // sizes that the C interface takes as int32
 void need_int32(int64_t n, const char* what) {
   if (n > 0x7fffffff) VALUE_ERROR("%s: %lld are more than 2^31 - 1", what, (long long)n);
@@ -1387,6 +1392,7 @@ PyObject* paged_decode(PyObject* const* argv) {
     on_device(out, dev, "out");
     if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || out.stride(2) != 1)
       VALUE_ERROR("out must be %s of q's type with a contiguous last dim", shape_text(q).c_str());
+    need_own_elements(out, "out");
   } else {
     out = mem.empty(q.sizes(), q.scalar_type());
   }
@@ -1435,6 +1441,8 @@ PyObject* write_kv(PyObject* const* argv) {
   hipattn_write_kv_params_t p;
   memset(&p, 0, sizeof(p));
   kv_pools(kc, vc, table, lens, k.scalar_type(), &p.k_pool, &p.v_pool);
+  need_own_elements(kc, "k_cache");
+  need_own_elements(vc, "v_cache");
   const c10::Device dev = kc.device();
   on_device(k, dev, "k");
   on_device(v, dev, "v");

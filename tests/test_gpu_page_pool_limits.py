@@ -169,3 +169,19 @@ def test_sizes_beyond_32_bits_are_refused():
             bad()
     with pytest.raises(ValueError, match="at most"):
         HiPPagePool([pages], [pages], 2, 2)
+
+
+def test_expanded_tensors_are_not_written_to():
+    """They may be read: a cache of one page seen as many."""
+    from hip_attention_b200 import paged_decode_attention, write_paged_kv
+    c = torch.randn((4, 4, 2, 64), device="cuda").to(torch.bfloat16)
+    q, table, lens = torch.ones((2, 4, 64), dtype=torch.bfloat16, device="cuda"), ints([[0, 1], [2, 3]]), ints([3, 8])
+    k = torch.zeros((2, 2, 64), dtype=torch.bfloat16, device="cuda")
+    same = c[:1].expand(4, 4, 2, 64)
+    for bad in (lambda: paged_decode_attention(q, c, c, table, lens, out=q[:1].expand(2, 4, 64)), lambda: write_paged_kv(k, k, same, c, table, lens),
+                lambda: write_paged_kv(k, k, c, c[:, :, :1].expand(4, 4, 2, 64), table, lens)):
+        with pytest.raises(ValueError, match="share memory"):
+            bad()
+    got = paged_decode_attention(q, same, same, table, lens)
+    assert torch.equal(got, paged_decode_attention(q, same.contiguous(), same.contiguous(), table, lens))
+    assert torch.equal(got, paged_decode_attention(q, c, c, torch.zeros_like(table), lens))
