@@ -3,8 +3,10 @@
 
 namespace hipattn {
 
-// A launch that may be prepared while the kernel before it on the stream is still running, and a kernel so launched: in_turn() is its first
-// statement, waits for all of that kernel (and so for everything before it), and lets the launch behind this one be prepared.
+// A launch that may be prepared while the kernel before it on the stream is still running, and a kernel so launched: in_turn() stands before all that it
+// reads and writes, waits for all of that kernel (and so for everything before it), and lets the launch behind this one be prepared.
+// One exception: paged_decode_merge_kernel reads rows and lengths before it.  The launch before is always the kernel whose parts it joins, which has
+// waited itself before it let this one be prepared, so that all before it is over, and which writes neither.
 // Such a kernel may have begun before what it reads was written, so it reads nothing by way of the read-only cache (no __ldg).
 // Back to back on a stream: a few requests' pages freed and dealt out 10.2 us, 6.7 so.
 struct InTurn {

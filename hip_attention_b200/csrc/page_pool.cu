@@ -10,8 +10,8 @@ namespace hipattn {
 namespace {
 
 constexpr int kSMs = 148;
-constexpr int kPlanCtas = 8;           // of a cluster; one CTA plans for pools of up to kSmallPool pages
-constexpr int kSmallPool = 8192;
+constexpr int kPlanCtas = 8;           // of a cluster; one CTA plans for pools of up to kSmallPool pages (a few sequences freed and dealt out of 4096
+constexpr int kSmallPool = 8192;       // pages: 7.1 us, 8.6 by a cluster; of 8192 7.7 and 8.6; of 16000 8.5 and 7.7, of 30000 11.0 and 7.7)
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kMaxCachesPerLaunch = 128;
@@ -679,6 +679,7 @@ extern "C" int hipattn_pool_free(const hipattn_page_pool_t* p, const int32_t* ro
   if (rc) return rc;
   HIPATTN_REQUIRE(n > 0 && n <= HIPATTN_POOL_MAX_ENTRIES, HIPATTN_ERR_INVALID, "pool_free: %d entries outside [1, %d]", n, HIPATTN_POOL_MAX_ENTRIES);
   HIPATTN_REQUIRE(rows != nullptr, HIPATTN_ERR_INVALID, "pool_free: null pointer");
+  // rows of 512 pages: 3.0 us with a CTA each, 3.7 with a cluster; of 1024 3.4 and 3.6; of 2048 4.2 and 3.8; of 8192 8.7 and 4.3
   const int ctas = p->table_width > 1024 ? 8 : 1;
   InTurn launch((int64_t)n * ctas, 256, 0, (cudaStream_t)stream, ctas);
   HIPATTN_CUDA_OK(cudaLaunchKernelEx(&launch.cfg, free_rows_kernel, device_pool(*p), rows, ctas));

@@ -11,7 +11,8 @@
 // rows; paged_decode_fma_kernel: fp32.
 //
 // Measured: one sequence of 1048571 tokens, bf16, 8 KV heads of dimension 128 (4.3 GB) 620 us, 6.9 TB/s; 32 sequences of up to 16384
-// tokens (1.18 GB) 180 us, 6.5 TB/s; 12 fp8 sequences in pages of one token, soft-capped (0.56 GB) 111 us, 5.0 TB/s; one sequence of 389 tokens 5.0 us.
+// tokens (1.18 GB) 180 us, 6.5 TB/s; 12 fp8 sequences in pages of one token, soft-capped (0.56 GB) 109 to 115 us by box, 4.9 to 5.1 TB/s; one
+// fp16 sequence of 389 tokens, 16 heads over 4 of dimension 64, 5.1 to 5.4 us.
 #include <cfloat>
 #include <type_traits>
 
@@ -1089,17 +1090,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_decode_merge_kernel(co
   }
 }
 
-// The layout's bounds, in rounds.  A cluster whose CTAs have more than sixteen each gains less from its missing second launch (3 to 4 us)
-// than it loses where lengths differ.  Units to a CTA each: 32 sequences of up to 800 tokens (13 rounds) 16 us, in shares 19; 64 of 600 tokens 32
-// and 37; 64 of 2000 (32 rounds) 87 and 90, of up to 2000 60 and 55; 40 of 3000 (47 rounds) 107 and 84.
-constexpr int kLeastRounds = 2;       // rounds of a share
+// The layout's bounds, in rounds.  Measured in bf16 with 32 heads over 8, D 128 (rounds of 64 keys), device times in us.
+//
+// A share has two rounds at least (one round instead: a sequence of 389 tokens behind a wide table 12.0 -> 9.3, one of 100 7.3 -> 9.0, one of 1000
+// 10.2 -> 11.4, the rest the same).
+constexpr int kLeastRounds = 2;
 // Beginning and ending a unit takes as long as some four rounds (2.5 us); without them in the shares' sizes a CTA that got a dozen short or
-// empty sequences ended last by far (64 sequences of up to 1000 tokens behind a wide table: 50 us, 34 so).  Few units are cut as small as they may be.
+// empty sequences ended last by far (64 sequences of up to 1000 tokens behind a wide table: 45 without, 34 so; 12 of up to 8000 44.8 and 43.8).  Few units
+// are cut as small as they may be (4 sequences of 2000 behind a wide table: 14.1 so, 15.4 with beginnings counted; 4 of up to 20000 43.1 and 41.7).
 constexpr int kUnitRounds = 4;
 constexpr int kManyUnits = 64;
-constexpr int kMaxCluster = 16;       // CTAs of a cluster (beyond eight: allowed per kernel)
-constexpr int kClusterRounds = 16;    // most rounds of a CTA of a cluster
-constexpr int kWholeRounds = 24;      // most rounds of a unit that is a CTA's
+// CTAs of a cluster (beyond eight: allowed per kernel).  With eight at most: one sequence of 8000 16.6, 13.9 so; of 1000 6.7, 7.1 so.
+constexpr int kMaxCluster = 16;
+// Rounds of a CTA of a cluster.  Longer units gain less from the second launch that a cluster does without than they lose where lengths differ (one
+// sequence of 30000, no others beside it: 35.2 in shares, 33.4 with up to 32 rounds); with up to eight, 4 of 5000 21.5, 16.3 so.
+constexpr int kClusterRounds = 16;
+// Rounds of a unit that is a CTA's.  With up to 64: 40 sequences of 3000 (47 rounds) 106, in shares 83, of up to 3000 59 and 53; 64 of 2000 (32 rounds) 85 and 91,
+// of up to 2000 58 and 55.  With up to 12: 32 of 800 (13 rounds) 18.8 so, 24 in shares, of up to 800 16.4 and 19.9; 20 of up to 1500 25.6 and 19.6.
+constexpr int kWholeRounds = 24;
 
 int padded_dim(int D) { return D <= 64 ? 64 : (D <= 128 ? 128 : 256); }
 

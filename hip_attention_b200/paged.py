@@ -35,8 +35,8 @@ def paged_decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_ta
     before they are written.
 
     How the work is laid out follows from the width of ``block_table``, which is all the host knows of the lengths: give the
-    columns that the longest sequence can need (``block_table[:, :w]``; one sequence of 389 tokens takes 7 us behind a table of 400 and 12 us
-    behind one of 131072).
+    columns that the longest sequence can need (``block_table[:, :w]``; one bfloat16 sequence of 389 tokens, 32 heads over 8 of
+    dimension 128, takes 6.7 us behind a table of 448 tokens and 12 us behind one of 131072).
 
     Returns the context [B, H, D] (in ``out`` when given) and, with ``return_lse``, the base-2 log-sum-exp [B, H] (float32).
     A sequence without tokens gives zeros and -inf."""
