@@ -68,9 +68,9 @@ class HiPPagePool:
     * ``block_table`` [max_sequences, max_pages_per_sequence]: its pages; entries behind them mean nothing.
 
     A page that several sequences read is full and is not written again.  Pages are dealt out lowest number first, in the
-    order of a call's entries.  A call that cannot be carried out as a whole (too few free pages, a sequence outside the
-    table, named twice, not empty or too long) changes nothing and leaves its bit in the status word.  Entries that are negative
-    are left out, so a captured call can be replayed with fewer of them; a call takes up to 4096.  Calls on one pool, and calls
+    order of a call's entries.  An ``extend`` or ``fork`` that cannot be carried out as a whole (too few free pages, a sequence outside
+    the table, named twice, not empty or too long) changes nothing and leaves its bit in the status word; ``free`` takes every row
+    for itself.  Entries that are negative are left out, so a captured call can be replayed with fewer of them; a call takes up to 4096.  Calls on one pool, and calls
     that read its tables, have to be ordered: one stream, or events."""
 
     def __init__(self, k_caches: Sequence[Tensor], v_caches: Sequence[Tensor], max_sequences: int, max_pages_per_sequence: int) -> None:
@@ -109,7 +109,8 @@ class HiPPagePool:
         host().pool_fork(self._handle, parents, children)
 
     def free(self, rows: Tensor) -> None:
-        """The sequences become empty; pages that no other sequence reads are free again.  Naming a row twice frees it once."""
+        """The sequences become empty; pages that no other sequence reads are free again.  Naming a row twice frees it once; a
+        row beyond the table leaves its bit in the status word, the others are freed."""
         host().pool_free(self._handle, rows)
 
     def compact(self) -> Tensor:

@@ -35,7 +35,7 @@ extern "C" {
 #define HIPATTN_STATUS_CHUNK_SIZE 8u  /* a chunk was longer than the chunk size the scan was told; its tail was ignored */
 #define HIPATTN_STATUS_TIMEOUT 4u     /* a bounded on-chip wait ran out; the launch's output is invalid */
 #define HIPATTN_STATUS_NO_PAGES 16u   /* a page pool had too few free pages for a call, which changed nothing */
-#define HIPATTN_STATUS_SEQUENCE 32u   /* a call named a sequence that it cannot take (outside the table, twice, not empty, too long) */
+#define HIPATTN_STATUS_SEQUENCE 32u   /* a call named a sequence that it cannot take (outside the table; extend and fork: twice, not empty, too long) */
 
 #define HIPATTN_SCORE_INIT (-32000.0f) /* attention_extend.py:2040-2045 */
 #define HIPATTN_INDEX_PAD INT64_MAX    /* attention_extend.py:2913 */
@@ -363,8 +363,8 @@ int hipattn_write_kv(const hipattn_write_kv_params_t* p, void* stream);
 
 /*
  * The pages of a pool: which sequence reads which page, and how many do.  All state is on the device and every call is
- * stream-ordered; calls on one pool must be ordered by the caller.  A call that cannot be carried out as a whole changes nothing
- * and sets HIPATTN_STATUS_NO_PAGES or _SEQUENCE.  Pages are dealt out lowest number first, in the order of a call's entries, so a
+ * stream-ordered; calls on one pool must be ordered by the caller.  An extend or a fork that cannot be carried out as a whole changes
+ * nothing and sets HIPATTN_STATUS_NO_PAGES or _SEQUENCE; a free takes every row for itself.  Pages are dealt out lowest number first, in the order of a call's entries, so a
  * call's result does not depend on how it is scheduled.  Entries that are negative are left out.  At most
  * HIPATTN_POOL_MAX_ENTRIES entries a call.
  */
@@ -392,7 +392,8 @@ int hipattn_pool_extend(const hipattn_page_pool_t* pool, const int32_t* rows, co
 /* children[i], an empty sequence, becomes a copy of parents[i]: full pages are shared, the tokens of a begun page are copied to a
  * page of the child's own in all caches. */
 int hipattn_pool_fork(const hipattn_page_pool_t* pool, const int32_t* parents, const int32_t* children, int32_t n, void* stream);
-/* The sequences become empty; pages that no other sequence reads are free again.  A row named twice is freed once. */
+/* The sequences become empty; pages that no other sequence reads are free again.  A row named twice is freed once; a
+ * row beyond the table sets HIPATTN_STATUS_SEQUENCE, the others are freed. */
 int hipattn_pool_free(const hipattn_page_pool_t* pool, const int32_t* rows, int32_t n, void* stream);
 /* Moves the pages in use to the front: with m pages in use, those numbered m and more go, ascending, to the free ones below m,
  * in all caches, and the tables follow.  *pages_in_use (optional, device) receives m. */
