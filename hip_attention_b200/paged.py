@@ -4,12 +4,16 @@ sequence (``paged_decode_attention``) for the layers a server keeps dense.
 
 The pools, tables and lengths are the ones ``hip_attention_12`` takes (``args.k_cache / v_cache / block_table /
 cache_seq_lens``) and, with pages of one token, ``forward_paged_hip`` (``req_to_tokens``).  The reference leaves these to the
-inference server around it; its configuration only says which layers and steps are dense (``hip_config.py:97-102``).
+inference server around it; its configuration has switches for a server that decodes densely (``hip_config.py:97-102``).
+
+The exact attention uses keys as they lie in the pool, so they are rotated before they are written.  With ``using_extend``, the
+configuration's default, the sparse attention rotates keys itself and its pools hold them un-rotated: a layer is then exact in all of its
+steps, with a pool of rotated keys, or sparse in all of them.  Without ``using_extend`` both read one pool.
 
 Every call is stream-ordered on the current stream of the caches' device, synchronises nothing and can be captured into a
-CUDA graph.  They are calls of a server: no gradient passes through them.  What the device finds wrong is recorded in the status word (``read_status``): HIPATTN_STATUS_NO_PAGES (16), a
-pool had too few free pages; HIPATTN_STATUS_SEQUENCE (32), a call named a sequence it cannot take; pages and positions out
-of range as in the rest of the package.
+CUDA graph.  They are calls of a server: no gradient passes through them.  What the device finds wrong is recorded in the status word
+(``read_status``): HIPATTN_STATUS_NO_PAGES (16), a pool had too few free pages; HIPATTN_STATUS_SEQUENCE (32), a call named a sequence
+it cannot take; pages and positions out of range as in the rest of the package.
 """
 from __future__ import annotations
 
@@ -70,8 +74,8 @@ class HiPPagePool:
     A page that several sequences read is full and is not written again.  Pages are dealt out lowest number first, in the
     order of a call's entries.  An ``extend`` or ``fork`` that cannot be carried out as a whole (too few free pages, a sequence outside
     the table, named twice, not empty or too long) changes nothing and leaves its bit in the status word; ``free`` takes every row
-    for itself.  Entries that are negative are left out, so a captured call can be replayed with fewer of them; a call takes up to 4096.  Calls on one pool, and calls
-    that read its tables, have to be ordered: one stream, or events."""
+    for itself.  Entries that are negative are left out, so a captured call can be replayed with fewer of them; a call takes up to
+    4096.  Calls on one pool, and calls that read its tables, have to be ordered: one stream, or events."""
 
     def __init__(self, k_caches: Sequence[Tensor], v_caches: Sequence[Tensor], max_sequences: int, max_pages_per_sequence: int) -> None:
         k_caches, v_caches = list(k_caches), list(v_caches)

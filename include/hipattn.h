@@ -309,8 +309,9 @@ int hipattn_merge_partials(const float* part_o, const float* part_lse, int64_t r
 int hipattn_bsa_decode_noalloc(const hipattn_bsa_params_t* p, void* stream);
 
 /*
- * Exact attention of one new token per sequence over a page pool, for layers that are not sparse.
- * The reference hands such layers to another attention backend (hip_config.py:97-102: decode_always_dense, force_dense).
+ * Exact attention of one new token per sequence over a page pool, for layers that are not sparse (hip_config.py:97-102 has the switches of a
+ * server that decodes densely: decode_always_dense, force_dense).  Keys are used as they lie in the pool: a pool of un-rotated keys,
+ * which the kernels above rotate themselves (rope_mode), is not one for it.
  *
  * Entry b attends positions [max(0, n - window), n) of sequence r = rows[b] (b when rows is null), n = cache_seq_lens[r],
  * read through block_table[r]; logits are sm_scale * q.k, soft-capped when logit_softcap > 0.  out [B, H, D] in the element
