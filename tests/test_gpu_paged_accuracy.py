@@ -221,3 +221,40 @@ def test_scales_at_the_ends_of_their_range(dtype, fp8, scale, query, cap):
     tol = size * (100 * U + (2.0 ** -16 if dtype == "bf16" and not fp8 else 2.0 ** -22) + 2.0 ** -20 + 2 * short) + torch.finfo(q.dtype).eps / 2 * want.abs()
     assert bool(((out[0].double() - want).abs() <= tol).all())
     assert bool(((lse.double() - math.log2(n)).abs() <= 2.0 ** -18 + 1.5 * short).all())
+
+
+@pytest.mark.parametrize("lens,width", [([300, 0, 2000, 64, 1, 777, 5000, 33] * 5, 4096), ([700, 0, 90, 1300], 96), ([40] * 200, 4)])
+@pytest.mark.parametrize("dtype,fp8,D,H,HKV", [("bf16", False, 128, 32, 2), ("fp16", False, 64, 24, 2), ("bf16", True, 128, 16, 1), ("bf16", False, 256, 16, 1), ("fp16", True, 96, 48, 2),
+                                               ("bf16", False, 128, 16, 2), ("fp32", False, 64, 16, 2)])
+def test_other_columns_heads_and_sequences_keep_their_bits(dtype, fp8, D, H, HKV, lens, width):
+    """Values that are not finite in some columns of one KV head, NaN keys in one sequence: all else comes out bit for bit as without them."""
+    from hip_attention_b200 import paged_decode_attention
+    page = 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    need = [-(-n // page) for n in lens]
+    n_pages = sum(need)
+    table = torch.zeros((len(lens), width * 16 // page), dtype=torch.int32, device="cuda")
+    order, at = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32), 0
+    for b, m in enumerate(need):
+        table[b, :m] = order[at:at + m]
+        at += m
+    kc, vc = (torch.randn((n_pages, page, HKV, D), generator=g, device="cuda") for _ in range(2))
+    ct = FP8 if fp8 else DT[dtype]
+    sl = torch.tensor(lens, device="cuda")
+    q = torch.randn((len(lens), H, D), generator=g, device="cuda").to(DT[dtype])
+    call = lambda: paged_decode_attention(q, kc.to(ct), vc.to(ct), table, sl, sm_scale=D ** -0.5, return_lse=True)   # noqa: E731
+    want, want_lse = call()
+    vc[torch.rand(n_pages, generator=g, device="cuda") < 0.3, 5, HKV - 1, 3] = float("inf")
+    vc[torch.rand(n_pages, generator=g, device="cuda") < 0.3, 9, HKV - 1, D - 1] = float("nan")
+    bad = next(b for b, n in enumerate(lens) if n >= 40)
+    kc[table[bad, 1].long(), 4, 0, 1] = float("nan")
+    got, lse = call()
+    G = H // HKV
+    ok = torch.ones(got.shape, dtype=torch.bool, device="cuda")
+    ok[:, (HKV - 1) * G:, 3] = ok[:, (HKV - 1) * G:, D - 1] = False
+    ok[bad, :G] = False
+    assert torch.equal(got[ok], want[ok]) and bool(torch.isnan(got[bad, :G]).all()) and bool(torch.isnan(lse[bad, :G]).all())
+    keep = torch.ones(lse.shape, dtype=torch.bool, device="cuda")
+    keep[bad, :G] = False
+    assert torch.equal(lse[keep], want_lse[keep])
+    assert not bool(torch.isnan(got[:, (HKV - 1) * G:, 3][keep[:, (HKV - 1) * G:]]).any())       # infinite or finite, no NaN
