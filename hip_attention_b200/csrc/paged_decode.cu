@@ -4,7 +4,7 @@
 // Work is a row of rounds: for every sequence, for every unit of it (a KV head and a tile of its query heads), ROUND keys at a
 // time.  The host does not know the lengths, so every CTA adds them up itself and takes its share of the row, as many rounds
 // as any other, whatever the lengths are.  A unit that lies in one CTA's share is finished there; the parts of one that does not go
-// to scratch (numerators, maximum, denominator) and the merge kernel joins them in order.
+// to scratch (numerators, the base of their weights, denominator) and the merge kernel joins them in order.
 //
 // A warp takes KEYS keys at a time from a ring of its own in shared memory, filled with 16-byte asynchronous copies, and keeps
 // its own running maximum, sum and output: nothing in the loop waits for another warp.  paged_decode_mma_kernel: 16-bit and fp8
@@ -144,7 +144,7 @@ struct Plan {
   int vector_out;                     // output rows begin where four elements can be stored at once
 };
 
-// Columns 4 v .. 4 v + 3 of the output row of head h, from the joined maximum (base 2), numerators and denominator
+// Columns 4 v .. 4 v + 3 of the output row of head h, from the joined base of the weights, numerators and denominator
 template <int DT>
 __device__ __forceinline__ void finish(const Params& p, const Plan& plan, int b, int h, int v, float M, const float4& num, float den) {
   using T = typename Elem<DT>::type;
